@@ -49,6 +49,8 @@ EXPORTED_SYMBOLS = [
     "argus_hip_quant_attn_cap_is_nosub_device", "argus_hip_quant_attn_cap_attention_gen_quant",
     "argus_hip_quant_attn_cap_gather_update_quant", "argus_hip_quant_attn_cap_dequant_flush",
     "argus_hip_quant_attn_cap_scatter_residual", "argus_hip_quant_attn_get_vtable",
+    "argus_hip_page_plan", "argus_hip_qk_norm_rope", "argus_hip_paged_attention",
+    "argus_hip_paged_attention_workspace",
 ]
 
 if not os.path.exists(LIB_PATH):
@@ -220,6 +222,35 @@ class ScoreReduceArgs(C.Structure):
                 ("max_seq_len", C.c_size_t), ("layer_flat_importance", C.c_uint64)]
 
 
+class PagePlanArgs(C.Structure):
+    _fields_ = [("stream", C.c_void_p), ("past_len", C.c_void_p), ("new_len", C.c_void_p), ("free_pages", C.c_void_p),
+                ("page_table", C.c_void_p), ("cu_new", C.c_void_p), ("kv_len", C.c_void_p), ("positions", C.c_void_p),
+                ("slots", C.c_void_p), ("counts", C.c_void_p),
+                ("n_seqs", C.c_int32), ("n_free", C.c_int32), ("n_pages", C.c_int32), ("page_size", C.c_int32),
+                ("table_stride", C.c_int32), ("token_capacity", C.c_int32)]
+
+
+class QkNormRopeArgs(C.Structure):
+    _fields_ = [("stream", C.c_void_p), ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_weight", C.c_void_p),
+                ("k_weight", C.c_void_p), ("cos_sin", C.c_void_p), ("positions", C.c_void_p), ("slots", C.c_void_p),
+                ("q_out", C.c_void_p), ("k_cache", C.c_void_p), ("v_cache", C.c_void_p),
+                ("q_stride", C.c_int64), ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("q_out_stride", C.c_int64),
+                ("tokens", C.c_int32), ("heads_q", C.c_int32), ("heads_kv", C.c_int32), ("head_dim", C.c_int32),
+                ("rot_dim", C.c_int32), ("interleaved", C.c_int32), ("n_positions", C.c_int32), ("n_pages", C.c_int32),
+                ("page_size", C.c_int32), ("layout", C.c_int32), ("in_dtype", C.c_int32), ("out_dtype", C.c_int32),
+                ("eps", C.c_float), ("weight_bias", C.c_float)]
+
+
+class PagedAttentionArgs(C.Structure):
+    _fields_ = [("stream", C.c_void_p), ("q", C.c_void_p), ("k_cache", C.c_void_p), ("v_cache", C.c_void_p),
+                ("page_table", C.c_void_p), ("cu_new", C.c_void_p), ("kv_len", C.c_void_p), ("out", C.c_void_p),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t), ("q_stride", C.c_int64), ("out_stride", C.c_int64),
+                ("n_seqs", C.c_int32), ("n_tokens", C.c_int32), ("heads_q", C.c_int32), ("heads_kv", C.c_int32),
+                ("head_dim", C.c_int32), ("n_pages", C.c_int32), ("page_size", C.c_int32), ("table_stride", C.c_int32),
+                ("layout", C.c_int32), ("dtype", C.c_int32), ("min_new", C.c_int32), ("max_new", C.c_int32),
+                ("max_kv", C.c_int32), ("window", C.c_int32), ("softcap", C.c_float), ("scale", C.c_float)]
+
+
 def _bind():
     vp, i32 = C.c_void_p, C.c_int32
     lib.argus_hip_create.argtypes = [C.c_int, C.POINTER(vp)]
@@ -265,6 +296,10 @@ def _bind():
     lib.argus_hip_kv_scatter_f32_to_f16_batch.argtypes = sc16 + [i32]
     lib.argus_hip_kv_scatter_f32_batch.argtypes = sc16 + [i32]
     lib.argus_hip_quant_requant.argtypes = [vp, C.POINTER(QuantRequantArgs)]
+    lib.argus_hip_page_plan.argtypes = [vp, C.POINTER(PagePlanArgs)]
+    lib.argus_hip_qk_norm_rope.argtypes = [vp, C.POINTER(QkNormRopeArgs)]
+    lib.argus_hip_paged_attention.argtypes = [vp, C.POINTER(PagedAttentionArgs)]
+    lib.argus_hip_paged_attention_workspace.argtypes = [vp, C.POINTER(PagedAttentionArgs)]
     lib.argus_hip_quant_cache_make.argtypes = [C.POINTER(QuantCacheMakeArgs)]
     for name in ("current_pos", "capacity", "current_bits", "flush_if_full", "drop"):
         getattr(lib, "argus_hip_quant_cache_" + name).argtypes = [vp]
@@ -276,6 +311,7 @@ def _bind():
     for name in EXPORTED_SYMBOLS:
         if name != "argus_hip_last_error":
             getattr(lib, name).restype = C.c_int
+    lib.argus_hip_paged_attention_workspace.restype = C.c_int64
     lib.argus_hip_quant_attn_cap_make.argtypes = [C.POINTER(QuantAttnMakeArgs)]
     lib.argus_hip_quant_attn_cap_make.restype = vp
     lib.argus_hip_quant_attn_cap_drop.argtypes = [vp]
@@ -361,9 +397,9 @@ def _ptr(t):
     return 0 if t is None else t.data_ptr()
 
 
-def _stream():
+def _stream(device=None):
     import torch
-    return torch.cuda.current_stream().cuda_stream
+    return torch.cuda.current_stream(device).cuda_stream
 
 
 def _kv_dtype(t):
@@ -373,6 +409,41 @@ def _kv_dtype(t):
     if t.dtype == torch.float32:
         return F32
     raise TypeError("unsupported KV dtype %s" % t.dtype)
+
+
+def _int32(what, *tensors):
+    """Tables and lengths cross the ABI as packed device int32."""
+    import torch
+    for t in tensors:
+        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
+            raise TypeError(what + ": lengths, tables, positions and slots are contiguous int32 tensors")
+
+
+def _on_device(what, device, *tensors):
+    """A pointer to other memory would reach the kernels unchecked."""
+    for t in tensors:
+        if t is not None and (not t.is_cuda or t.device.index != device):
+            raise ValueError("%s: every tensor lies on the context's device (cuda:%d)" % (what, device))
+
+
+def _token_stride(t):
+    """Elements between the tokens of [tokens, heads, d], whose heads are packed."""
+    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
+        raise ValueError("the heads of a token must be packed")
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
+
+
+def _pool(what, k, v, layout, hkv, d):
+    """(n_pages, page_size) of a pair of page pools."""
+    import torch
+    if k.dtype != torch.float16 or v.dtype != torch.float16:
+        raise TypeError(what + ": page pools are float16")
+    if k.dim() != 4 or k.shape != v.shape or not k.is_contiguous() or not v.is_contiguous():
+        raise ValueError(what + ": page pools are contiguous tensors of one shape")
+    n, heads, size = (k.shape[0], k.shape[1], k.shape[2]) if layout == HEAD_MAJOR else (k.shape[0], k.shape[2], k.shape[1])
+    if heads != hkv or k.shape[3] != d:
+        raise ValueError(what + ": the pools belong to other heads")
+    return n, size
 
 
 class Context:
@@ -389,6 +460,7 @@ class Context:
         if rc != OK:
             raise ArgusHipError(rc, "argus_hip_create failed (no HIP device?)")
         self.handle = h
+        self.device = device
 
     def close(self):
         if self.handle:
@@ -632,3 +704,88 @@ class Context:
         else:
             rc = lib.argus_hip_kv_scatter_f32_to_f16_batch(*args, seq_len)
         return self._check(rc, check)
+
+    # -- paged caches ----------------------------------------------------------------------
+    def page_plan(self, past_len, new_len, free_pages, page_table, page_size, n_pages, cu_new, kv_len, positions, slots, counts,
+                  check=True):
+        """Device int32 tensors: past_len, new_len, kv_len [n], free_pages [f], page_table [n, c] (in place), cu_new [n + 1],
+        positions and slots [token_capacity], counts [3]."""
+        _int32("page_plan", past_len, new_len, free_pages, page_table, cu_new, kv_len, positions, slots, counts)
+        _on_device("page_plan", self.device, past_len, new_len, free_pages, page_table, cu_new, kv_len, positions, slots, counts)
+        n = past_len.numel()
+        if (new_len.numel() != n or kv_len.numel() != n or cu_new.numel() != n + 1 or counts.numel() != 3 or page_table.dim() != 2
+                or page_table.shape[0] != n or slots.numel() != positions.numel()):
+            raise ValueError("page_plan: shapes do not belong together")
+        a = PagePlanArgs(stream=_stream(self.device), past_len=_ptr(past_len), new_len=_ptr(new_len), free_pages=_ptr(free_pages),
+                         page_table=_ptr(page_table), cu_new=_ptr(cu_new), kv_len=_ptr(kv_len), positions=_ptr(positions),
+                         slots=_ptr(slots), counts=_ptr(counts), n_seqs=n,
+                         n_free=0 if free_pages is None else free_pages.numel(), n_pages=n_pages, page_size=page_size,
+                         table_stride=page_table.shape[1], token_capacity=positions.numel())
+        return self._check(lib.argus_hip_page_plan(self.handle, C.byref(a)), check)
+
+    def qk_norm_rope(self, q, k, v, positions, cos_sin, q_out, k_cache, v_cache, slots, q_weight=None, k_weight=None, eps=1e-6,
+                     weight_bias=0.0, interleaved=False, layout=HEAD_MAJOR, check=True):
+        """q [t, Hq, d], k / v [t, Hkv, d] (heads packed, any token stride), q_out [t, Hq, d]; pools as in
+        argus_hip.h; cos_sin [n_positions, rot_dim] F32 or None (no rotation); positions, slots [t] int32."""
+        import torch
+        _int32("qk_norm_rope", positions, slots)
+        t, hq, d = q.shape
+        hkv = k.shape[1]
+        n_pages, page_size = _pool("qk_norm_rope", k_cache, v_cache, layout, hkv, d)
+        if (k.shape != (t, hkv, d) or v.shape != k.shape or q_out.shape != q.shape or slots.numel() != t
+                or (positions is not None and positions.numel() != t)):
+            raise ValueError("qk_norm_rope: shapes do not belong together")
+        if k.dtype != q.dtype or v.dtype != q.dtype:
+            raise TypeError("qk_norm_rope: q, k and v have one dtype")
+        for w in (q_weight, k_weight, cos_sin):
+            if w is not None and (w.dtype != torch.float32 or not w.is_contiguous()):
+                raise TypeError("qk_norm_rope: weights and cos_sin are contiguous float32")
+        for w in (q_weight, k_weight):
+            if w is not None and w.numel() != d:
+                raise ValueError("qk_norm_rope: a weight has head_dim elements")
+        if cos_sin is not None and (cos_sin.dim() != 2 or positions is None):
+            raise ValueError("qk_norm_rope: cos_sin is [n_positions, rot_dim] and needs positions")
+        _on_device("qk_norm_rope", self.device, q, k, v, positions, cos_sin, q_out, k_cache, v_cache, slots, q_weight, k_weight)
+        a = QkNormRopeArgs(stream=_stream(self.device), q=_ptr(q), k=_ptr(k), v=_ptr(v), q_weight=_ptr(q_weight), k_weight=_ptr(k_weight),
+                           cos_sin=_ptr(cos_sin), positions=_ptr(positions), slots=_ptr(slots), q_out=_ptr(q_out),
+                           k_cache=_ptr(k_cache), v_cache=_ptr(v_cache), q_stride=_token_stride(q), k_stride=_token_stride(k),
+                           v_stride=_token_stride(v), q_out_stride=_token_stride(q_out), tokens=t, heads_q=hq, heads_kv=hkv,
+                           head_dim=d, rot_dim=0 if cos_sin is None else cos_sin.shape[1], interleaved=int(interleaved),
+                           n_positions=0 if cos_sin is None else cos_sin.shape[0], n_pages=n_pages, page_size=page_size,
+                           layout=layout, in_dtype=_kv_dtype(q), out_dtype=_kv_dtype(q_out), eps=eps, weight_bias=weight_bias)
+        return self._check(lib.argus_hip_qk_norm_rope(self.handle, C.byref(a)), check)
+
+    def _paged_args(self, q, k_cache, v_cache, page_table, cu_new, kv_len, out, max_new, max_kv, min_new, softcap, scale, window,
+                    layout, workspace):
+        _int32("paged_attention", page_table, cu_new, kv_len)
+        t, hq, d = q.shape
+        hkv = k_cache.shape[1] if layout == HEAD_MAJOR else k_cache.shape[2]
+        n_pages, page_size = _pool("paged_attention", k_cache, v_cache, layout, hkv, d)
+        n = kv_len.numel()
+        if cu_new.numel() != n + 1 or page_table.dim() != 2 or page_table.shape[0] != n or out.shape != q.shape:
+            raise ValueError("paged_attention: shapes do not belong together")
+        if out.dtype != q.dtype:
+            raise TypeError("paged_attention: q and out have one dtype")
+        _on_device("paged_attention", self.device, q, k_cache, v_cache, page_table, cu_new, kv_len, out, workspace)
+        return PagedAttentionArgs(
+            stream=_stream(self.device), q=_ptr(q), k_cache=_ptr(k_cache), v_cache=_ptr(v_cache), page_table=_ptr(page_table),
+            cu_new=_ptr(cu_new), kv_len=_ptr(kv_len), out=_ptr(out), workspace=_ptr(workspace),
+            workspace_bytes=0 if workspace is None else workspace.numel() * workspace.element_size(), q_stride=_token_stride(q),
+            out_stride=_token_stride(out), n_seqs=n, n_tokens=t, heads_q=hq, heads_kv=hkv, head_dim=d, n_pages=n_pages,
+            page_size=page_size, table_stride=page_table.shape[1], layout=layout, dtype=_kv_dtype(q), min_new=min_new,
+            max_new=max_new, max_kv=max_kv, window=window, softcap=softcap, scale=scale)
+
+    def paged_attention(self, q, k_cache, v_cache, page_table, cu_new, kv_len, out, max_new=0, max_kv=0, min_new=0, softcap=0.0,
+                        scale=0.0, window=0, layout=HEAD_MAJOR, workspace=None, check=True):
+        """q / out [n_tokens, Hq, d] (heads packed, any token stride); pools, tables and hints as in argus_hip.h.
+        workspace: a device tensor of paged_attention_workspace() bytes (None: the context's)."""
+        a = self._paged_args(q, k_cache, v_cache, page_table, cu_new, kv_len, out, max_new, max_kv, min_new, softcap, scale, window,
+                             layout, workspace)
+        return self._check(lib.argus_hip_paged_attention(self.handle, C.byref(a)), check)
+
+    def paged_attention_workspace(self, q, k_cache, v_cache, page_table, cu_new, kv_len, out, max_new=0, max_kv=0, min_new=0,
+                                  softcap=0.0, scale=0.0, window=0, layout=HEAD_MAJOR, check=True):
+        """Bytes of workspace paged_attention needs for the same arguments."""
+        a = self._paged_args(q, k_cache, v_cache, page_table, cu_new, kv_len, out, max_new, max_kv, min_new, softcap, scale, window,
+                             layout, None)
+        return self._check(lib.argus_hip_paged_attention_workspace(self.handle, C.byref(a)), check)

@@ -641,6 +641,153 @@ int argus_hip_kv_scatter_f32_batch(argus_hip_ctx *ctx, void *stream, const float
                                    int32_t head_dim, int32_t capacity, int32_t write_pos_start,
                                    int32_t seq_len);
 
+/* ---- paged F16 caches: requests of different lengths in one call ------------------------------------
+ * No counterpart in the reference, whose caches hold one sequence each.  A paged cache is a pool of
+ * pages of `page_size` tokens, K and V each
+ *   ARGUS_HIP_HEAD_MAJOR  [n_pages, kv_heads, page_size, head_dim]
+ *   ARGUS_HIP_SEQ_MAJOR   [n_pages, page_size, kv_heads, head_dim]
+ * in F16; token t of request s lies in page page_table[s * table_stride + t / page_size], row
+ * t % page_size.  Lengths, page numbers and positions live on the device and are not read by the host,
+ * so a step can be captured into a graph and replayed with other requests; a page number outside
+ * [0, n_pages) never reaches memory outside the pool.
+ *   page_plan        once per step: prefix sums, page tables, positions and write slots from the lengths
+ *   qk_norm_rope     per layer: norm and rotation of the new queries and keys, K and V into their slots
+ *   paged_attention  per layer: the new tokens of every request over that request's pages
+ * page_size is a power of two from 16 to 1024; head_dim 64, 128 or 256; pools 16-byte aligned. */
+#define ARGUS_HIP_MAX_PAGE_SIZE 1024
+
+/* One step of a scheduler over n_seqs requests, request s bringing new_len[s] tokens (0: idle this
+ * step) behind past_len[s] cached ones.  Rows of page_table hold ceil(past_len / page_size) pages on
+ * entry; the pages the new tokens need are taken from the front of free_pages in request order and
+ * appended (-1 where the list is exhausted).  With need_s the pages of request s:
+ *   cu_new[s] = sum of new_len before s (cu_new[n_seqs] = total), kv_len[s] = past_len[s] + new_len[s];
+ *   token t = cu_new[s] + i: positions[t] = past_len[s] + i,
+ *     slots[t] = page * page_size + position % page_size, -1 for a token without a page;
+ *   rows [total, token_capacity) of positions and slots are set to -1 (padding of fixed-size batches);
+ *   counts = { total tokens, pages needed, requests that ran short of free pages or of table_stride }.
+ * Negative lengths count as 0, sums saturate at 2^31 - 1, tokens past token_capacity are left out (the
+ * caller sees counts[0] > token_capacity).  Everything is written in place and depends on the inputs
+ * alone: the same call again gives the same tables.  n_seqs at most 16384. */
+typedef struct argus_hip_page_plan_args {
+  void *stream;
+  const int32_t *past_len;   /* device [n_seqs] */
+  const int32_t *new_len;    /* device [n_seqs] */
+  const int32_t *free_pages; /* device [n_free]; NULL when n_free is 0 */
+  int32_t *page_table;       /* device [n_seqs, table_stride], in place */
+  int32_t *cu_new;           /* device [n_seqs + 1] */
+  int32_t *kv_len;           /* device [n_seqs] */
+  int32_t *positions;        /* device [token_capacity] */
+  int32_t *slots;            /* device [token_capacity] */
+  int32_t *counts;           /* device [3] */
+  int32_t n_seqs;
+  int32_t n_free;
+  int32_t n_pages;           /* pages of the pool; n_pages * page_size < 2^31 */
+  int32_t page_size;
+  int32_t table_stride;      /* pages per request at most */
+  int32_t token_capacity;
+} argus_hip_page_plan_args;
+int argus_hip_page_plan(argus_hip_ctx *ctx, const argus_hip_page_plan_args *args);
+
+/* The new tokens' queries and keys of one layer, and the cache write.  Per head x of q and k:
+ *   y = x * rsqrt(mean(x^2) + eps) * (weight + weight_bias)     (no norm where the weight is NULL)
+ *   rotation of the first rot_dim channels by row positions[t] of cos_sin = [cos(rot_dim/2) | sin(rot_dim/2)]:
+ *     pairs (i, i + rot_dim/2), or (2i, 2i + 1) with interleaved != 0:
+ *     (a, b) -> (a cos - b sin, b cos + a sin)
+ * in F32, rounded once.  q goes to q_out, k and v (v only converted) to row slots[t] of the pools.
+ * A token whose slot lies outside the pool leaves the pool alone (its q_out row is written); a token
+ * whose position lies outside [0, n_positions) is padding: nothing is written for it.  Two tokens with
+ * the same slot leave one of the two rows there.  q_out may be q itself (same type and stride).
+ * rot_dim is a multiple of 8, at most head_dim, or 0: no rotation, cos_sin and positions may be NULL
+ * (positions that are given mark padding by being negative).
+ * Row strides are in elements between tokens, multiples of 4, 0 = packed; rows are 16-byte (F32) or
+ * 8-byte (F16) aligned, so slices of one projection's output are read in place. */
+typedef struct argus_hip_qk_norm_rope_args {
+  void *stream;
+  const void *q;            /* [tokens, heads_q, head_dim] of in_dtype */
+  const void *k;            /* [tokens, heads_kv, head_dim] */
+  const void *v;
+  const float *q_weight;    /* [head_dim] F32 or NULL */
+  const float *k_weight;
+  const float *cos_sin;     /* [n_positions, rot_dim] F32 */
+  const int32_t *positions; /* device [tokens] */
+  const int32_t *slots;     /* device [tokens] */
+  void *q_out;              /* [tokens, heads_q, head_dim] of out_dtype */
+  void *k_cache;
+  void *v_cache;
+  int64_t q_stride;
+  int64_t k_stride;
+  int64_t v_stride;
+  int64_t q_out_stride;
+  int32_t tokens;
+  int32_t heads_q;
+  int32_t heads_kv;
+  int32_t head_dim;
+  int32_t rot_dim;
+  int32_t interleaved;
+  int32_t n_positions;
+  int32_t n_pages;
+  int32_t page_size;
+  int32_t layout;
+  int32_t in_dtype;         /* ARGUS_HIP_F32 / ARGUS_HIP_F16 */
+  int32_t out_dtype;
+  float eps;
+  float weight_bias;        /* added to the weights: 1 where they are stored as w - 1 */
+} argus_hip_qk_norm_rope_args;
+int argus_hip_qk_norm_rope(argus_hip_ctx *ctx, const argus_hip_qk_norm_rope_args *args);
+
+/* Causal GQA attention of the new tokens of every request over its pages, chunks and single tokens
+ * mixed.  Row cu_new[s] + i of q belongs to request s, stands at position p = kv_len[s] - new + i
+ * (new = cu_new[s+1] - cu_new[s]) and sees keys c <= p, and c > p - window with window > 0:
+ *   s_c = (q . k_c) * scale; softcap > 0: softcap * tanh(s_c / softcap); out = sum_c softmax(s)_c v_c
+ * Rows that see nothing, or whose logits are all -inf, give zeros; a NaN logit gives a NaN row; what
+ * a key the row does not see holds (NaN, infinities, rows of a page behind the last token) has no
+ * influence.  Rows of q / out behind cu_new[n_seqs] are neither read nor written.  The keys of a page
+ * number outside the pool, and those past table_stride pages, read as zeros: such a request's rows are
+ * finite and otherwise unspecified.
+ * dtype F16: logits and sums in F32, probabilities rounded to F16 for the second product; dtype F32: q and
+ * the probabilities as F16 pairs (hi + lo), so the result is that of F32 arithmetic.
+ * max_new / max_kv: no request brings more new tokens / holds more tokens than this (0 = not known).
+ * They choose kernels, and rows of a request that brings more than max_new may be left unwritten.
+ * min_new: no request with any new token brings fewer (0 = not known).
+ * The partial results of requests cut along their length need a workspace: the caller's
+ * (argus_hip_paged_attention_workspace bytes at least, 256-byte aligned, one per stream at a time), or
+ * with workspace NULL the context's, which grows with a device synchronisation -- a call under stream
+ * capture has to bring its own (ARGUS_HIP_ERR_INVALID otherwise). */
+typedef struct argus_hip_paged_attention_args {
+  void *stream;
+  const void *q;             /* [n_tokens, heads_q, head_dim] */
+  const void *k_cache;
+  const void *v_cache;
+  const int32_t *page_table; /* device [n_seqs, table_stride] */
+  const int32_t *cu_new;     /* device [n_seqs + 1] */
+  const int32_t *kv_len;     /* device [n_seqs] */
+  void *out;                 /* [n_tokens, heads_q, head_dim] */
+  void *workspace;
+  size_t workspace_bytes;
+  int64_t q_stride;          /* elements between tokens, 0 = packed */
+  int64_t out_stride;
+  int32_t n_seqs;
+  int32_t n_tokens;          /* rows of q and out */
+  int32_t heads_q;
+  int32_t heads_kv;
+  int32_t head_dim;
+  int32_t n_pages;
+  int32_t page_size;
+  int32_t table_stride;
+  int32_t layout;
+  int32_t dtype;             /* of q and out: ARGUS_HIP_F32 / ARGUS_HIP_F16 */
+  int32_t min_new;
+  int32_t max_new;
+  int32_t max_kv;
+  int32_t window;            /* 0 = none */
+  float softcap;             /* 0 = none */
+  float scale;               /* 0 selects 1/sqrt(head_dim) */
+} argus_hip_paged_attention_args;
+int argus_hip_paged_attention(argus_hip_ctx *ctx, const argus_hip_paged_attention_args *args);
+/* Bytes of workspace that suffice for `args` (pointers are not looked at) and for every call with the
+ * same shapes and hints; negative error code for arguments the call would refuse. */
+int64_t argus_hip_paged_attention_workspace(const argus_hip_ctx *ctx, const argus_hip_paged_attention_args *args);
+
 #ifdef __cplusplus
 }
 #endif
