@@ -1,93 +1,399 @@
 // Causal GQA attention of the new tokens of many requests over their pages (include/argus_hip.h,
-// argus_hip_paged_attention).
+// argus_hip_paged_attention): the chunk kernel, the merge of requests cut along their length, and the
+// entry point.  Requests of at most 16 rows (tokens x heads of a group) take the decode kernel of
+// paged_decode.hip.
 //
 //   s_c = cap((q . k_c) * scale) for the visible keys c of a row;  out = sum_c softmax(s)_c v_c
 //
-// One wave per (token, query head): 64 keys per step, one lane per key for the logits, one lane per
-// D / 64 channels for the weighted sum, running maximum and sum in F32.
+// Chunk kernel: one workgroup = 128 rows of one KV head, four waves of 32.  A row is a (token, head of the
+// group) pair, so the whole group shares each K / V tile and a short chunk fills its rows with heads.
+// v_mfma_f32_32x32x16_f16 in the transposed form
+//     S^T = K . Q^T  (A = K rows from LDS, B = Q rows in registers)
+//     O^T = V^T . P^T (A = V^T through a transposing LDS read, B = the S^T accumulators' own layout)
+// a lane owns one row: the softmax is in-lane plus one exchange between the wave's halves, the running
+// maximum and sum are F32, and P never goes through LDS.
 #include "paged_common.hpp"
 
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
+
+namespace argus_paged {
 
 namespace {
 
-struct PagedParams {
-  const void *q;
-  const _Float16 *k, *v;
-  const int32_t *page_table, *cu_new, *kv_len;
-  void *out;
-  int64_t q_stride, out_stride;
-  PoolStrides pool;
-  int32_t n_seqs, n_tokens, heads_q, heads_kv, group, n_pages, page_shift, table_stride, window;
-  float softcap, scale;
+typedef float float16_t __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ half4_t lds_read_tr16(const _Float16 *p) {
+  typedef short short4_t __attribute__((ext_vector_type(4)));
+  typedef __attribute__((address_space(3))) short4_t lds_short4_t;
+  return __builtin_bit_cast(half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t *)p));
+}
+
+template <int D>
+struct ChunkTile {
+  static constexpr int BN = chunk_align(D);            // keys per tile
+  static constexpr int KP = D + 8, VP = D + 32;        // row pitches (halfs): no bank is hit twice by one read
+  static constexpr int HALFS = BN * (KP + VP);
+  static constexpr int LDS_BYTES = 2 * HALFS * 2;      // two tile buffers
 };
 
-template <int D, typename T>
-__global__ __launch_bounds__(64) void paged_row_kernel(const PagedParams p) {
-  const int h = blockIdx.x % p.heads_q, token = blockIdx.x / p.heads_q, lane = threadIdx.x;
-  if (token >= p.cu_new[p.n_seqs]) return;
-  int lo = 0, hi = p.n_seqs;  // the request with cu_new[lo] <= token < cu_new[lo + 1]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.cu_new[mid] <= token) lo = mid;
-    else hi = mid;
-  }
-  const int len = min(max(p.kv_len[lo], 0), (int)min((int64_t)p.table_stride << p.page_shift, (int64_t)0x7fffffff));
-  const int pos = p.kv_len[lo] - (p.cu_new[lo + 1] - token);
-  const int end = min(pos + 1, len);
-  const int begin = p.window > 0 ? max(0, pos - p.window + 1) : 0;
+template <int D, typename T, bool CAP>
+__global__ __launch_bounds__(256, (D <= 128 && std::is_same<T, _Float16>::value) ? 2 : 1) void paged_chunk_kernel(const PagedParams p) {
+  using TL = ChunkTile<D>;
+  constexpr bool F32 = std::is_same<T, float>::value;
+  constexpr int BN = TL::BN, KP = TL::KP, VP = TL::VP;
+  constexpr int KK = D / 16, KB = BN / 32, RB = D / 32;
+  constexpr int CH = BN * D / 8 / 256;  // 16-byte pieces of a K (or V) tile per thread
+  constexpr int RPW = 64 / (D / 8);     // rows of a piece that one wave covers
+  constexpr float kLog2e = 1.4426950408889634f;
 
-  __shared__ float q_lds[D];
-  __shared__ float p_lds[64];
-  const T *q = (const T *)p.q + token * p.q_stride + (int64_t)h * D;
-  for (int c = lane; c < D; c += 64) q_lds[c] = (float)q[c];
-  __syncthreads();
-  const int64_t head_off = (int64_t)(h / p.group) * p.pool.head;
-  const int32_t *table = p.page_table + (int64_t)lo * p.table_stride;
-  auto row_of = [&](int key) -> int64_t {  // element offset of a key's row, -1: not in the pool
-    const int page = table[key >> p.page_shift];
-    if ((uint32_t)page >= (uint32_t)p.n_pages) return -1;
-    return page * p.pool.page + head_off + (key & ((1 << p.page_shift) - 1)) * p.pool.row;
-  };
-  float m = kNegInf, l = 0.0f, o[D / 64];
+  extern __shared__ __attribute__((aligned(16))) _Float16 smem[];
+  _Float16 *const sK = smem, *const sV = smem + 2 * BN * KP;  // [2][BN][KP], [2][BN][VP]
+  __shared__ int bad_tile[2];  // tile whose V held infinities or NaN under a mask
+
+  PagedItem it;
+  if (!sched_find<false>(p.sched, p.cu_new, p.kv_len, BN, blockIdx.x / p.heads_kv, it)) return;
+  if (it.nsplit > 1 && (uint32_t)(it.slot + it.split) >= (uint32_t)p.n_slots) return;
+  const int kvh = blockIdx.x % p.heads_kv;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int ln = lane & 31, hl = lane >> 5;
+  const int G = p.sched.group;
+  const int n_rows = (int)std::min<int64_t>((int64_t)(it.s.q_end - it.s.q_begin) * G, 0x7fffffff);
+  const int row0 = it.tile * kChunkRows;
+  const int row_last = min(n_rows, row0 + kChunkRows) - 1;
+
+  const int row = row0 + 32 * wave + ln;
+  const bool row_ok = row < n_rows;
+  const int rr = min(row, row_last);  // rows past the last one repeat it and are not stored
+  const int tok = rr / G, head = kvh * G + rr % G;
+  const int pos = it.s.pos0 + tok;
+  const int wg_first = it.s.pos0 + row0 / G, wg_last = it.s.pos0 + row_last / G;  // positions of the workgroup's rows
+  const bool windowed = p.sched.window > 0;
+  const int window = p.sched.window;
+
+  // keys the tile's rows see, and this part of them
+  const int key_end = min(it.s.len, max(wg_last, -1) + 1);
+  const int key_begin = windowed && wg_first >= window ? (wg_first - window + 1) / BN * BN : 0;
+  const int n_tiles = key_end > key_begin ? (key_end - key_begin + BN - 1) / BN : 0;
+  const int per = (n_tiles + it.nsplit - 1) / it.nsplit;
+  const int t0 = min(n_tiles, it.split * per), n_it = min(n_tiles, t0 + per) - t0;
+  const int base0 = key_begin + t0 * BN;
+
+  // ---- Q as the B operand: lane (row ln, half hl) holds channels 16 kk + 8 hl .. + 7
+  half8_t qh[KK], ql[F32 ? KK : 1];
+  const float c = p.scale * kLog2e;
+  {
+    const T *qp = (const T *)p.q + (int64_t)(it.s.q_begin + tok) * p.q_stride + (int64_t)head * D + 8 * hl;
 #pragma unroll
-  for (int c = 0; c < D / 64; ++c) o[c] = 0.0f;
-  for (int base = begin; base < end; base += 64) {
-    float s = kNegInf;
-    if (base + lane < end) {
-      const int64_t off = row_of(base + lane);
-      s = 0.0f;
-      if (off >= 0)
-        for (int c = 0; c < D; c += 8) {
-          const half8_t kv = *(const half8_t *)(p.k + off + c);
+    for (int kk = 0; kk < KK; ++kk) {
+      if constexpr (F32) {
+        const float4_t a = *(const float4_t *)(qp + 16 * kk), b = *(const float4_t *)(qp + 16 * kk + 4);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) s += q_lds[c + e] * (float)kv[e];
+        for (int e = 0; e < 8; ++e) {
+          _Float16 hi, lo;
+          split_f16((e < 4 ? a[e] : b[e - 4]) * (CAP ? p.scale : c), hi, lo);
+          qh[kk][e] = hi;
+          ql[kk][e] = lo;
         }
-      s *= p.scale;
-      if (p.softcap > 0.0f) s = p.softcap * tanhf(s / p.softcap);
+      } else {
+        qh[kk] = *(const half8_t *)(qp + 16 * kk);
+      }
     }
-    const float m_new = fmaxf(m, wave_allreduce_max(s));
+  }
+  const float inv_cap = CAP ? 1.0f / p.softcap : 0.0f;
+
+  // ---- tiles: piece i of a thread is 16 bytes of row (threadIdx + 256 i) / (D / 8) of the tile; the rows
+  // one wave covers with a piece lie in one page
+  PageWindow pages(p, it.seq, base0 >> p.page_shift, lane);
+  const int page_mask = (1 << p.page_shift) - 1;
+  const uint32_t row_bytes = (uint32_t)p.pool.row * 2;
+  const int my_row = lane / (D / 8), my_col = lane % (D / 8);
+  const uint32_t lane_off = my_row * row_bytes + 16 * my_col;
+  half8_t kpre[CH], vpre[CH];
+  auto fetch = [&](const _Float16 *pool, int base, half8_t(&pre)[CH]) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int key = base + wave * RPW + 4 * RPW * i;
+      const bool some = key < key_end;
+      const int page = (some ? key : key_end) >> p.page_shift;
+      const __amdgpu_buffer_rsrc_t rsrc =
+          page_rows(pool, p, pages.number(page), kvh, some ? min(key_end - (page << p.page_shift), page_mask + 1) : 0, D);
+      pre[i] = __builtin_bit_cast(half8_t, __builtin_amdgcn_raw_buffer_load_b128(rsrc, lane_off, some ? (uint32_t)(key & page_mask) * row_bytes : 0, 0));
+    }
+  };
+  // does some row of the workgroup not see some key of the tile?
+  auto edge_tile = [&](int base) { return base + BN - 1 > wg_first || base + BN > key_end || (windowed && base <= wg_last - window); };
+  auto stage = [&](int buf, int tile, int base) {
+    if (edge_tile(base)) {
+      // A weight of zero does not keep an infinity or a NaN out of the product: such values of V leave the
+      // tile here and are added, by themselves, to the rows that see their key.
+      bool bad = false;
+#pragma unroll
+      for (int i = 0; i < CH; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (not_finite(vpre[i][e])) {
+            bad = true;
+            vpre[i][e] = (_Float16)0.0f;
+          }
+      if (bad) bad_tile[buf] = tile;
+    }
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int key = wave * RPW + 4 * RPW * i + my_row;
+      *(half8_t *)(sK + (buf * BN + key) * KP + 8 * my_col) = kpre[i];
+      *(half8_t *)(sV + (buf * BN + key) * VP + 8 * my_col) = vpre[i];
+    }
+  };
+
+  float16_t o_acc[RB];
+#pragma unroll
+  for (int r = 0; r < RB; ++r)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o_acc[r][i] = 0.0f;
+  float m_run = kNegInf, l_run = 0.0f;
+
+  // V^T operand: ds_read_b64_tr_b16 gives lane i of 16 channel ch0 + i of keys key0 .. key0 + 3 when lane s
+  // addresses V[key0 + s / 4][ch0 + 4 (s % 4)]; P^T holds keys 4 hl + {0..3} and 8 + 4 hl + {0..3} of 16
+  const int g16 = lane >> 4, s16 = lane & 15;
+  const int vlane_off = (4 * (g16 >> 1) + (s16 >> 2)) * VP + 16 * (g16 & 1) + 4 * (s16 & 3);
+
+  if (threadIdx.x < 2) bad_tile[threadIdx.x] = -1;
+  if (n_it > 0) {
+    fetch(p.k, base0, kpre);
+    fetch(p.v, base0, vpre);
+  }
+  __syncthreads();
+  if (n_it > 0) stage(0, 0, base0);
+  __syncthreads();
+
+  for (int t = 0; t < n_it; ++t) {
+    const int base = base0 + t * BN, buf = t & 1;
+    pages.advance(base >> p.page_shift, lane);
+    if (t + 1 < n_it) {
+      fetch(p.k, base + BN, kpre);
+      fetch(p.v, base + BN, vpre);
+    }
+    float16_t s[KB];
+    const _Float16 *kt = sK + buf * BN * KP;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const half8_t a = *(const half8_t *)(kt + (32 * kb + ln) * KP + 16 * kk + 8 * hl);
+        s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[kk], kk == 0 ? float16_t{0.0f} : s[kb], 0, 0, 0);
+        if constexpr (F32) s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[kk], s[kb], 0, 0, 0);
+      }
+    const bool edge = edge_tile(base);
+    float mt = kNegInf;
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float x = s[kb][i];
+        if constexpr (CAP) x = soft_cap(F32 ? x : x * p.scale, p.softcap, inv_cap) * kLog2e;
+        else if constexpr (!F32) x *= c;
+        if (edge) {
+          const int key = base + 32 * kb + 8 * (i / 4) + 4 * hl + (i % 4);
+          if (key > pos || key >= key_end || (windowed && key <= pos - window)) x = kNegInf;
+        }
+        s[kb][i] = x;
+        mt = fmaxf(mt, x);
+      }
+    mt = xor32_combine(mt, [](float a, float b) { return fmaxf(a, b); });
+    const float m_new = fmaxf(m_run, mt);
     const float m_ref = m_new == kNegInf ? 0.0f : m_new;
-    const float w = expf(s - m_ref), alpha = expf(m - m_ref);
-    l = l * alpha + wave_allreduce_sum(w);
-    m = m_new;
+    const float alpha = __builtin_amdgcn_exp2f(m_run - m_ref);
+    m_run = m_new;
+    float lsum = 0.0f;
+    half8_t ph[BN / 16], pl[F32 ? BN / 16 : 1];
 #pragma unroll
-    for (int c = 0; c < D / 64; ++c) o[c] *= alpha;
-    p_lds[lane] = w;
-    __syncthreads();
-    const int n = min(64, end - base);
-    for (int t = 0; t < n; ++t) {
-      const int64_t off = row_of(base + t);
-      if (off < 0) continue;
+    for (int jn = 0; jn < BN / 16; ++jn)
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c) o[c] += p_lds[t] * (float)p.v[off + c * 64 + lane];
+      for (int e = 0; e < 8; ++e) {
+        const float w = __builtin_amdgcn_exp2f(s[jn / 2][8 * (jn % 2) + e] - m_ref);
+        lsum += w;
+        if constexpr (F32) {
+          _Float16 hi, lo;
+          split_f16(w, hi, lo);
+          ph[jn][e] = hi;
+          pl[jn][e] = lo;
+        } else {
+          ph[jn][e] = (_Float16)w;
+        }
+      }
+    l_run = l_run * alpha + lsum;
+    if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
+#pragma unroll
+      for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o_acc[r][i] *= alpha;
     }
+    const _Float16 *vt = sV + buf * BN * VP + vlane_off;
+#pragma unroll
+    for (int jn = 0; jn < BN / 16; ++jn)
+#pragma unroll
+      for (int r = 0; r < RB; ++r) {
+        const _Float16 *vp = vt + 16 * jn * VP + 32 * r;
+        const half4_t lo = lds_read_tr16(vp), hi = lds_read_tr16(vp + 8 * VP);
+        const half8_t a = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+        o_acc[r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[jn], o_acc[r], 0, 0, 0);
+        if constexpr (F32) o_acc[r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[jn], o_acc[r], 0, 0, 0);
+      }
+    if (edge && bad_tile[buf] == t) {
+      for (int k = 0; k < BN; ++k) {
+        const int key = base + k;
+        if (key >= key_end) break;
+        const int number = pages.row[key >> p.page_shift];  // key < key_end <= the table's room
+        if ((uint32_t)number >= (uint32_t)p.n_pages) continue;
+        const _Float16 *vrow = p.v + number * p.pool.page + kvh * p.pool.head + (key & page_mask) * p.pool.row;
+        const bool sees = key <= pos && !(windowed && key <= pos - window);
+#pragma unroll
+        for (int r = 0; r < RB; ++r)
+#pragma unroll
+          for (int i4 = 0; i4 < 4; ++i4) {
+            const half4_t x = *(const half4_t *)(vrow + 32 * r + 8 * i4 + 4 * hl);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (sees && not_finite(x[e])) o_acc[r][4 * i4 + e] += (float)x[e];
+          }
+      }
+    }
+    if (t + 1 < n_it) stage(buf ^ 1, t + 1, base + BN);
     __syncthreads();
   }
-  T *out = (T *)p.out + token * p.out_stride + (int64_t)h * D;
+
+  l_run += __shfl_xor(l_run, 32, 64);
+  if (it.nsplit > 1) {
+    const int64_t at = ((int64_t)(it.slot + it.split) * p.heads_kv + kvh) * kChunkRows + 32 * wave + ln;
+    if (row_ok) {
+      float *o = p.ws_o + at * D;
 #pragma unroll
-  for (int c = 0; c < D / 64; ++c) out[c * 64 + lane] = (T)(l == 0.0f ? 0.0f : o[c] / l);
+      for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4)
+          *(float4_t *)(o + 32 * r + 8 * i4 + 4 * hl) = float4_t{o_acc[r][4 * i4], o_acc[r][4 * i4 + 1], o_acc[r][4 * i4 + 2], o_acc[r][4 * i4 + 3]};
+      if (hl == 0) {
+        p.ws_ml[at * 2] = m_run;
+        p.ws_ml[at * 2 + 1] = l_run;
+      }
+    }
+    return;
+  }
+  if (row_ok) {
+    const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
+    T *out = (T *)p.out + (int64_t)(it.s.q_begin + tok) * p.out_stride + (int64_t)head * D;
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (int i4 = 0; i4 < 4; ++i4) {
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        T4 o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = (T)(l_run == 0.0f ? 0.0f : o_acc[r][4 * i4 + e] * inv);
+        *(T4 *)(out + 32 * r + 8 * i4 + 4 * hl) = o;
+      }
+  }
+}
+
+// Merge of the parts of cut tiles: row m of a tile is sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m), in the
+// order of the parts.  D / 4 threads share a row.
+template <int D, typename T>
+__global__ __launch_bounds__(256) void paged_combine_kernel(const PagedParams p, int align) {
+  constexpr int RPB = 256 / (D / 4);
+  const int R = p.sched.tile_rows, chunks = (R + RPB - 1) / RPB;
+  const int x = blockIdx.x / chunks, kvh = x % p.heads_kv;
+  PagedItem it;
+  if (!sched_find<true>(p.sched, p.cu_new, p.kv_len, align, x / p.heads_kv, it)) return;
+  if (it.slot < 0 || (int64_t)it.slot + it.nsplit > p.n_slots) return;
+  const int G = p.sched.group;
+  const int lr = blockIdx.x % chunks * RPB + threadIdx.x / (D / 4), ch = threadIdx.x % (D / 4) * 4;
+  const int64_t row = (int64_t)it.tile * R + lr;
+  if (lr >= R || row >= (int64_t)(it.s.q_end - it.s.q_begin) * G) return;
+  const int64_t step = (int64_t)p.heads_kv * R, at = (int64_t)it.slot * step + (int64_t)kvh * R + lr;
+  float m = kNegInf;
+  for (int i = 0; i < it.nsplit; ++i) m = fmaxf(m, p.ws_ml[(at + i * step) * 2]);
+  const float m_ref = m == kNegInf ? 0.0f : m;
+  float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+  float l = 0.0f;
+#pragma unroll 4
+  for (int i = 0; i < it.nsplit; ++i) {
+    const float f = __builtin_amdgcn_exp2f(p.ws_ml[(at + i * step) * 2] - m_ref);
+    l += p.ws_ml[(at + i * step) * 2 + 1] * f;
+    const float4_t part = *(const float4_t *)(p.ws_o + (at + i * step) * D + ch);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[e] += part[e] * f;
+  }
+  T *out = (T *)p.out + (int64_t)(it.s.q_begin + row / G) * p.out_stride + (int64_t)(kvh * G + row % G) * D + ch;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) out[e] = (T)(l == 0.0f ? 0.0f : o[e] / l);
+}
+
+template <int D, typename T>
+int launch_chunk(argus_hip_ctx *ctx, const PagedParams &p, int items, hipStream_t stream) {
+  auto kern = p.softcap > 0.0f ? paged_chunk_kernel<D, T, true> : paged_chunk_kernel<D, T, false>;
+  ARGUS_HIP_CHECK(ctx, argus_raise_lds_limit(ctx, kern, ChunkTile<D>::LDS_BYTES));
+  hipLaunchKernelGGL(kern, dim3((unsigned)(items * p.heads_kv)), dim3(256), ChunkTile<D>::LDS_BYTES, stream, p);
+  ARGUS_HIP_CHECK(ctx, hipGetLastError());
+  return ARGUS_HIP_OK;
+}
+
+// How a call is cut: which kernels run, with how many workgroups, and where their partial results lie.
+struct CallPlan {
+  bool decode, chunk;
+  PagedSched ds, cs;
+  int64_t d_items, c_items, d_cut, c_cut, d_slots, c_slots;
+  int64_t ws_floats;  // [decode ml][decode o][chunk ml][chunk o]
+};
+
+int make_plan(argus_hip_ctx *ctx, int compute_units, const argus_hip_paged_attention_args *a, CallPlan &pl) {
+  const int G = a->heads_q / a->heads_kv, d = a->head_dim;
+  const int64_t room = std::min<int64_t>((int64_t)a->table_stride * a->page_size, 0x7fffffff - 4096);
+  PagedSched s{};
+  s.n_seqs = a->n_seqs;
+  s.n_tokens = a->n_tokens;
+  s.group = G;
+  s.window = a->window;
+  s.max_len = (int)room;
+  pl = CallPlan{};
+  pl.decode = G <= kDecodeRows && (int64_t)a->min_new * G <= kDecodeRows;
+  pl.chunk = !pl.decode || a->max_new == 0 || (int64_t)a->max_new * G > kDecodeRows;
+  const int64_t longest = a->max_kv > 0 ? std::min<int64_t>(a->max_kv, room) : room;
+  if (pl.decode) {
+    pl.ds = s;
+    pl.ds.rows_over = 0;
+    pl.ds.rows_upto = kDecodeRows;
+    pl.ds.tile_rows = kDecodeRows;
+    pl.ds.unit = 4 * decode_align(d);
+    pl.ds.min_units = 2;
+    pl.ds.target = std::max(1, compute_units * 3 / a->heads_kv);
+    pl.ds.max_splits = (int)std::min<int64_t>(128, std::max<int64_t>(1, (longest + pl.ds.unit - 1) / pl.ds.unit / pl.ds.min_units));
+    const int64_t tiles = std::min<int64_t>(a->n_seqs, a->n_tokens);
+    pl.d_items = sched_items_bound(pl.ds, tiles);
+    pl.d_slots = sched_slots_bound(pl.ds, tiles);
+    pl.d_cut = sched_cut_tiles_bound(pl.ds, tiles);
+  }
+  if (pl.chunk) {
+    pl.cs = s;
+    pl.cs.rows_over = pl.decode ? kDecodeRows : 0;
+    pl.cs.rows_upto = 0x7fffffff;
+    pl.cs.tile_rows = kChunkRows;
+    pl.cs.unit = 128;
+    pl.cs.min_units = 4;
+    pl.cs.target = std::max(1, compute_units * 2 / a->heads_kv);
+    pl.cs.max_splits = (int)std::min<int64_t>(64, std::max<int64_t>(1, (longest + pl.cs.unit - 1) / pl.cs.unit / pl.cs.min_units));
+    const int64_t tiles = sched_tiles_bound(pl.cs, a->min_new);
+    if (tiles == 0) pl.chunk = false;  // too few rows for any request of this class
+    pl.c_items = tiles ? sched_items_bound(pl.cs, tiles) : 0;
+    pl.c_slots = sched_slots_bound(pl.cs, tiles);
+    pl.c_cut = sched_cut_tiles_bound(pl.cs, tiles);
+  }
+  constexpr int64_t kGrid = 0x7fffffff;
+  if (pl.d_items * a->heads_kv > kGrid || pl.c_items * a->heads_kv > kGrid)
+    return argus_fail(ctx, ARGUS_HIP_ERR_UNSUPPORTED, "paged_attention: %d rows are too many for one call", a->n_tokens);
+  pl.ws_floats = (pl.d_slots * kDecodeRows + pl.c_slots * kChunkRows) * a->heads_kv * (d + 2);
+  return ARGUS_HIP_OK;
 }
 
 int check(argus_hip_ctx *ctx, const argus_hip_paged_attention_args *a) {
@@ -100,6 +406,8 @@ int check(argus_hip_ctx *ctx, const argus_hip_paged_attention_args *a) {
   if (!argus_page_size_ok(a->page_size))
     return argus_fail(ctx, ARGUS_HIP_ERR_UNSUPPORTED, "paged_attention: page_size %d is not a power of two from 16 to %d", a->page_size,
                       ARGUS_HIP_MAX_PAGE_SIZE);
+  if ((int64_t)a->heads_kv * a->page_size * a->head_dim * 2 > 0x7fffffff)
+    return argus_fail(ctx, ARGUS_HIP_ERR_UNSUPPORTED, "paged_attention: a page of %d heads x %d tokens is larger than 2 GiB", a->heads_kv, a->page_size);
   if (a->layout != ARGUS_HIP_HEAD_MAJOR && a->layout != ARGUS_HIP_SEQ_MAJOR)
     return argus_fail(ctx, ARGUS_HIP_ERR_INVALID, "paged_attention: layout %d", a->layout);
   if (a->dtype != ARGUS_HIP_F32 && a->dtype != ARGUS_HIP_F16)
@@ -115,37 +423,96 @@ int check(argus_hip_ctx *ctx, const argus_hip_paged_attention_args *a) {
 
 }  // namespace
 
+int launch_paged_chunk(argus_hip_ctx *ctx, const PagedParams &p, int D, bool f32, int items, hipStream_t stream) {
+  switch (D) {
+    case 64: return f32 ? launch_chunk<64, float>(ctx, p, items, stream) : launch_chunk<64, _Float16>(ctx, p, items, stream);
+    case 128: return f32 ? launch_chunk<128, float>(ctx, p, items, stream) : launch_chunk<128, _Float16>(ctx, p, items, stream);
+    default: return f32 ? launch_chunk<256, float>(ctx, p, items, stream) : launch_chunk<256, _Float16>(ctx, p, items, stream);
+  }
+}
+
+int launch_paged_combine(argus_hip_ctx *ctx, const PagedParams &p, int D, bool f32, int align, int tiles, hipStream_t stream) {
+  const int rpb = 256 / (D / 4), chunks = (p.sched.tile_rows + rpb - 1) / rpb;
+  auto kern = D == 64 ? (f32 ? paged_combine_kernel<64, float> : paged_combine_kernel<64, _Float16>)
+              : D == 128 ? (f32 ? paged_combine_kernel<128, float> : paged_combine_kernel<128, _Float16>)
+                         : (f32 ? paged_combine_kernel<256, float> : paged_combine_kernel<256, _Float16>);
+  hipLaunchKernelGGL(kern, dim3((unsigned)(tiles * p.heads_kv * chunks)), dim3(256), 0, stream, p, align);
+  ARGUS_HIP_CHECK(ctx, hipGetLastError());
+  return ARGUS_HIP_OK;
+}
+
+}  // namespace argus_paged
+
+using namespace argus_paged;
+
 ARGUS_API int64_t argus_hip_paged_attention_workspace(const argus_hip_ctx *ctx, const argus_hip_paged_attention_args *a) {
   if (!a) return ARGUS_HIP_ERR_INVALID;
-  const int rc = check(const_cast<argus_hip_ctx *>(ctx), a);
-  return rc != ARGUS_HIP_OK ? rc : 0;
+  argus_hip_ctx *c = const_cast<argus_hip_ctx *>(ctx);  // for the error text
+  int rc = check(c, a);
+  CallPlan pl;
+  if (rc == ARGUS_HIP_OK) rc = make_plan(c, ctx ? ctx->compute_units : 256, a, pl);
+  return rc != ARGUS_HIP_OK ? rc : pl.ws_floats * (int64_t)sizeof(float);
 }
 
 ARGUS_API int argus_hip_paged_attention(argus_hip_ctx *ctx, const argus_hip_paged_attention_args *a) {
   if (!ctx || !a) return ARGUS_HIP_ERR_INVALID;
-  const int rc = check(ctx, a);
+  int rc = check(ctx, a);
+  CallPlan pl;
+  if (rc == ARGUS_HIP_OK) rc = make_plan(ctx, ctx->compute_units, a, pl);
   if (rc != ARGUS_HIP_OK) return rc;
   if (a->n_seqs == 0 || a->n_tokens == 0) return ARGUS_HIP_OK;
   if (!a->q || !a->k_cache || !a->v_cache || !a->page_table || !a->cu_new || !a->kv_len || !a->out)
     return argus_fail(ctx, ARGUS_HIP_ERR_INVALID, "paged_attention: null pointer");
   if (((uintptr_t)a->q | (uintptr_t)a->k_cache | (uintptr_t)a->v_cache | (uintptr_t)a->out) & 15)
     return argus_fail(ctx, ARGUS_HIP_ERR_INVALID, "paged_attention: q, out and the pools are 16-byte aligned");
-  const int d = a->head_dim;
-  const int64_t grid = (int64_t)a->n_tokens * a->heads_q;
-  if (grid > 0x7fffffff) return argus_fail(ctx, ARGUS_HIP_ERR_UNSUPPORTED, "paged_attention: too many rows");
   const DeviceGuard guard(ctx);
-  PagedParams p{a->q, (const _Float16 *)a->k_cache, (const _Float16 *)a->v_cache, a->page_table, a->cu_new, a->kv_len, a->out,
-                a->q_stride ? a->q_stride : (int64_t)a->heads_q * d, a->out_stride ? a->out_stride : (int64_t)a->heads_q * d,
-                argus_pool_strides(a->layout, a->heads_kv, a->page_size, d), a->n_seqs, a->n_tokens, a->heads_q, a->heads_kv,
-                a->heads_q / a->heads_kv, a->n_pages, argus_log2(a->page_size), a->table_stride, a->window, a->softcap,
-                a->scale != 0.0f ? a->scale : 1.0f / sqrtf((float)d)};
   const hipStream_t stream = (hipStream_t)a->stream;
-  const bool f16 = a->dtype == ARGUS_HIP_F16;
-  auto kern = d == 64 ? (f16 ? paged_row_kernel<64, _Float16> : paged_row_kernel<64, float>)
-              : d == 128 ? (f16 ? paged_row_kernel<128, _Float16> : paged_row_kernel<128, float>)
-                         : (f16 ? paged_row_kernel<256, _Float16> : paged_row_kernel<256, float>);
+  const size_t need = (size_t)pl.ws_floats * sizeof(float);
+  float *ws = (float *)a->workspace;
+  if (ws) {
+    if ((uintptr_t)ws & 255) return argus_fail(ctx, ARGUS_HIP_ERR_INVALID, "paged_attention: the workspace is not 256-byte aligned");
+    if (a->workspace_bytes < need)
+      return argus_fail(ctx, ARGUS_HIP_ERR_NOMEM, "paged_attention: the workspace holds %zu bytes, the call needs %zu", a->workspace_bytes, need);
+  } else if (need) {
+    // A captured call keeps the workspace's address: the context's may be replaced by a larger one.
+    hipStreamCaptureStatus capturing = hipStreamCaptureStatusNone;
+    ARGUS_HIP_CHECK(ctx, hipStreamIsCapturing(stream, &capturing));
+    if (capturing != hipStreamCaptureStatusNone)
+      return argus_fail(ctx, ARGUS_HIP_ERR_INVALID, "paged_attention: a call under stream capture brings its own workspace (%zu bytes)", need);
+    rc = argus_ws_reserve(ctx, need);
+    if (rc != ARGUS_HIP_OK) return rc;
+    ws = argus_ws(ctx);
+  }
+  const int d = a->head_dim;
+  const bool f32 = a->dtype == ARGUS_HIP_F32;
+  PagedParams p{};
+  p.q = a->q, p.k = (const _Float16 *)a->k_cache, p.v = (const _Float16 *)a->v_cache, p.out = a->out;
+  p.page_table = a->page_table, p.cu_new = a->cu_new, p.kv_len = a->kv_len;
+  p.q_stride = a->q_stride ? a->q_stride : (int64_t)a->heads_q * d;
+  p.out_stride = a->out_stride ? a->out_stride : (int64_t)a->heads_q * d;
+  p.pool = argus_pool_strides(a->layout, a->heads_kv, a->page_size, d);
+  p.heads_kv = a->heads_kv, p.n_pages = a->n_pages, p.page_shift = argus_log2(a->page_size), p.table_stride = a->table_stride;
+  p.softcap = a->softcap, p.scale = a->scale != 0.0f ? a->scale : 1.0f / std::sqrt((float)d);
   KernelTimer timer(ctx, stream);
-  hipLaunchKernelGGL(kern, dim3((unsigned)grid), dim3(64), 0, stream, p);
-  ARGUS_HIP_CHECK(ctx, hipGetLastError());
-  return ARGUS_HIP_OK;
+  if (pl.decode) {
+    p.sched = pl.ds;
+    p.n_slots = (int)pl.d_slots;
+    p.ws_o = ws;  // output rows first: they are read and written 16 bytes at a time
+    p.ws_ml = ws + pl.d_slots * kDecodeRows * a->heads_kv * d;
+    rc = launch_paged_decode(ctx, p, d, f32, (int)pl.d_items, stream);
+    if (rc == ARGUS_HIP_OK && !pl.chunk) timer.mark();
+    if (rc == ARGUS_HIP_OK && pl.d_cut) rc = launch_paged_combine(ctx, p, d, f32, decode_align(d), (int)pl.d_cut, stream);
+    if (rc != ARGUS_HIP_OK) return rc;
+    if (ws) ws += pl.d_slots * kDecodeRows * a->heads_kv * (d + 2);
+  }
+  if (pl.chunk) {
+    p.sched = pl.cs;
+    p.n_slots = (int)pl.c_slots;
+    p.ws_o = ws;
+    p.ws_ml = ws + pl.c_slots * kChunkRows * a->heads_kv * d;
+    rc = launch_paged_chunk(ctx, p, d, f32, (int)pl.c_items, stream);
+    timer.mark();
+    if (rc == ARGUS_HIP_OK && pl.c_cut) rc = launch_paged_combine(ctx, p, d, f32, chunk_align(d), (int)pl.c_cut, stream);
+  }
+  return rc;
 }

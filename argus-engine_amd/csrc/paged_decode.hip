@@ -1,0 +1,340 @@
+// paged_attention of requests with few rows (new tokens x heads of a GQA group, at most 16): decode
+// steps and short drafts.  Split over the keys, both products on the matrix cores.
+//
+//   S^T[key][row] = K . Q^T   v_mfma_f32_16x16x32_f16: A lane (j, r) = chunk 4 kk + j of key r's row -- 16
+//                             consecutive keys lie in one page, so this is one 16-byte load per lane with the
+//                             page's descriptor in scalar registers; B = the same chunk of row r of Q
+//   O[row][channel] = P . V   A = the lane's own probabilities (keys 4j .. 4j + 3 of each 16), B = V rows
+//                             transposed 4 x 8 in registers
+//
+// Nothing goes through LDS in the key loop.  F16 queries are held as they are (the products are exact, the
+// scale is applied to the F32 logit) and probabilities are rounded to F16, as the output will be; F32
+// queries and the probabilities of their rows are held as F16 pairs, hi + lo, in two MFMAs each, which
+// leaves F32's error.  Bound by HBM: every key is read once per KV head for all rows.
+#include "paged_common.hpp"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace argus_paged {
+
+namespace {
+
+template <int D>
+struct DecodeShape {
+  static constexpr int KK = D / 32;              // logits MFMAs per 16 keys
+  static constexpr int VC = D >= 128 ? 8 : 4;    // channels of a V piece
+  static constexpr int VSEG = D / (16 * VC);     // pieces per row and lane
+  static constexpr int NACC = VC * VSEG;
+  static constexpr int TW = D <= 128 ? 2 : 1;    // blocks of 16 keys per wave step
+};
+constexpr int kWaves = 4;
+
+template <typename T>
+__device__ __forceinline__ T load_stream(__amdgpu_buffer_rsrc_t rsrc, uint32_t voff, uint32_t soff);
+template <>
+__device__ __forceinline__ half8_t load_stream<half8_t>(__amdgpu_buffer_rsrc_t rsrc, uint32_t voff, uint32_t soff) {
+  return __builtin_bit_cast(half8_t, __builtin_amdgcn_raw_buffer_load_b128(rsrc, voff, soff, 2));
+}
+template <>
+__device__ __forceinline__ half4_t load_stream<half4_t>(__amdgpu_buffer_rsrc_t rsrc, uint32_t voff, uint32_t soff) {
+  return __builtin_bit_cast(half4_t, __builtin_amdgcn_raw_buffer_load_b64(rsrc, voff, soff, 2));
+}
+
+template <int D, typename T, bool CAP>
+__global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(const PagedParams p) {
+  using SH = DecodeShape<D>;
+  constexpr int KK = SH::KK, VC = SH::VC, VSEG = SH::VSEG, NACC = SH::NACC, TW = SH::TW;
+  constexpr int STEP = 16 * TW;
+  static_assert(STEP == decode_align(D), "key ranges start on a step");
+  constexpr bool F32 = std::is_same<T, float>::value;
+  typedef typename std::conditional<VC == 8, half8_t, half4_t>::type vpiece_t;
+  constexpr float kLog2e = 1.4426950408889634f;
+
+  PagedItem it;
+  if (!sched_find<false>(p.sched, p.cu_new, p.kv_len, STEP, blockIdx.x / p.heads_kv, it)) return;
+  if (it.nsplit > 1 && (uint32_t)(it.slot + it.split) >= (uint32_t)p.n_slots) return;
+  const int kvh = blockIdx.x % p.heads_kv;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int j = lane >> 4, r = lane & 15;
+  const int G = p.sched.group;
+  const int rows = (it.s.q_end - it.s.q_begin) * G;  // at most 16: one tile
+
+  // keys of this part: whole units behind key_begin
+  const int64_t part = it.nsplit > 1 ? (sched_units(p.sched, it.s) + it.nsplit - 1) / it.nsplit * (int64_t)p.sched.unit : 0;
+  const int begin = (int)std::min<int64_t>(it.s.key_end, it.s.key_begin + it.split * part);
+  const int end = it.nsplit > 1 ? (int)std::min<int64_t>(it.s.key_end, begin + part) : it.s.key_end;
+
+  // row r: token r / G, head r % G; columns past the last row repeat it and are never stored
+  const int rr = min(r, rows - 1);
+  const int pos = it.s.pos0 + rr / G;
+  const int pos_last = it.s.pos0 + (rows - 1) / G;
+  const int window = p.sched.window > 0 ? p.sched.window : 0x7fffffff;
+
+  PageWindow pages(p, it.seq, begin >> p.page_shift, lane);
+  const int page_mask = (1 << p.page_shift) - 1;
+  const uint32_t row_bytes = (uint32_t)p.pool.row * 2;
+  const uint32_t k_lane = r * row_bytes + 16 * j, v_lane = 4 * j * row_bytes + 2 * VC * r;
+  half8_t kr[TW][KK];
+  vpiece_t vr[TW][VSEG][4];
+  // the page of 16 keys from `key` on, ended at this part's last key (behind it: no rows at all), and the
+  // offset of the first of them
+  auto rows_at = [&](const _Float16 *pool, int key, uint32_t &soff) {
+    const bool some = key < end;
+    const int page = (some ? key : end) >> p.page_shift;
+    soff = some ? (uint32_t)(key & page_mask) * row_bytes : 0;
+    return page_rows(pool, p, pages.number(page), kvh, some ? min(end - (page << p.page_shift), page_mask + 1) : 0, D);
+  };
+  auto load_k = [&](int base) {
+#pragma unroll
+    for (int tw = 0; tw < TW; ++tw) {
+      uint32_t soff;
+      const __amdgpu_buffer_rsrc_t rsrc = rows_at(p.k, base + 16 * tw, soff);
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) kr[tw][kk] = load_stream<half8_t>(rsrc, k_lane + 64 * kk, soff);
+    }
+  };
+  auto load_v = [&](int base) {
+#pragma unroll
+    for (int tw = 0; tw < TW; ++tw) {
+      uint32_t soff;
+      const __amdgpu_buffer_rsrc_t rsrc = rows_at(p.v, base + 16 * tw, soff);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+#pragma unroll
+        for (int sg = 0; sg < VSEG; ++sg) vr[tw][sg][e] = load_stream<vpiece_t>(rsrc, v_lane + e * row_bytes + 32 * VC * sg, soff);
+    }
+  };
+  const int base0 = begin + wave * STEP;
+  load_k(base0);
+  load_v(base0);
+
+  // Q: lane (j, r) holds chunk 4 kk + j of row r
+  half8_t qh[KK], ql[F32 ? KK : 1];
+  const float c = p.scale * kLog2e;
+  {
+    const T *qp = (const T *)p.q + (int64_t)(it.s.q_begin + rr / G) * p.q_stride + (int64_t)(kvh * G + rr % G) * D;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      if constexpr (F32) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = qp[(4 * kk + j) * 8 + e];
+        loaded8(x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          _Float16 hi, lo;
+          split_f16(CAP ? x[e] * p.scale : x[e] * c, hi, lo);
+          qh[kk][e] = hi;
+          ql[kk][e] = lo;
+        }
+      } else {
+        qh[kk] = *(const half8_t *)(qp + (4 * kk + j) * 8);
+      }
+    }
+  }
+  const float inv_cap = CAP ? 1.0f / p.softcap : 0.0f;
+
+  float4_t o_acc[NACC];
+#pragma unroll
+  for (int a = 0; a < NACC; ++a) o_acc[a] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  float m_run = kNegInf, l_run = 0.0f;  // of row r; l: this lane group's keys
+
+  for (int base = base0; base < end; base += kWaves * STEP) {
+    float4_t s[TW];
+#pragma unroll
+    for (int tw = 0; tw < TW; ++tw) {
+      s[tw] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        s[tw] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kr[tw][kk], qh[kk], s[tw], 0, 0, 0);
+        if constexpr (F32) s[tw] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kr[tw][kk], ql[kk], s[tw], 0, 0, 0);
+      }
+    }
+    pages.advance(base >> p.page_shift, lane);
+    load_k(base + kWaves * STEP);
+    // keys some row does not see: past the first token's position, in front of the last one's window, past the part
+    const bool edge = base + STEP - 1 > it.s.pos0 || base + STEP > end || (window != 0x7fffffff && base <= pos_last - window);
+    float mt = kNegInf;
+#pragma unroll
+    for (int tw = 0; tw < TW; ++tw)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x = s[tw][i];
+        if constexpr (CAP) x = soft_cap(F32 ? x : x * p.scale, p.softcap, inv_cap) * kLog2e;
+        else if constexpr (!F32) x *= c;
+        if (edge) {
+          const int key = base + 16 * tw + 4 * j + i;
+          if (key > pos || key >= end || (window != 0x7fffffff && key <= pos - window)) x = kNegInf;
+        }
+        s[tw][i] = x;
+        mt = fmaxf(mt, x);
+      }
+    mt = rows_allreduce_max(mt);
+    const float m_new = fmaxf(m_run, mt);
+    const float m_ref = m_new == kNegInf ? 0.0f : m_new;
+    const float alpha = __builtin_amdgcn_exp2f(m_run - m_ref);
+    m_run = m_new;
+    half4_t pa[TW], pl[F32 ? TW : 1];
+    float lsum = 0.0f;
+#pragma unroll
+    for (int tw = 0; tw < TW; ++tw)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float w = __builtin_amdgcn_exp2f(s[tw][i] - m_ref);
+        lsum += w;
+        if constexpr (F32) {
+          _Float16 hi, lo;
+          split_f16(w, hi, lo);
+          pa[tw][i] = hi;
+          pl[tw][i] = lo;
+        } else {
+          pa[tw][i] = (_Float16)w;
+        }
+      }
+    l_run = l_run * alpha + lsum;
+    if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
+      float al[4];  // accumulator register i of lane group j belongs to row 4j + i
+#pragma unroll
+      for (int i = 0; i < 4; ++i) al[i] = __shfl(alpha, 4 * j + i, 64);
+#pragma unroll
+      for (int a = 0; a < NACC; ++a)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o_acc[a][i] *= al[i];
+    }
+    if (edge) {
+      // A weight of zero does not keep an infinity or a NaN out of the product.  Such values of V leave
+      // the operands here and are added, by themselves, to the rows that see their key.
+      bool any = false;
+#pragma unroll
+      for (int tw = 0; tw < TW; ++tw)
+#pragma unroll
+        for (int sg = 0; sg < VSEG; ++sg)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+#pragma unroll
+            for (int ch = 0; ch < VC; ++ch) any |= not_finite(vr[tw][sg][e][ch]);
+      if (__builtin_amdgcn_ballot_w64(any) != 0) {
+#pragma unroll
+        for (int tw = 0; tw < TW; ++tw)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            for (int jj = 0; jj < 4; ++jj) {
+              const int key = base + 16 * tw + 4 * jj + e;
+              bool sees[4];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int row_pos = it.s.pos0 + min(4 * j + i, rows - 1) / G;
+                sees[i] = key <= row_pos && key < end && !(window != 0x7fffffff && key <= row_pos - window);
+              }
+#pragma unroll
+              for (int sg = 0; sg < VSEG; ++sg)
+#pragma unroll
+                for (int ch = 0; ch < VC; ++ch) {
+                  const float x = __shfl((float)vr[tw][sg][e][ch], 16 * jj + r, 64);
+                  if (!(__builtin_fabsf(x) < __builtin_huge_valf()))
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                      if (sees[i]) o_acc[sg * VC + ch][i] += x;
+                }
+            }
+#pragma unroll
+        for (int tw = 0; tw < TW; ++tw)
+#pragma unroll
+          for (int sg = 0; sg < VSEG; ++sg)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int ch = 0; ch < VC; ++ch)
+                if (not_finite(vr[tw][sg][e][ch])) vr[tw][sg][e][ch] = (_Float16)0.0f;
+      }
+    }
+#pragma unroll
+    for (int sg = 0; sg < VSEG; ++sg)
+#pragma unroll
+      for (int ch = 0; ch < VC; ++ch) {
+        float4_t &o = o_acc[sg * VC + ch];
+        if constexpr (TW == 2) {
+          // contraction slots 8j + e hold keys 4j + e of the first block, 8j + 4 + e those of the second
+          const half8_t bv = {vr[0][sg][0][ch], vr[0][sg][1][ch], vr[0][sg][2][ch], vr[0][sg][3][ch],
+                              vr[1][sg][0][ch], vr[1][sg][1][ch], vr[1][sg][2][ch], vr[1][sg][3][ch]};
+          const half8_t av = {pa[0][0], pa[0][1], pa[0][2], pa[0][3], pa[1][0], pa[1][1], pa[1][2], pa[1][3]};
+          o = __builtin_amdgcn_mfma_f32_16x16x32_f16(av, bv, o, 0, 0, 0);
+          if constexpr (F32) {
+            const half8_t lv = {pl[0][0], pl[0][1], pl[0][2], pl[0][3], pl[1][0], pl[1][1], pl[1][2], pl[1][3]};
+            o = __builtin_amdgcn_mfma_f32_16x16x32_f16(lv, bv, o, 0, 0, 0);
+          }
+        } else {
+          const half4_t bv = {vr[0][sg][0][ch], vr[0][sg][1][ch], vr[0][sg][2][ch], vr[0][sg][3][ch]};
+          o = __builtin_amdgcn_mfma_f32_16x16x16f16(pa[0], bv, o, 0, 0, 0);
+          if constexpr (F32) o = __builtin_amdgcn_mfma_f32_16x16x16f16(pl[0], bv, o, 0, 0, 0);
+        }
+      }
+    load_v(base + kWaves * STEP);
+  }
+
+  // ---- merge: lane groups (row sum), then the waves through LDS -----------------------------------
+  l_run += __shfl_xor(l_run, 16, 64);
+  l_run += __shfl_xor(l_run, 32, 64);
+  __shared__ float lds_m[kWaves][16], lds_l[kWaves][16];
+  extern __shared__ __attribute__((aligned(16))) float lds_acc[];  // [kWaves][16][D + 4]
+  if (j == 0) {
+    lds_m[wave][r] = m_run;
+    lds_l[wave][r] = l_run;
+  }
+#pragma unroll
+  for (int sg = 0; sg < VSEG; ++sg)
+#pragma unroll
+    for (int ch = 0; ch < VC; ++ch)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (4 * j + i < rows) lds_acc[(wave * 16 + 4 * j + i) * (D + 4) + 16 * VC * sg + VC * r + ch] = o_acc[sg * VC + ch][i];
+  __syncthreads();
+  for (int x = threadIdx.x; x < rows * D; x += 64 * kWaves) {
+    const int row = x / D, ch = x % D;
+    float mm = lds_m[0][row];
+#pragma unroll
+    for (int w = 1; w < kWaves; ++w) mm = fmaxf(mm, lds_m[w][row]);
+    const float m_ref = mm == kNegInf ? 0.0f : mm;
+    float o = 0.0f, l = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) {
+      const float f = __builtin_amdgcn_exp2f(lds_m[w][row] - m_ref);
+      o += lds_acc[(w * 16 + row) * (D + 4) + ch] * f;
+      l += lds_l[w][row] * f;
+    }
+    if (it.nsplit == 1) {
+      T *out = (T *)p.out + (int64_t)(it.s.q_begin + row / G) * p.out_stride + (int64_t)(kvh * G + row % G) * D;
+      out[ch] = (T)(l == 0.0f ? 0.0f : o / l);
+    } else {
+      const int64_t at = ((int64_t)(it.slot + it.split) * p.heads_kv + kvh) * kDecodeRows + row;
+      p.ws_o[at * D + ch] = o;
+      if (ch == 0) {
+        p.ws_ml[at * 2] = mm;
+        p.ws_ml[at * 2 + 1] = l;
+      }
+    }
+  }
+}
+
+template <int D, typename T>
+int launch(argus_hip_ctx *ctx, const PagedParams &p, int items, hipStream_t stream) {
+  constexpr size_t lds = (size_t)kWaves * 16 * (D + 4) * sizeof(float);
+  auto kern = p.softcap > 0.0f ? paged_decode_kernel<D, T, true> : paged_decode_kernel<D, T, false>;
+  ARGUS_HIP_CHECK(ctx, argus_raise_lds_limit(ctx, kern, (int)lds));
+  hipLaunchKernelGGL(kern, dim3((unsigned)(items * p.heads_kv)), dim3(64 * kWaves), lds, stream, p);
+  ARGUS_HIP_CHECK(ctx, hipGetLastError());
+  return ARGUS_HIP_OK;
+}
+
+}  // namespace
+
+int launch_paged_decode(argus_hip_ctx *ctx, const PagedParams &p, int D, bool f32, int items, hipStream_t stream) {
+  switch (D) {
+    case 64: return f32 ? launch<64, float>(ctx, p, items, stream) : launch<64, _Float16>(ctx, p, items, stream);
+    case 128: return f32 ? launch<128, float>(ctx, p, items, stream) : launch<128, _Float16>(ctx, p, items, stream);
+    default: return f32 ? launch<256, float>(ctx, p, items, stream) : launch<256, _Float16>(ctx, p, items, stream);
+  }
+}
+
+}  // namespace argus_paged
