@@ -7,6 +7,7 @@ missing, importing this module raises.
 """
 import ctypes as C
 import os
+import struct
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # ARGUS_HIP_LIB selects another build of the same library (profiling / A-B runs).
@@ -397,9 +398,15 @@ def _ptr(t):
     return 0 if t is None else t.data_ptr()
 
 
-def _stream(device=None):
+def _stream():
     import torch
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch.cuda.current_stream().cuda_stream
+
+
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)  # current_stream(device) without the object around it
+if _raw_stream is None:
+    def _raw_stream(device):
+        return torch.cuda.current_stream(device).cuda_stream
 
 
 def _kv_dtype(t):
@@ -411,39 +418,75 @@ def _kv_dtype(t):
     raise TypeError("unsupported KV dtype %s" % t.dtype)
 
 
-def _int32(what, *tensors):
-    """Tables and lengths cross the ABI as packed device int32."""
-    import torch
+class _Call:
+    """An entry point taking (context, const struct *): the struct's values are packed in field order with
+    the C compiler's alignment, which costs a fraction of filling a ctypes structure."""
+
+    def __init__(self, name, cls):
+        codes = {C.c_void_p: "P", C.c_size_t: "N", C.c_int64: "q", C.c_int32: "i", C.c_float: "f"}
+        self.pack = struct.Struct("@" + "".join(codes[t] for _, t in cls._fields_) + "0P").pack
+        self.fn = lib[name]  # a function object of its own
+        self.fn.argtypes, self.fn.restype = [C.c_void_p, C.c_char_p], C.c_int64 if name.endswith("_workspace") else C.c_int
+
+    def __call__(self, handle, *values):
+        return self.fn(handle, self.pack(*values))
+
+
+_page_plan = _Call("argus_hip_page_plan", PagePlanArgs)
+_qk_norm_rope = _Call("argus_hip_qk_norm_rope", QkNormRopeArgs)
+_paged_attention = _Call("argus_hip_paged_attention", PagedAttentionArgs)
+_paged_attention_workspace = _Call("argus_hip_paged_attention_workspace", PagedAttentionArgs)
+
+
+def _refuse(what, device, t, dtype):
+    """Why `t` cannot cross the ABI; a pointer to other memory would reach the kernels unchecked."""
+    if t.get_device() != device:
+        raise ValueError("%s: every tensor lies on the context's device (cuda:%d)" % (what, device))
+    if t.dtype != dtype:
+        raise TypeError("%s: expected a tensor of %s, got %s" % (what, dtype, t.dtype))
+    raise ValueError(what + ": lengths, tables, weights, pools and workspaces are contiguous")
+
+
+def _packed(what, device, dtype, *tensors):
+    """Their addresses (0 for None): contiguous tensors of one dtype on the context's device."""
+    found = []
     for t in tensors:
-        if t is not None and (t.dtype != torch.int32 or not t.is_contiguous()):
-            raise TypeError(what + ": lengths, tables, positions and slots are contiguous int32 tensors")
+        if t is None:
+            found.append(0)
+            continue
+        if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
+            _refuse(what, device, t, dtype)
+        found.append(t.data_ptr())
+    return found
 
 
-def _on_device(what, device, *tensors):
-    """A pointer to other memory would reach the kernels unchecked."""
-    for t in tensors:
-        if t is not None and (not t.is_cuda or t.device.index != device):
-            raise ValueError("%s: every tensor lies on the context's device (cuda:%d)" % (what, device))
+def _heads(what, device, dtype, heads, d, t):
+    """(address, elements between tokens) of [tokens, heads, d] with packed heads."""
+    if t.dtype is not dtype or t.get_device() != device:
+        _refuse(what, device, t, dtype)
+    token, head, one = t.stride()
+    if (one != 1 and d > 1) or (head != d and heads > 1):
+        raise ValueError(what + ": the heads of a token must be packed")
+    return t.data_ptr(), token if t.shape[0] > 1 else heads * d
 
 
-def _token_stride(t):
-    """Elements between the tokens of [tokens, heads, d], whose heads are packed."""
-    if t.stride(2) != 1 or (t.shape[1] > 1 and t.stride(1) != t.shape[2]):
-        raise ValueError("the heads of a token must be packed")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1] * t.shape[2]
-
-
-def _pool(what, k, v, layout, hkv, d):
-    """(n_pages, page_size) of a pair of page pools."""
-    import torch
-    if k.dtype != torch.float16 or v.dtype != torch.float16:
-        raise TypeError(what + ": page pools are float16")
-    if k.dim() != 4 or k.shape != v.shape or not k.is_contiguous() or not v.is_contiguous():
-        raise ValueError(what + ": page pools are contiguous tensors of one shape")
-    n, heads, size = (k.shape[0], k.shape[1], k.shape[2]) if layout == HEAD_MAJOR else (k.shape[0], k.shape[2], k.shape[1])
-    if heads != hkv or k.shape[3] != d:
+def _pool(what, device, k, v, layout, hkv, d):
+    """(addresses, n_pages, page_size) of a pair of page pools."""
+    n, a, b, e = k.shape
+    heads, size = (a, b) if layout == HEAD_MAJOR else (b, a)
+    if k.shape != v.shape or e != d or (hkv is not None and heads != hkv):
         raise ValueError(what + ": the pools belong to other heads")
-    return n, size
+    return _packed(what, device, torch.float16, k, v), n, heads, size
+
+
+_FLOATS = {torch.float32: F32, torch.float16: F16}
+
+
+def _float(what, t):
+    code = _FLOATS.get(t.dtype)
+    if code is None:
+        raise TypeError("%s: dtype %s is not float32 or float16" % (what, t.dtype))
+    return code
 
 
 class Context:
@@ -710,82 +753,67 @@ class Context:
                   check=True):
         """Device int32 tensors: past_len, new_len, kv_len [n], free_pages [f], page_table [n, c] (in place), cu_new [n + 1],
         positions and slots [token_capacity], counts [3]."""
-        _int32("page_plan", past_len, new_len, free_pages, page_table, cu_new, kv_len, positions, slots, counts)
-        _on_device("page_plan", self.device, past_len, new_len, free_pages, page_table, cu_new, kv_len, positions, slots, counts)
-        n = past_len.numel()
-        if (new_len.numel() != n or kv_len.numel() != n or cu_new.numel() != n + 1 or counts.numel() != 3 or page_table.dim() != 2
-                or page_table.shape[0] != n or slots.numel() != positions.numel()):
+        dev = self.device
+        ptrs = _packed("page_plan", dev, torch.int32, past_len, new_len, free_pages, page_table, cu_new, kv_len, positions, slots, counts)
+        n, tokens = past_len.numel(), positions.numel()
+        rows, width = page_table.shape
+        if (new_len.numel() != n or kv_len.numel() != n or cu_new.numel() != n + 1 or counts.numel() != 3 or rows != n
+                or slots.numel() != tokens):
             raise ValueError("page_plan: shapes do not belong together")
-        a = PagePlanArgs(stream=_stream(self.device), past_len=_ptr(past_len), new_len=_ptr(new_len), free_pages=_ptr(free_pages),
-                         page_table=_ptr(page_table), cu_new=_ptr(cu_new), kv_len=_ptr(kv_len), positions=_ptr(positions),
-                         slots=_ptr(slots), counts=_ptr(counts), n_seqs=n,
-                         n_free=0 if free_pages is None else free_pages.numel(), n_pages=n_pages, page_size=page_size,
-                         table_stride=page_table.shape[1], token_capacity=positions.numel())
-        return self._check(lib.argus_hip_page_plan(self.handle, C.byref(a)), check)
+        return self._check(_page_plan(self.handle, _raw_stream(dev), *ptrs, n, 0 if free_pages is None else free_pages.numel(), n_pages,
+                                      page_size, width, tokens), check)
 
     def qk_norm_rope(self, q, k, v, positions, cos_sin, q_out, k_cache, v_cache, slots, q_weight=None, k_weight=None, eps=1e-6,
                      weight_bias=0.0, interleaved=False, layout=HEAD_MAJOR, check=True):
         """q [t, Hq, d], k / v [t, Hkv, d] (heads packed, any token stride), q_out [t, Hq, d]; pools as in
         argus_hip.h; cos_sin [n_positions, rot_dim] F32 or None (no rotation); positions, slots [t] int32."""
-        import torch
-        _int32("qk_norm_rope", positions, slots)
+        what, dev, ty = "qk_norm_rope", self.device, q.dtype
+        in_dtype, out_dtype = _float(what, q), _float(what, q_out)
         t, hq, d = q.shape
         hkv = k.shape[1]
-        n_pages, page_size = _pool("qk_norm_rope", k_cache, v_cache, layout, hkv, d)
-        if (k.shape != (t, hkv, d) or v.shape != k.shape or q_out.shape != q.shape or slots.numel() != t
-                or (positions is not None and positions.numel() != t)):
+        pools, n_pages, _, page_size = _pool(what, dev, k_cache, v_cache, layout, hkv, d)
+        if k.shape != (t, hkv, d) or v.shape != k.shape or q_out.shape != q.shape:
             raise ValueError("qk_norm_rope: shapes do not belong together")
-        if k.dtype != q.dtype or v.dtype != q.dtype:
-            raise TypeError("qk_norm_rope: q, k and v have one dtype")
-        for w in (q_weight, k_weight, cos_sin):
-            if w is not None and (w.dtype != torch.float32 or not w.is_contiguous()):
-                raise TypeError("qk_norm_rope: weights and cos_sin are contiguous float32")
-        for w in (q_weight, k_weight):
-            if w is not None and w.numel() != d:
-                raise ValueError("qk_norm_rope: a weight has head_dim elements")
-        if cos_sin is not None and (cos_sin.dim() != 2 or positions is None):
-            raise ValueError("qk_norm_rope: cos_sin is [n_positions, rot_dim] and needs positions")
-        _on_device("qk_norm_rope", self.device, q, k, v, positions, cos_sin, q_out, k_cache, v_cache, slots, q_weight, k_weight)
-        a = QkNormRopeArgs(stream=_stream(self.device), q=_ptr(q), k=_ptr(k), v=_ptr(v), q_weight=_ptr(q_weight), k_weight=_ptr(k_weight),
-                           cos_sin=_ptr(cos_sin), positions=_ptr(positions), slots=_ptr(slots), q_out=_ptr(q_out),
-                           k_cache=_ptr(k_cache), v_cache=_ptr(v_cache), q_stride=_token_stride(q), k_stride=_token_stride(k),
-                           v_stride=_token_stride(v), q_out_stride=_token_stride(q_out), tokens=t, heads_q=hq, heads_kv=hkv,
-                           head_dim=d, rot_dim=0 if cos_sin is None else cos_sin.shape[1], interleaved=int(interleaved),
-                           n_positions=0 if cos_sin is None else cos_sin.shape[0], n_pages=n_pages, page_size=page_size,
-                           layout=layout, in_dtype=_kv_dtype(q), out_dtype=_kv_dtype(q_out), eps=eps, weight_bias=weight_bias)
-        return self._check(lib.argus_hip_qk_norm_rope(self.handle, C.byref(a)), check)
+        (qp, qs), (kp, ks), (vp, vs) = _heads(what, dev, ty, hq, d, q), _heads(what, dev, ty, hkv, d, k), _heads(what, dev, ty, hkv, d, v)
+        op, os_ = _heads(what, dev, q_out.dtype, hq, d, q_out)
+        wq, wk, cs = _packed(what, dev, torch.float32, q_weight, k_weight, cos_sin)
+        pos, slot = _packed(what, dev, torch.int32, positions, slots)
+        if slots.numel() != t or (pos and positions.numel() != t):
+            raise ValueError("qk_norm_rope: one position and one slot per token")
+        if (wq and q_weight.numel() != d) or (wk and k_weight.numel() != d):
+            raise ValueError("qk_norm_rope: a weight has head_dim elements")
+        n_pos, rot = (0, 0) if cos_sin is None else cos_sin.shape
+        return self._check(_qk_norm_rope(
+            self.handle, _raw_stream(dev), qp, kp, vp, wq, wk, cs, pos, slot, op, pools[0], pools[1], qs, ks, vs, os_, t, hq, hkv, d, rot,
+            1 if interleaved else 0, n_pos, n_pages, page_size, layout, in_dtype, out_dtype, eps, weight_bias), check)
 
-    def _paged_args(self, q, k_cache, v_cache, page_table, cu_new, kv_len, out, max_new, max_kv, min_new, softcap, scale, window,
-                    layout, workspace):
-        _int32("paged_attention", page_table, cu_new, kv_len)
+    def _paged(self, fn, q, k_cache, v_cache, page_table, cu_new, kv_len, out, max_new, max_kv, min_new, softcap, scale, window, layout,
+               workspace, check):
+        what, dev = "paged_attention", self.device
+        dtype = _float(what, q)
         t, hq, d = q.shape
-        hkv = k_cache.shape[1] if layout == HEAD_MAJOR else k_cache.shape[2]
-        n_pages, page_size = _pool("paged_attention", k_cache, v_cache, layout, hkv, d)
+        pools, n_pages, hkv, page_size = _pool(what, dev, k_cache, v_cache, layout, None, d)
+        table, cu, kv = _packed(what, dev, torch.int32, page_table, cu_new, kv_len)
+        (qp, qs), (op, os_) = _heads(what, dev, q.dtype, hq, d, q), _heads(what, dev, q.dtype, hq, d, out)
         n = kv_len.numel()
-        if cu_new.numel() != n + 1 or page_table.dim() != 2 or page_table.shape[0] != n or out.shape != q.shape:
+        rows, width = page_table.shape
+        if cu_new.numel() != n + 1 or rows != n or out.shape != q.shape:
             raise ValueError("paged_attention: shapes do not belong together")
-        if out.dtype != q.dtype:
-            raise TypeError("paged_attention: q and out have one dtype")
-        _on_device("paged_attention", self.device, q, k_cache, v_cache, page_table, cu_new, kv_len, out, workspace)
-        return PagedAttentionArgs(
-            stream=_stream(self.device), q=_ptr(q), k_cache=_ptr(k_cache), v_cache=_ptr(v_cache), page_table=_ptr(page_table),
-            cu_new=_ptr(cu_new), kv_len=_ptr(kv_len), out=_ptr(out), workspace=_ptr(workspace),
-            workspace_bytes=0 if workspace is None else workspace.numel() * workspace.element_size(), q_stride=_token_stride(q),
-            out_stride=_token_stride(out), n_seqs=n, n_tokens=t, heads_q=hq, heads_kv=hkv, head_dim=d, n_pages=n_pages,
-            page_size=page_size, table_stride=page_table.shape[1], layout=layout, dtype=_kv_dtype(q), min_new=min_new,
-            max_new=max_new, max_kv=max_kv, window=window, softcap=softcap, scale=scale)
+        ws, ws_bytes = 0, 0
+        if workspace is not None:
+            (ws,), ws_bytes = _packed(what, dev, workspace.dtype, workspace), workspace.numel() * workspace.element_size()
+        return self._check(fn(self.handle, _raw_stream(dev), qp, pools[0], pools[1], table, cu, kv, op, ws, ws_bytes, qs, os_, n, t, hq, hkv,
+                              d, n_pages, page_size, width, layout, dtype, min_new, max_new, max_kv, window, softcap, scale), check)
 
     def paged_attention(self, q, k_cache, v_cache, page_table, cu_new, kv_len, out, max_new=0, max_kv=0, min_new=0, softcap=0.0,
                         scale=0.0, window=0, layout=HEAD_MAJOR, workspace=None, check=True):
         """q / out [n_tokens, Hq, d] (heads packed, any token stride); pools, tables and hints as in argus_hip.h.
         workspace: a device tensor of paged_attention_workspace() bytes (None: the context's)."""
-        a = self._paged_args(q, k_cache, v_cache, page_table, cu_new, kv_len, out, max_new, max_kv, min_new, softcap, scale, window,
-                             layout, workspace)
-        return self._check(lib.argus_hip_paged_attention(self.handle, C.byref(a)), check)
+        return self._paged(_paged_attention, q, k_cache, v_cache, page_table, cu_new, kv_len, out, max_new, max_kv, min_new, softcap, scale,
+                           window, layout, workspace, check)
 
     def paged_attention_workspace(self, q, k_cache, v_cache, page_table, cu_new, kv_len, out, max_new=0, max_kv=0, min_new=0,
                                   softcap=0.0, scale=0.0, window=0, layout=HEAD_MAJOR, check=True):
         """Bytes of workspace paged_attention needs for the same arguments."""
-        a = self._paged_args(q, k_cache, v_cache, page_table, cu_new, kv_len, out, max_new, max_kv, min_new, softcap, scale, window,
-                             layout, None)
-        return self._check(lib.argus_hip_paged_attention_workspace(self.handle, C.byref(a)), check)
+        return self._paged(_paged_attention_workspace, q, k_cache, v_cache, page_table, cu_new, kv_len, out, max_new, max_kv, min_new,
+                           softcap, scale, window, layout, None, check)

@@ -52,13 +52,34 @@ __global__ __launch_bounds__(256, (D <= 128 && std::is_same<T, _Float16>::value)
   _Float16 *const sK = smem, *const sV = smem + 2 * BN * KP;  // [2][BN][KP], [2][BN][VP]
   __shared__ int bad_tile[2];  // tile whose V held infinities or NaN under a mask
 
-  PagedItem it;
-  if (!sched_find<false>(p.sched, p.cu_new, p.kv_len, BN, blockIdx.x / p.heads_kv, it)) return;
-  if (it.nsplit > 1 && (uint32_t)(it.slot + it.split) >= (uint32_t)p.n_slots) return;
-  const int kvh = blockIdx.x % p.heads_kv;
+  const int kvh = blockIdx.x % p.heads_kv, w = blockIdx.x / p.heads_kv;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 31, hl = lane >> 5;
   const int G = p.sched.group;
+  const bool windowed = p.sched.window > 0;
+  const int window = p.sched.window;
+  const int page_mask = (1 << p.page_shift) - 1;
+  const uint32_t row_bytes = (uint32_t)p.pool.row * 2;
+  const int my_row = lane / (D / 8), my_col = lane % (D / 8);
+  const uint32_t lane_off = my_row * row_bytes + 16 * my_col;
+  const float c = p.scale * kLog2e;
+  const float inv_cap = CAP ? 1.0f / p.softcap : 0.0f;
+  // V^T operand: ds_read_b64_tr_b16 gives lane i of 16 channel ch0 + i of keys key0 .. key0 + 3 when lane s
+  // addresses V[key0 + s / 4][ch0 + 4 (s % 4)]; P^T holds keys 4 hl + {0..3} and 8 + 4 hl + {0..3} of 16
+  const int g16 = lane >> 4, s16 = lane & 15;
+  const int vlane_off = (4 * (g16 >> 1) + (s16 >> 2)) * VP + 16 * (g16 & 1) + 4 * (s16 & 3);
+
+  const PagedLine line(p.sched, p.cu_new, p.kv_len);
+  const bool whole = line.whole(p.sched);
+  int64_t x = whole ? w : w * line.share;
+  const int64_t x_end = whole ? std::min<int64_t>(line.tiles, x + 1) : std::min<int64_t>(line.work, x + line.share);
+  while (x < x_end) {  // the tiles this share touches
+  PagedPlace it;
+  if (!sched_find(p.sched, p.cu_new, p.kv_len, whole, x, it)) return;
+  const int64_t from = whole ? 0 : x - it.start, upto = whole ? it.cost : std::min<int64_t>(x_end - it.start, it.cost);
+  x = whole ? x_end : it.start + upto;
+  const bool entire = from == 0 && upto == it.cost;
+  const int slot = 2 * w + (from == 0 ? 1 : 0);
   const int n_rows = (int)std::min<int64_t>((int64_t)(it.s.q_end - it.s.q_begin) * G, 0x7fffffff);
   const int row0 = it.tile * kChunkRows;
   const int row_last = min(n_rows, row0 + kChunkRows) - 1;
@@ -69,20 +90,16 @@ __global__ __launch_bounds__(256, (D <= 128 && std::is_same<T, _Float16>::value)
   const int tok = rr / G, head = kvh * G + rr % G;
   const int pos = it.s.pos0 + tok;
   const int wg_first = it.s.pos0 + row0 / G, wg_last = it.s.pos0 + row_last / G;  // positions of the workgroup's rows
-  const bool windowed = p.sched.window > 0;
-  const int window = p.sched.window;
 
   // keys the tile's rows see, and this part of them
   const int key_end = min(it.s.len, max(wg_last, -1) + 1);
   const int key_begin = windowed && wg_first >= window ? (wg_first - window + 1) / BN * BN : 0;
   const int n_tiles = key_end > key_begin ? (key_end - key_begin + BN - 1) / BN : 0;
-  const int per = (n_tiles + it.nsplit - 1) / it.nsplit;
-  const int t0 = min(n_tiles, it.split * per), n_it = min(n_tiles, t0 + per) - t0;
+  const int t0 = (int)((double)from * n_tiles / it.cost), n_it = (int)((double)upto * n_tiles / it.cost) - t0;
   const int base0 = key_begin + t0 * BN;
 
   // ---- Q as the B operand: lane (row ln, half hl) holds channels 16 kk + 8 hl .. + 7
   half8_t qh[KK], ql[F32 ? KK : 1];
-  const float c = p.scale * kLog2e;
   {
     const T *qp = (const T *)p.q + (int64_t)(it.s.q_begin + tok) * p.q_stride + (int64_t)head * D + 8 * hl;
 #pragma unroll
@@ -101,15 +118,10 @@ __global__ __launch_bounds__(256, (D <= 128 && std::is_same<T, _Float16>::value)
       }
     }
   }
-  const float inv_cap = CAP ? 1.0f / p.softcap : 0.0f;
 
   // ---- tiles: piece i of a thread is 16 bytes of row (threadIdx + 256 i) / (D / 8) of the tile; the rows
   // one wave covers with a piece lie in one page
   PageWindow pages(p, it.seq, base0 >> p.page_shift, lane);
-  const int page_mask = (1 << p.page_shift) - 1;
-  const uint32_t row_bytes = (uint32_t)p.pool.row * 2;
-  const int my_row = lane / (D / 8), my_col = lane % (D / 8);
-  const uint32_t lane_off = my_row * row_bytes + 16 * my_col;
   half8_t kpre[CH], vpre[CH];
   auto fetch = [&](const _Float16 *pool, int base, half8_t(&pre)[CH]) {
 #pragma unroll
@@ -153,11 +165,6 @@ __global__ __launch_bounds__(256, (D <= 128 && std::is_same<T, _Float16>::value)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o_acc[r][i] = 0.0f;
   float m_run = kNegInf, l_run = 0.0f;
-
-  // V^T operand: ds_read_b64_tr_b16 gives lane i of 16 channel ch0 + i of keys key0 .. key0 + 3 when lane s
-  // addresses V[key0 + s / 4][ch0 + 4 (s % 4)]; P^T holds keys 4 hl + {0..3} and 8 + 4 hl + {0..3} of 16
-  const int g16 = lane >> 4, s16 = lane & 15;
-  const int vlane_off = (4 * (g16 >> 1) + (s16 >> 2)) * VP + 16 * (g16 & 1) + 4 * (s16 & 3);
 
   if (threadIdx.x < 2) bad_tile[threadIdx.x] = -1;
   if (n_it > 0) {
@@ -265,9 +272,9 @@ __global__ __launch_bounds__(256, (D <= 128 && std::is_same<T, _Float16>::value)
   }
 
   l_run += __shfl_xor(l_run, 32, 64);
-  if (it.nsplit > 1) {
-    const int64_t at = ((int64_t)(it.slot + it.split) * p.heads_kv + kvh) * kChunkRows + 32 * wave + ln;
+  if (!entire) {
     if (row_ok) {
+      const int64_t at = ((int64_t)slot * p.heads_kv + kvh) * kChunkRows + 32 * wave + ln;
       float *o = p.ws_o + at * D;
 #pragma unroll
       for (int r = 0; r < RB; ++r)
@@ -279,9 +286,7 @@ __global__ __launch_bounds__(256, (D <= 128 && std::is_same<T, _Float16>::value)
         p.ws_ml[at * 2 + 1] = l_run;
       }
     }
-    return;
-  }
-  if (row_ok) {
+  } else if (row_ok) {
     const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
     T *out = (T *)p.out + (int64_t)(it.s.q_begin + tok) * p.out_stride + (int64_t)head * D;
 #pragma unroll
@@ -295,35 +300,44 @@ __global__ __launch_bounds__(256, (D <= 128 && std::is_same<T, _Float16>::value)
         *(T4 *)(out + 32 * r + 8 * i4 + 4 * hl) = o;
       }
   }
+  }
 }
 
 // Merge of the parts of cut tiles: row m of a tile is sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m), in the
-// order of the parts.  D / 4 threads share a row.
+// order of the parts.  The end of share b - 1 cuts at most one tile; of a tile cut more than once the
+// first cut's workgroups do the merge.  D / 4 threads share a row.
 template <int D, typename T>
-__global__ __launch_bounds__(256) void paged_combine_kernel(const PagedParams p, int align) {
+__global__ __launch_bounds__(256) void paged_combine_kernel(const PagedParams p) {
   constexpr int RPB = 256 / (D / 4);
   const int R = p.sched.tile_rows, chunks = (R + RPB - 1) / RPB;
-  const int x = blockIdx.x / chunks, kvh = x % p.heads_kv;
-  PagedItem it;
-  if (!sched_find<true>(p.sched, p.cu_new, p.kv_len, align, x / p.heads_kv, it)) return;
-  if (it.slot < 0 || (int64_t)it.slot + it.nsplit > p.n_slots) return;
+  const int b = blockIdx.x / (chunks * p.heads_kv) + 1, kvh = blockIdx.x / chunks % p.heads_kv;
+  const PagedLine line(p.sched, p.cu_new, p.kv_len);
+  if (line.whole(p.sched) || b * line.share >= line.work) return;
+  PagedPlace it;
+  if (!sched_find(p.sched, p.cu_new, p.kv_len, false, b * line.share, it)) return;
+  if (it.start == b * line.share || it.start < (b - 1) * line.share) return;  // not cut here, or cut before
+  const int last = (int)((it.start + it.cost - 1) / line.share);               // the share the tile ends in
   const int G = p.sched.group;
   const int lr = blockIdx.x % chunks * RPB + threadIdx.x / (D / 4), ch = threadIdx.x % (D / 4) * 4;
   const int64_t row = (int64_t)it.tile * R + lr;
   if (lr >= R || row >= (int64_t)(it.s.q_end - it.s.q_begin) * G) return;
-  const int64_t step = (int64_t)p.heads_kv * R, at = (int64_t)it.slot * step + (int64_t)kvh * R + lr;
+  // parts: slot 2 (b - 1) + 1, then 2 b, 2 (b + 1), .. 2 last
+  const int64_t step = (int64_t)p.heads_kv * R, row_at = (int64_t)kvh * R + lr;
+  auto part = [&](int i) { return (int64_t)(i == 0 ? 2 * b - 1 : 2 * (b + i - 1)) * step + row_at; };
+  const int n = last - b + 2;
   float m = kNegInf;
-  for (int i = 0; i < it.nsplit; ++i) m = fmaxf(m, p.ws_ml[(at + i * step) * 2]);
+  for (int i = 0; i < n; ++i) m = fmaxf(m, p.ws_ml[part(i) * 2]);
   const float m_ref = m == kNegInf ? 0.0f : m;
   float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
   float l = 0.0f;
 #pragma unroll 4
-  for (int i = 0; i < it.nsplit; ++i) {
-    const float f = __builtin_amdgcn_exp2f(p.ws_ml[(at + i * step) * 2] - m_ref);
-    l += p.ws_ml[(at + i * step) * 2 + 1] * f;
-    const float4_t part = *(const float4_t *)(p.ws_o + (at + i * step) * D + ch);
+  for (int i = 0; i < n; ++i) {
+    const int64_t at = part(i);
+    const float f = __builtin_amdgcn_exp2f(p.ws_ml[at * 2] - m_ref);
+    l += p.ws_ml[at * 2 + 1] * f;
+    const float4_t x = *(const float4_t *)(p.ws_o + at * D + ch);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] += part[e] * f;
+    for (int e = 0; e < 4; ++e) o[e] += x[e] * f;
   }
   T *out = (T *)p.out + (int64_t)(it.s.q_begin + row / G) * p.out_stride + (int64_t)(kvh * G + row % G) * D + ch;
 #pragma unroll
@@ -343,13 +357,14 @@ int launch_chunk(argus_hip_ctx *ctx, const PagedParams &p, int items, hipStream_
 struct CallPlan {
   bool decode, chunk;
   PagedSched ds, cs;
-  int64_t d_items, c_items, d_cut, c_cut, d_slots, c_slots;
-  int64_t ws_floats;  // [decode ml][decode o][chunk ml][chunk o]
+  int64_t d_items, c_items, d_slots, c_slots;
+  int64_t ws_floats;  // [decode o][decode ml][chunk o][chunk ml]
 };
 
 int make_plan(argus_hip_ctx *ctx, int compute_units, const argus_hip_paged_attention_args *a, CallPlan &pl) {
   const int G = a->heads_q / a->heads_kv, d = a->head_dim;
   const int64_t room = std::min<int64_t>((int64_t)a->table_stride * a->page_size, 0x7fffffff - 4096);
+  const int64_t longest = a->max_kv > 0 ? std::min<int64_t>(a->max_kv, room) : room;
   PagedSched s{};
   s.n_seqs = a->n_seqs;
   s.n_tokens = a->n_tokens;
@@ -359,38 +374,37 @@ int make_plan(argus_hip_ctx *ctx, int compute_units, const argus_hip_paged_atten
   pl = CallPlan{};
   pl.decode = G <= kDecodeRows && (int64_t)a->min_new * G <= kDecodeRows;
   pl.chunk = !pl.decode || a->max_new == 0 || (int64_t)a->max_new * G > kDecodeRows;
-  const int64_t longest = a->max_kv > 0 ? std::min<int64_t>(a->max_kv, room) : room;
   if (pl.decode) {
-    pl.ds = s;
-    pl.ds.rows_over = 0;
-    pl.ds.rows_upto = kDecodeRows;
-    pl.ds.tile_rows = kDecodeRows;
-    pl.ds.unit = 4 * decode_align(d);
-    pl.ds.min_units = 2;
-    pl.ds.target = std::max(1, compute_units * 3 / a->heads_kv);
-    pl.ds.max_splits = (int)std::min<int64_t>(128, std::max<int64_t>(1, (longest + pl.ds.unit - 1) / pl.ds.unit / pl.ds.min_units));
-    const int64_t tiles = std::min<int64_t>(a->n_seqs, a->n_tokens);
-    pl.d_items = sched_items_bound(pl.ds, tiles);
-    pl.d_slots = sched_slots_bound(pl.ds, tiles);
-    pl.d_cut = sched_cut_tiles_bound(pl.ds, tiles);
+    PagedSched &c = pl.ds = s;
+    c.rows_upto = c.tile_rows = kDecodeRows;
+    c.align = decode_align(d);
+    c.unit = 4 * c.align;
+    c.min_share = 2;
+    c.whole_from = 0x7fffffff;
+    // resident workgroups, and no more shares than the longest lengths make
+    const int64_t tiles = sched_tiles_bound(c, a->min_new);
+    const int64_t most = tiles * std::max<int64_t>(1, (longest + 2 * c.align) / c.unit + 1);
+    c.target = (int)std::min<int64_t>(std::max(1, compute_units * 2 / a->heads_kv), std::max<int64_t>(1, most / c.min_share));
+    pl.d_items = c.target;
+    pl.d_slots = c.target > 1 ? sched_slots_bound(c) : 0;
   }
   if (pl.chunk) {
-    pl.cs = s;
-    pl.cs.rows_over = pl.decode ? kDecodeRows : 0;
-    pl.cs.rows_upto = 0x7fffffff;
-    pl.cs.tile_rows = kChunkRows;
-    pl.cs.unit = 128;
-    pl.cs.min_units = 4;
-    pl.cs.target = std::max(1, compute_units * 2 / a->heads_kv);
-    pl.cs.max_splits = (int)std::min<int64_t>(64, std::max<int64_t>(1, (longest + pl.cs.unit - 1) / pl.cs.unit / pl.cs.min_units));
-    const int64_t tiles = sched_tiles_bound(pl.cs, a->min_new);
-    if (tiles == 0) pl.chunk = false;  // too few rows for any request of this class
-    pl.c_items = tiles ? sched_items_bound(pl.cs, tiles) : 0;
-    pl.c_slots = sched_slots_bound(pl.cs, tiles);
-    pl.c_cut = sched_cut_tiles_bound(pl.cs, tiles);
+    PagedSched &c = pl.cs = s;
+    c.rows_over = pl.decode ? kDecodeRows : 0;
+    c.rows_upto = 0x7fffffff;
+    c.tile_rows = kChunkRows;
+    c.align = chunk_align(d);
+    c.min_share = 512;
+    const int64_t tiles = sched_tiles_bound(c, a->min_new);
+    c.target = std::max(1, compute_units * 2 / a->heads_kv);
+    c.whole_from = 4 * c.target;
+    if (longest + 96 <= c.min_share / 2) c.whole_from = 0;  // tiles too short to be cut
+    if (tiles == 0) pl.chunk = false;                       // too few rows for any request of this class
+    pl.c_items = sched_items_bound(c, tiles);
+    pl.c_slots = c.whole_from > 0 && pl.chunk ? sched_slots_bound(c) : 0;
   }
   constexpr int64_t kGrid = 0x7fffffff;
-  if (pl.d_items * a->heads_kv > kGrid || pl.c_items * a->heads_kv > kGrid)
+  if (pl.c_items * a->heads_kv > kGrid)
     return argus_fail(ctx, ARGUS_HIP_ERR_UNSUPPORTED, "paged_attention: %d rows are too many for one call", a->n_tokens);
   pl.ws_floats = (pl.d_slots * kDecodeRows + pl.c_slots * kChunkRows) * a->heads_kv * (d + 2);
   return ARGUS_HIP_OK;
@@ -431,12 +445,12 @@ int launch_paged_chunk(argus_hip_ctx *ctx, const PagedParams &p, int D, bool f32
   }
 }
 
-int launch_paged_combine(argus_hip_ctx *ctx, const PagedParams &p, int D, bool f32, int align, int tiles, hipStream_t stream) {
-  const int rpb = 256 / (D / 4), chunks = (p.sched.tile_rows + rpb - 1) / rpb;
+int launch_paged_combine(argus_hip_ctx *ctx, const PagedParams &p, int D, bool f32, hipStream_t stream) {
+  const int rpb = 256 / (D / 4), chunks = (p.sched.tile_rows + rpb - 1) / rpb, cuts = p.sched.target - 1;
   auto kern = D == 64 ? (f32 ? paged_combine_kernel<64, float> : paged_combine_kernel<64, _Float16>)
               : D == 128 ? (f32 ? paged_combine_kernel<128, float> : paged_combine_kernel<128, _Float16>)
                          : (f32 ? paged_combine_kernel<256, float> : paged_combine_kernel<256, _Float16>);
-  hipLaunchKernelGGL(kern, dim3((unsigned)(tiles * p.heads_kv * chunks)), dim3(256), 0, stream, p, align);
+  hipLaunchKernelGGL(kern, dim3((unsigned)(cuts * p.heads_kv * chunks)), dim3(256), 0, stream, p);
   ARGUS_HIP_CHECK(ctx, hipGetLastError());
   return ARGUS_HIP_OK;
 }
@@ -496,23 +510,21 @@ ARGUS_API int argus_hip_paged_attention(argus_hip_ctx *ctx, const argus_hip_page
   KernelTimer timer(ctx, stream);
   if (pl.decode) {
     p.sched = pl.ds;
-    p.n_slots = (int)pl.d_slots;
     p.ws_o = ws;  // output rows first: they are read and written 16 bytes at a time
     p.ws_ml = ws + pl.d_slots * kDecodeRows * a->heads_kv * d;
     rc = launch_paged_decode(ctx, p, d, f32, (int)pl.d_items, stream);
     if (rc == ARGUS_HIP_OK && !pl.chunk) timer.mark();
-    if (rc == ARGUS_HIP_OK && pl.d_cut) rc = launch_paged_combine(ctx, p, d, f32, decode_align(d), (int)pl.d_cut, stream);
+    if (rc == ARGUS_HIP_OK && pl.d_slots) rc = launch_paged_combine(ctx, p, d, f32, stream);
     if (rc != ARGUS_HIP_OK) return rc;
     if (ws) ws += pl.d_slots * kDecodeRows * a->heads_kv * (d + 2);
   }
   if (pl.chunk) {
     p.sched = pl.cs;
-    p.n_slots = (int)pl.c_slots;
     p.ws_o = ws;
     p.ws_ml = ws + pl.c_slots * kChunkRows * a->heads_kv * d;
     rc = launch_paged_chunk(ctx, p, d, f32, (int)pl.c_items, stream);
     timer.mark();
-    if (rc == ARGUS_HIP_OK && pl.c_cut) rc = launch_paged_combine(ctx, p, d, f32, chunk_align(d), (int)pl.c_cut, stream);
+    if (rc == ARGUS_HIP_OK && pl.c_slots) rc = launch_paged_combine(ctx, p, d, f32, stream);
   }
   return rc;
 }

@@ -40,12 +40,13 @@ struct PagedParams {
   const _Float16 *k, *v;
   const int32_t *page_table, *cu_new, *kv_len;
   void *out;
+  // Partial results of tiles that are cut: slot 2 w for the end of a tile begun before share w, 2 w + 1 for
+  // the begin of one that ends behind it.
   float *ws_ml;  // [slots, Hkv, tile_rows, 2]: running maximum (log2 units) and sum of a part's rows
   float *ws_o;   // [slots, Hkv, tile_rows, D]: un-normalised output rows
   int64_t q_stride, out_stride;
   PoolStrides pool;  // elements
   PagedSched sched;
-  int32_t n_slots;
   int32_t heads_kv, n_pages, page_shift, table_stride;
   float scale, softcap;
 };
@@ -56,7 +57,7 @@ constexpr int kChunkRows = 128;  // rows per workgroup of the chunk kernel
 
 int launch_paged_decode(argus_hip_ctx *ctx, const PagedParams &p, int D, bool f32, int items, hipStream_t stream);
 int launch_paged_chunk(argus_hip_ctx *ctx, const PagedParams &p, int D, bool f32, int items, hipStream_t stream);
-int launch_paged_combine(argus_hip_ctx *ctx, const PagedParams &p, int D, bool f32, int align, int tiles, hipStream_t stream);
+int launch_paged_combine(argus_hip_ctx *ctx, const PagedParams &p, int D, bool f32, hipStream_t stream);
 constexpr int decode_align(int D) { return D <= 128 ? 32 : 16; }   // keys per wave step of the decode kernel
 constexpr int chunk_align(int D) { return D <= 64 ? 64 : 32; }     // keys per tile of the chunk kernel
 

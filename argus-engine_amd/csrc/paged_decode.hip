@@ -51,30 +51,39 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(const PagedPa
   typedef typename std::conditional<VC == 8, half8_t, half4_t>::type vpiece_t;
   constexpr float kLog2e = 1.4426950408889634f;
 
-  PagedItem it;
-  if (!sched_find<false>(p.sched, p.cu_new, p.kv_len, STEP, blockIdx.x / p.heads_kv, it)) return;
-  if (it.nsplit > 1 && (uint32_t)(it.slot + it.split) >= (uint32_t)p.n_slots) return;
-  const int kvh = blockIdx.x % p.heads_kv;
+  const int kvh = blockIdx.x % p.heads_kv, w = blockIdx.x / p.heads_kv;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int j = lane >> 4, r = lane & 15;
   const int G = p.sched.group;
-  const int rows = (it.s.q_end - it.s.q_begin) * G;  // at most 16: one tile
+  const int window = p.sched.window > 0 ? p.sched.window : 0x7fffffff;
+  const int page_mask = (1 << p.page_shift) - 1;
+  const uint32_t row_bytes = (uint32_t)p.pool.row * 2;
+  const uint32_t k_lane = r * row_bytes + 16 * j, v_lane = 4 * j * row_bytes + 2 * VC * r;
+  const float c = p.scale * kLog2e;
+  const float inv_cap = CAP ? 1.0f / p.softcap : 0.0f;
+  __shared__ float lds_m[kWaves][16], lds_l[kWaves][16];
+  extern __shared__ __attribute__((aligned(16))) float lds_acc[];  // [kWaves][16][D + 4]
 
-  // keys of this part: whole units behind key_begin
-  const int64_t part = it.nsplit > 1 ? (sched_units(p.sched, it.s) + it.nsplit - 1) / it.nsplit * (int64_t)p.sched.unit : 0;
-  const int begin = (int)std::min<int64_t>(it.s.key_end, it.s.key_begin + it.split * part);
-  const int end = it.nsplit > 1 ? (int)std::min<int64_t>(it.s.key_end, begin + part) : it.s.key_end;
+  const PagedLine line(p.sched, p.cu_new, p.kv_len);
+  int64_t x = w * line.share;
+  const int64_t x_end = std::min<int64_t>(line.work, x + line.share);
+  while (x < x_end) {  // the requests this share touches
+  PagedPlace it;
+  if (!sched_find(p.sched, p.cu_new, p.kv_len, false, x, it)) return;
+  const int rows = (it.s.q_end - it.s.q_begin) * G;  // at most 16: one tile
+  const int64_t from = x - it.start, upto = std::min<int64_t>(x_end - it.start, it.cost);
+  x = it.start + upto;
+  const bool entire = from == 0 && upto == it.cost;
+  const int slot = 2 * w + (from == 0 ? 1 : 0);
+  const int begin = std::min<int64_t>(it.s.key_end, it.s.key_begin + from * p.sched.unit);
+  const int end = std::min<int64_t>(it.s.key_end, it.s.key_begin + upto * p.sched.unit);
 
   // row r: token r / G, head r % G; columns past the last row repeat it and are never stored
   const int rr = min(r, rows - 1);
   const int pos = it.s.pos0 + rr / G;
   const int pos_last = it.s.pos0 + (rows - 1) / G;
-  const int window = p.sched.window > 0 ? p.sched.window : 0x7fffffff;
 
   PageWindow pages(p, it.seq, begin >> p.page_shift, lane);
-  const int page_mask = (1 << p.page_shift) - 1;
-  const uint32_t row_bytes = (uint32_t)p.pool.row * 2;
-  const uint32_t k_lane = r * row_bytes + 16 * j, v_lane = 4 * j * row_bytes + 2 * VC * r;
   half8_t kr[TW][KK];
   vpiece_t vr[TW][VSEG][4];
   // the page of 16 keys from `key` on, ended at this part's last key (behind it: no rows at all), and the
@@ -111,7 +120,6 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(const PagedPa
 
   // Q: lane (j, r) holds chunk 4 kk + j of row r
   half8_t qh[KK], ql[F32 ? KK : 1];
-  const float c = p.scale * kLog2e;
   {
     const T *qp = (const T *)p.q + (int64_t)(it.s.q_begin + rr / G) * p.q_stride + (int64_t)(kvh * G + rr % G) * D;
 #pragma unroll
@@ -133,7 +141,6 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(const PagedPa
       }
     }
   }
-  const float inv_cap = CAP ? 1.0f / p.softcap : 0.0f;
 
   float4_t o_acc[NACC];
 #pragma unroll
@@ -276,8 +283,6 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(const PagedPa
   // ---- merge: lane groups (row sum), then the waves through LDS -----------------------------------
   l_run += __shfl_xor(l_run, 16, 64);
   l_run += __shfl_xor(l_run, 32, 64);
-  __shared__ float lds_m[kWaves][16], lds_l[kWaves][16];
-  extern __shared__ __attribute__((aligned(16))) float lds_acc[];  // [kWaves][16][D + 4]
   if (j == 0) {
     lds_m[wave][r] = m_run;
     lds_l[wave][r] = l_run;
@@ -290,30 +295,32 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(const PagedPa
       for (int i = 0; i < 4; ++i)
         if (4 * j + i < rows) lds_acc[(wave * 16 + 4 * j + i) * (D + 4) + 16 * VC * sg + VC * r + ch] = o_acc[sg * VC + ch][i];
   __syncthreads();
-  for (int x = threadIdx.x; x < rows * D; x += 64 * kWaves) {
-    const int row = x / D, ch = x % D;
+  for (int i = threadIdx.x; i < rows * D; i += 64 * kWaves) {
+    const int row = i / D, ch = i % D;
     float mm = lds_m[0][row];
 #pragma unroll
-    for (int w = 1; w < kWaves; ++w) mm = fmaxf(mm, lds_m[w][row]);
+    for (int v = 1; v < kWaves; ++v) mm = fmaxf(mm, lds_m[v][row]);
     const float m_ref = mm == kNegInf ? 0.0f : mm;
     float o = 0.0f, l = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float f = __builtin_amdgcn_exp2f(lds_m[w][row] - m_ref);
-      o += lds_acc[(w * 16 + row) * (D + 4) + ch] * f;
-      l += lds_l[w][row] * f;
+    for (int v = 0; v < kWaves; ++v) {
+      const float f = __builtin_amdgcn_exp2f(lds_m[v][row] - m_ref);
+      o += lds_acc[(v * 16 + row) * (D + 4) + ch] * f;
+      l += lds_l[v][row] * f;
     }
-    if (it.nsplit == 1) {
+    if (entire) {
       T *out = (T *)p.out + (int64_t)(it.s.q_begin + row / G) * p.out_stride + (int64_t)(kvh * G + row % G) * D;
       out[ch] = (T)(l == 0.0f ? 0.0f : o / l);
     } else {
-      const int64_t at = ((int64_t)(it.slot + it.split) * p.heads_kv + kvh) * kDecodeRows + row;
+      const int64_t at = ((int64_t)slot * p.heads_kv + kvh) * kDecodeRows + row;
       p.ws_o[at * D + ch] = o;
       if (ch == 0) {
         p.ws_ml[at * 2] = mm;
         p.ws_ml[at * 2 + 1] = l;
       }
     }
+  }
+  __syncthreads();  // the merge area is free for the next request
   }
 }
 
