@@ -30,23 +30,36 @@ __device__ __forceinline__ half4_t lds_read_tr16(const _Float16 *p) {
   return __builtin_bit_cast(half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t *)p));
 }
 
-template <int D>
+template <int D, bool F32>
 struct ChunkTile {
   static constexpr int BN = chunk_align(D);            // keys per tile
   static constexpr int KP = D + 8, VP = D + 32;        // row pitches (halfs): no bank is hit twice by one read
-  static constexpr int HALFS = BN * (KP + VP);
-  static constexpr int LDS_BYTES = 2 * HALFS * 2;      // two tile buffers
+  static constexpr int LDS_BYTES = 2 * BN * (KP + VP) * 2;  // two buffers each of K and V tiles
+  static constexpr bool DEEP = !F32 && D <= 128;       // tiles are requested a step earlier (registers allow a second set)
+  static constexpr int WAVES_PER_SIMD = D <= 128 ? 2 : 1;
 };
 
+// Software pipeline of a wave, as the logits of tile t + 1 are formed while tile t is exponentiated:
+//   phase A   S(t+1) = K . Q^T on the matrix cores  beside  the second half of tile t's exponentials
+//   phase B   O += V . P(t)                         beside  the first half of tile t + 1's
+// K tiles are staged in LDS two steps ahead, V tiles one; one barrier per step.  Interior steps -- every row
+// of the workgroup sees all of tiles t and t + 1 -- carry no masks and take no maximum: their exponents
+// stand against a reference some earlier tile of the row set, and a probability only leaves F16's range
+// where a logit exceeds it by 16 (log2), which shows in the row sum.
 template <int D, typename T, bool CAP>
-__global__ __launch_bounds__(256, (D <= 128 && std::is_same<T, _Float16>::value) ? 2 : 1) void paged_chunk_kernel(const PagedParams p) {
-  using TL = ChunkTile<D>;
+__global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::WAVES_PER_SIMD)) void paged_chunk_kernel(const PagedParams p) {
   constexpr bool F32 = std::is_same<T, float>::value;
+  using TL = ChunkTile<D, F32>;
   constexpr int BN = TL::BN, KP = TL::KP, VP = TL::VP;
-  constexpr int KK = D / 16, KB = BN / 32, RB = D / 32;
+  constexpr int KK = D / 16, KB = BN / 32, RB = D / 32, PS = BN / 16;  // logits MFMAs per 32 keys, row blocks of S^T and O^T, P^T slices
   constexpr int CH = BN * D / 8 / 256;  // 16-byte pieces of a K (or V) tile per thread
   constexpr int RPW = 64 / (D / 8);     // rows of a piece that one wave covers
+  constexpr bool DEEP = TL::DEEP;
+  constexpr int SETS = DEEP ? 2 : 1;
   constexpr float kLog2e = 1.4426950408889634f;
+  constexpr int kSplit = PS / 2;        // slices of P^T formed in phase B of the step before
+  constexpr int kAhead = 4, kVAhead = D <= 64 ? 4 : 3;  // operand reads kept in flight
+  constexpr int kPhaseValu = D <= 64 ? 5 : 4;           // vector-ALU instructions placed behind each MFMA
 
   extern __shared__ __attribute__((aligned(16))) _Float16 smem[];
   _Float16 *const sK = smem, *const sV = smem + 2 * BN * KP;  // [2][BN][KP], [2][BN][VP]
@@ -62,27 +75,27 @@ __global__ __launch_bounds__(256, (D <= 128 && std::is_same<T, _Float16>::value)
   const uint32_t row_bytes = (uint32_t)p.pool.row * 2;
   const int my_row = lane / (D / 8), my_col = lane % (D / 8);
   const uint32_t lane_off = my_row * row_bytes + 16 * my_col;
-  const float c = p.scale * kLog2e;
+  const PagePool k_pool(p.k, p, kvh, D), v_pool(p.v, p, kvh, D);
+  // exponents are logit * ce - m_ref; a negative scale turns the queries round instead
+  const float ce = CAP ? kLog2e : __builtin_fabsf(p.scale) * kLog2e;
+  const float q_sign = !CAP && p.scale < 0.0f ? -1.0f : 1.0f;
   const float inv_cap = CAP ? 1.0f / p.softcap : 0.0f;
   // V^T operand: ds_read_b64_tr_b16 gives lane i of 16 channel ch0 + i of keys key0 .. key0 + 3 when lane s
   // addresses V[key0 + s / 4][ch0 + 4 (s % 4)]; P^T holds keys 4 hl + {0..3} and 8 + 4 hl + {0..3} of 16
   const int g16 = lane >> 4, s16 = lane & 15;
   const int vlane_off = (4 * (g16 >> 1) + (s16 >> 2)) * VP + 16 * (g16 & 1) + 4 * (s16 & 3);
 
-  const PagedLine line(p.sched, p.cu_new, p.kv_len);
-  const bool whole = line.whole(p.sched);
-  int64_t x = whole ? w : w * line.share;
-  const int64_t x_end = whole ? std::min<int64_t>(line.tiles, x + 1) : std::min<int64_t>(line.work, x + line.share);
-  while (x < x_end) {  // the tiles this share touches
-  PagedPlace it;
-  if (!sched_find(p.sched, p.cu_new, p.kv_len, whole, x, it)) return;
-  const int64_t from = whole ? 0 : x - it.start, upto = whole ? it.cost : std::min<int64_t>(x_end - it.start, it.cost);
-  x = whole ? x_end : it.start + upto;
+  PagedCut cut{0, 0, 0, 0};
+  PagedShare work(p.sched, p.cu_new, p.kv_len, w);
+  while (work.found) {  // the tiles this share touches
+  const PagedPlace it = work.at;
+  const int64_t from = work.from(), upto = work.upto();
   const bool entire = from == 0 && upto == it.cost;
   const int slot = 2 * w + (from == 0 ? 1 : 0);
   const int n_rows = (int)std::min<int64_t>((int64_t)(it.s.q_end - it.s.q_begin) * G, 0x7fffffff);
   const int row0 = it.tile * kChunkRows;
   const int row_last = min(n_rows, row0 + kChunkRows) - 1;
+  if (!entire && from == 0) cut = PagedCut{(int)((it.start + it.cost - 1) / work.share) - w + 1, it.s.q_begin, row0, row_last + 1 - row0};
 
   const int row = row0 + 32 * wave + ln;
   const bool row_ok = row < n_rows;
@@ -97,10 +110,65 @@ __global__ __launch_bounds__(256, (D <= 128 && std::is_same<T, _Float16>::value)
   const int n_tiles = key_end > key_begin ? (key_end - key_begin + BN - 1) / BN : 0;
   const int t0 = (int)((double)from * n_tiles / it.cost), n_it = (int)((double)upto * n_tiles / it.cost) - t0;
   const int base0 = key_begin + t0 * BN;
+  const int part_end = min(key_end, base0 + n_it * BN);
+  // key tiles that every row sees whole
+  const int full_from = windowed && wg_last >= window ? max(0, (wg_last - window + BN - base0) / BN) : 0;
+  const int full_upto = min(n_it, max(0, min(wg_first + 1, key_end) - base0) / BN);
+
+  // ---- tiles: piece i of a thread is 16 bytes of row (threadIdx + 256 i) / (D / 8) of the tile; the rows
+  // one wave covers with a piece lie in one page
+  constexpr int SPAN = BN / 16;  // pages a tile touches at most
+  PageWindow pages;
+  pages.start<SPAN>(p, it.seq, base0 >> p.page_shift);
+  half8_t kpre[SETS][CH], vpre[SETS][CH];
+  uint64_t page_off[CH];  // of the K tile requested last; its V tile follows a step later
+  uint32_t row_off[CH];
+  auto fetch_k = [&](int t, half8_t(&pre)[CH]) {  // behind the part: its last page again
+    const int base = base0 + t * BN;
+    pages.advance<SPAN>(min(base, part_end - 1) >> p.page_shift);
+#pragma unroll
+    for (int i = 0; i < CH; ++i) {
+      const int key = base + wave * RPW + 4 * RPW * i;
+      page_off[i] = pages.offset(min(key, part_end - 1) >> p.page_shift);
+      row_off[i] = (uint32_t)(key & page_mask) * row_bytes;
+      pre[i] = __builtin_bit_cast(half8_t, __builtin_amdgcn_raw_buffer_load_b128(k_pool.rows(page_off[i]), lane_off, row_off[i], 0));
+    }
+  };
+  auto fetch_v = [&](half8_t(&pre)[CH]) {  // of the K tile requested last
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+      pre[i] = __builtin_bit_cast(half8_t, __builtin_amdgcn_raw_buffer_load_b128(v_pool.rows(page_off[i]), lane_off, row_off[i], 0));
+  };
+  const int stage_row = wave * RPW + my_row;
+  auto stage_k = [&](auto buf_c, half8_t(&pre)[CH]) {
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+      *(half8_t *)(sK + stage_row * KP + 8 * my_col + (decltype(buf_c)::value * BN + 4 * RPW * i) * KP) = pre[i];
+  };
+  auto stage_v = [&](auto buf_c, int t, half8_t(&pre)[CH], bool seen_whole) {  // tile t into buffer t % 2
+    if (!seen_whole) {
+      // A weight of zero does not keep an infinity or a NaN out of the product: such values of V leave the
+      // tile here and are added, by themselves, to the rows that see their key.
+      bool bad = false;
+#pragma unroll
+      for (int i = 0; i < CH; ++i)
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (not_finite(pre[i][e])) {
+            bad = true;
+            pre[i][e] = (_Float16)0.0f;
+          }
+      if (bad) bad_tile[decltype(buf_c)::value] = t;
+    }
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+      *(half8_t *)(sV + stage_row * VP + 8 * my_col + (decltype(buf_c)::value * BN + 4 * RPW * i) * VP) = pre[i];
+  };
+  auto seen_whole = [&](int t) { return t >= full_from && t < full_upto; };
 
   // ---- Q as the B operand: lane (row ln, half hl) holds channels 16 kk + 8 hl .. + 7
   half8_t qh[KK], ql[F32 ? KK : 1];
-  {
+  auto load_q = [&]() {
     const T *qp = (const T *)p.q + (int64_t)(it.s.q_begin + tok) * p.q_stride + (int64_t)head * D + 8 * hl;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
@@ -109,53 +177,14 @@ __global__ __launch_bounds__(256, (D <= 128 && std::is_same<T, _Float16>::value)
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           _Float16 hi, lo;
-          split_f16((e < 4 ? a[e] : b[e - 4]) * (CAP ? p.scale : c), hi, lo);
+          split_f16((e < 4 ? a[e] : b[e - 4]) * q_sign, hi, lo);
           qh[kk][e] = hi;
           ql[kk][e] = lo;
         }
       } else {
         qh[kk] = *(const half8_t *)(qp + 16 * kk);
+        if (q_sign < 0.0f) qh[kk] = -qh[kk];
       }
-    }
-  }
-
-  // ---- tiles: piece i of a thread is 16 bytes of row (threadIdx + 256 i) / (D / 8) of the tile; the rows
-  // one wave covers with a piece lie in one page
-  PageWindow pages(p, it.seq, base0 >> p.page_shift, lane);
-  half8_t kpre[CH], vpre[CH];
-  auto fetch = [&](const _Float16 *pool, int base, half8_t(&pre)[CH]) {
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const int key = base + wave * RPW + 4 * RPW * i;
-      const bool some = key < key_end;
-      const int page = (some ? key : key_end) >> p.page_shift;
-      const __amdgpu_buffer_rsrc_t rsrc =
-          page_rows(pool, p, pages.number(page), kvh, some ? min(key_end - (page << p.page_shift), page_mask + 1) : 0, D);
-      pre[i] = __builtin_bit_cast(half8_t, __builtin_amdgcn_raw_buffer_load_b128(rsrc, lane_off, some ? (uint32_t)(key & page_mask) * row_bytes : 0, 0));
-    }
-  };
-  // does some row of the workgroup not see some key of the tile?
-  auto edge_tile = [&](int base) { return base + BN - 1 > wg_first || base + BN > key_end || (windowed && base <= wg_last - window); };
-  auto stage = [&](int buf, int tile, int base) {
-    if (edge_tile(base)) {
-      // A weight of zero does not keep an infinity or a NaN out of the product: such values of V leave the
-      // tile here and are added, by themselves, to the rows that see their key.
-      bool bad = false;
-#pragma unroll
-      for (int i = 0; i < CH; ++i)
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (not_finite(vpre[i][e])) {
-            bad = true;
-            vpre[i][e] = (_Float16)0.0f;
-          }
-      if (bad) bad_tile[buf] = tile;
-    }
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const int key = wave * RPW + 4 * RPW * i + my_row;
-      *(half8_t *)(sK + (buf * BN + key) * KP + 8 * my_col) = kpre[i];
-      *(half8_t *)(sV + (buf * BN + key) * VP + 8 * my_col) = vpre[i];
     }
   };
 
@@ -164,82 +193,37 @@ __global__ __launch_bounds__(256, (D <= 128 && std::is_same<T, _Float16>::value)
   for (int r = 0; r < RB; ++r)
 #pragma unroll
     for (int i = 0; i < 16; ++i) o_acc[r][i] = 0.0f;
-  float m_run = kNegInf, l_run = 0.0f;
+  float m_run = kNegInf, m_ref = 0.0f, l_run = 0.0f;  // m_ref: what exponents stand against; m_run the same, -inf while no key was seen
 
-  if (threadIdx.x < 2) bad_tile[threadIdx.x] = -1;
-  if (n_it > 0) {
-    fetch(p.k, base0, kpre);
-    fetch(p.v, base0, vpre);
-  }
-  __syncthreads();
-  if (n_it > 0) stage(0, 0, base0);
-  __syncthreads();
-
-  for (int t = 0; t < n_it; ++t) {
-    const int base = base0 + t * BN, buf = t & 1;
-    pages.advance(base >> p.page_shift, lane);
-    if (t + 1 < n_it) {
-      fetch(p.k, base + BN, kpre);
-      fetch(p.v, base + BN, vpre);
-    }
-    float16_t s[KB];
-    const _Float16 *kt = sK + buf * BN * KP;
+  typedef float16_t STile[KB];
+  typedef half8_t PTile[PS];
+  // Instruction order of a phase, given once all of its code has been emitted: operand reads a few MFMAs
+  // ahead, and behind every MFMA some of the other tile's exponentials (a wave issues in order).
+  auto qk_tile = [&](auto buf_c, STile &s) {
+    const _Float16 *kt = sK + ln * KP + 8 * hl + decltype(buf_c)::value * BN * KP;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) {
-        const half8_t a = *(const half8_t *)(kt + (32 * kb + ln) * KP + 16 * kk + 8 * hl);
+        const half8_t a = *(const half8_t *)(kt + 32 * kb * KP + 16 * kk);
         s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[kk], kk == 0 ? float16_t{0.0f} : s[kb], 0, 0, 0);
         if constexpr (F32) s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[kk], s[kb], 0, 0, 0);
       }
-    const bool edge = edge_tile(base);
-    float mt = kNegInf;
+  };
+  auto sched_qk = [&](auto nv_c) {
+    constexpr int NV = decltype(nv_c)::value, N = KK * KB, AH = kAhead < N ? kAhead : N;
+    __builtin_amdgcn_sched_group_barrier(0x100, AH, 0);
 #pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        float x = s[kb][i];
-        if constexpr (CAP) x = soft_cap(F32 ? x : x * p.scale, p.softcap, inv_cap) * kLog2e;
-        else if constexpr (!F32) x *= c;
-        if (edge) {
-          const int key = base + 32 * kb + 8 * (i / 4) + 4 * hl + (i % 4);
-          if (key > pos || key >= key_end || (windowed && key <= pos - window)) x = kNegInf;
-        }
-        s[kb][i] = x;
-        mt = fmaxf(mt, x);
-      }
-    mt = xor32_combine(mt, [](float a, float b) { return fmaxf(a, b); });
-    const float m_new = fmaxf(m_run, mt);
-    const float m_ref = m_new == kNegInf ? 0.0f : m_new;
-    const float alpha = __builtin_amdgcn_exp2f(m_run - m_ref);
-    m_run = m_new;
-    float lsum = 0.0f;
-    half8_t ph[BN / 16], pl[F32 ? BN / 16 : 1];
-#pragma unroll
-    for (int jn = 0; jn < BN / 16; ++jn)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float w = __builtin_amdgcn_exp2f(s[jn / 2][8 * (jn % 2) + e] - m_ref);
-        lsum += w;
-        if constexpr (F32) {
-          _Float16 hi, lo;
-          split_f16(w, hi, lo);
-          ph[jn][e] = hi;
-          pl[jn][e] = lo;
-        } else {
-          ph[jn][e] = (_Float16)w;
-        }
-      }
-    l_run = l_run * alpha + lsum;
-    if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
-#pragma unroll
-      for (int r = 0; r < RB; ++r)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o_acc[r][i] *= alpha;
+    for (int i = 0; i < N; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, F32 ? 2 : 1, 0);
+      if (i < N - AH) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      if constexpr (NV > 0) __builtin_amdgcn_sched_group_barrier(0x402, NV, 0);
     }
-    const _Float16 *vt = sV + buf * BN * VP + vlane_off;
+  };
+  auto pv_tile = [&](auto buf_c, PTile &ph, PTile &pl) {
+    const _Float16 *vt = sV + vlane_off + decltype(buf_c)::value * BN * VP;
 #pragma unroll
-    for (int jn = 0; jn < BN / 16; ++jn)
+    for (int jn = 0; jn < PS; ++jn)
 #pragma unroll
       for (int r = 0; r < RB; ++r) {
         const _Float16 *vp = vt + 16 * jn * VP + 32 * r;
@@ -248,30 +232,236 @@ __global__ __launch_bounds__(256, (D <= 128 && std::is_same<T, _Float16>::value)
         o_acc[r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[jn], o_acc[r], 0, 0, 0);
         if constexpr (F32) o_acc[r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[jn], o_acc[r], 0, 0, 0);
       }
-    if (edge && bad_tile[buf] == t) {
-      for (int k = 0; k < BN; ++k) {
-        const int key = base + k;
-        if (key >= key_end) break;
-        const int number = pages.row[key >> p.page_shift];  // key < key_end <= the table's room
-        if ((uint32_t)number >= (uint32_t)p.n_pages) continue;
-        const _Float16 *vrow = p.v + number * p.pool.page + kvh * p.pool.head + (key & page_mask) * p.pool.row;
-        const bool sees = key <= pos && !(windowed && key <= pos - window);
+  };
+  auto sched_pv = [&](auto nv_c) {
+    constexpr int NV = decltype(nv_c)::value, N = PS * RB, AH = kVAhead < N ? kVAhead : N;
+    __builtin_amdgcn_sched_group_barrier(0x100, 2 * AH, 0);
 #pragma unroll
-        for (int r = 0; r < RB; ++r)
+    for (int i = 0; i < N; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, F32 ? 2 : 1, 0);
+      if (i < N - AH) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      if constexpr (NV > 0) __builtin_amdgcn_sched_group_barrier(0x402, NV, 0);
+    }
+  };
+  auto row_max = [&](STile &s) {
+    float mt = kNegInf;
 #pragma unroll
-          for (int i4 = 0; i4 < 4; ++i4) {
-            const half4_t x = *(const half4_t *)(vrow + 32 * r + 8 * i4 + 4 * hl);
+    for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (sees && not_finite(x[e])) o_acc[r][4 * i4 + e] += (float)x[e];
+      for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[kb][i]);
+    return xor32_combine(mt, [](float a, float b) { return fmaxf(a, b); }) * ce;
+  };
+  constexpr float kLazy = 8.0f;
+  // Cap, mask and maximum of tile t.  The reference moves where a row's maximum exceeds it by more than
+  // kLazy (log2), or when the row sees its first key; the factor its sums take with it is returned.
+  auto mask_max = [&](auto buf_c, int t, STile &s) -> float {
+    const int base = base0 + t * BN;
+    if constexpr (CAP) {
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[kb][i] = soft_cap(s[kb][i] * p.scale, p.softcap, inv_cap);
+    }
+    if (!seen_whole(t)) {
+      const int hi = min(pos, key_end - 1), lo = windowed ? pos - window : -1;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = base + 32 * kb + 8 * (i / 4) + 4 * hl + (i % 4);
+          s[kb][i] = key <= hi && key > lo ? s[kb][i] : kNegInf;
+        }
+    }
+    if constexpr (F32) {
+      // An infinite key times the two halves of a query is infinity minus infinity, or infinity times zero:
+      // where a logit is NaN, the high half alone says whether it is infinite.
+      float any = 0.0f;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) any += s[kb][i];
+      if (__builtin_amdgcn_ballot_w64(any != any) != 0) {
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb) {
+          float16_t high = {0.0f};
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk)
+            high = __builtin_amdgcn_mfma_f32_32x32x16_f16(
+                *(const half8_t *)(sK + ln * KP + 8 * hl + (decltype(buf_c)::value * BN + 32 * kb) * KP + 16 * kk), qh[kk], high, 0, 0, 0);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float x = high[i];
+            if constexpr (CAP) x = soft_cap(x * p.scale, p.softcap, inv_cap);
+            if (s[kb][i] != s[kb][i] && __builtin_isinf(high[i])) s[kb][i] = x;
           }
+        }
       }
     }
-    if (t + 1 < n_it) stage(buf ^ 1, t + 1, base + BN);
+    const float mt = row_max(s);
+    const bool first = m_run == kNegInf;
+    const float over = mt - m_ref;
+    const float delta = first ? (mt == kNegInf ? 0.0f : over) : over > kLazy ? over : 0.0f;
+    m_ref += delta;
+    if (!first || mt != kNegInf) m_run = m_ref;
+    return first ? 0.0f : __builtin_amdgcn_exp2f(-delta);
+  };
+  auto rescale = [&](float alpha) {
+    if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
+#pragma unroll
+      for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o_acc[r][i] *= alpha;
+      l_run *= alpha;
+    }
+  };
+  // probabilities of slices [J0, J1) of a tile; returns their row sum (this half's keys)
+  auto exp_part = [&](STile &s, PTile &ph, PTile &pl, auto j0_c, auto j1_c) -> float {
+    float sum = 0.0f;
+#pragma unroll
+    for (int jn = decltype(j0_c)::value; jn < decltype(j1_c)::value; ++jn) {
+      typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[jn / 2][8 * (jn % 2) + e], ce, -m_ref));
+        if constexpr (F32) {
+          _Float16 hi, lo;
+          split_f16(x, hi, lo);
+          ph[jn][e] = hi;
+          pl[jn][e] = lo;
+          sum += x;
+        } else {
+          ph[jn][e] = (_Float16)x;
+        }
+      }
+      if constexpr (!F32) {
+        // the sum takes the rounded weights the matrix cores consume
+#pragma unroll
+        for (int e = 0; e < 8; e += 2) {
+          const half2_t pr = {ph[jn][e], ph[jn][e + 1]}, one = {(_Float16)1.0f, (_Float16)1.0f};
+          sum = __builtin_amdgcn_fdot2(pr, one, sum, false);
+        }
+      }
+    }
+    return sum;
+  };
+  typedef std::integral_constant<int, 0> J0;
+  typedef std::integral_constant<int, kSplit> JS;
+  typedef std::integral_constant<int, PS> JN;
+  // the infinities and NaN that were taken out of V tile t, to the rows that see them
+  auto add_bad = [&](int t) {
+    for (int k = 0; k < BN; ++k) {
+      const int key = base0 + t * BN + k;
+      if (key >= part_end) break;
+      const int number = pages.row[key >> p.page_shift];  // key < key_end <= the table's room
+      if ((uint32_t)number >= pages.n_pages) continue;
+      const _Float16 *vrow = (const _Float16 *)(v_pool.base + (uint64_t)(uint32_t)number * pages.page_bytes + (uint32_t)(key & page_mask) * row_bytes);
+      const bool sees = key <= pos && !(windowed && key <= pos - window);
+#pragma unroll
+      for (int r = 0; r < RB; ++r)
+#pragma unroll
+        for (int i4 = 0; i4 < 4; ++i4) {
+          const half4_t x = *(const half4_t *)(vrow + 32 * r + 8 * i4 + 4 * hl);
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (sees && not_finite(x[e])) o_acc[r][4 * i4 + e] += (float)x[e];
+          __builtin_amdgcn_sched_barrier(0);  // a few conditions at a time: this path is rare and must not cost the common one registers
+        }
+    }
+  };
+
+  PTile p_a, p_b, p_lo;
+  float l_head = 0.0f;   // row sum of the slices formed early
+  // One step: on entry s_cur holds the logits of tile t (edge steps: masked, their reference set, the sums'
+  // factor in alpha; interior steps: the first slices of P formed).
+  auto step = [&](int t, STile &s_cur, STile &s_next, PTile &p_cur, PTile &p_next, float &alpha, auto interior_c, auto parity_c) {
+    constexpr bool INTERIOR = decltype(interior_c)::value;
+    typedef std::integral_constant<int, decltype(parity_c)::value> Buf;         // t % 2
+    typedef std::integral_constant<int, 1 - decltype(parity_c)::value> Other;
+    constexpr int FETCH = DEEP ? Buf::value : 0, STAGE = DEEP ? Other::value : 0;
+    constexpr int AHEAD = DEEP ? 1 : 0;
+    if constexpr (!INTERIOR) rescale(alpha);
+    fetch_v(vpre[FETCH]);                  // tile t + 1 + AHEAD
+    fetch_k(t + 2 + AHEAD, kpre[FETCH]);
+    qk_tile(Other{}, s_next);  // behind the last tile: of zeros, or of what is staged, and not used
+    if constexpr (INTERIOR) {
+      float sum = l_head + exp_part(s_cur, p_cur, p_lo, JS{}, JN{});
+      sched_qk(std::integral_constant<int, kPhaseValu>{});
+      if (__builtin_amdgcn_ballot_w64(!(sum < 1e30f)) != 0) {
+        const float over = row_max(s_cur) - m_ref, delta = over > kLazy ? over : 0.0f;
+        rescale(__builtin_amdgcn_exp2f(-delta));
+        m_ref += delta;
+        m_run = m_ref;
+        sum = exp_part(s_cur, p_cur, p_lo, J0{}, JN{});
+      }
+      l_run += sum;
+    } else {
+      sched_qk(std::integral_constant<int, 0>{});
+      l_run += exp_part(s_cur, p_cur, p_lo, J0{}, JN{});
+    }
+    pv_tile(Buf{}, p_cur, p_lo);
+    if constexpr (INTERIOR) {
+      l_head = exp_part(s_next, p_next, p_lo, J0{}, JS{});
+      // formed here, beside the MFMAs, and not where they are first used
+#pragma unroll
+      for (int jn = 0; jn < kSplit; ++jn) asm volatile("" : "+v"(p_next[jn]));
+      asm volatile("" : "+v"(l_head));
+      sched_pv(std::integral_constant<int, kPhaseValu>{});
+    } else {
+      sched_pv(std::integral_constant<int, 0>{});
+      if (!seen_whole(t) && bad_tile[Buf::value] == t) add_bad(t);
+      if (t + 1 < n_it) alpha = mask_max(Other{}, t + 1, s_next);
+    }
+    stage_k(Buf{}, kpre[STAGE]);
+    stage_v(Other{}, t + 1, vpre[STAGE], INTERIOR || seen_whole(t + 1));
+    __syncthreads();  // fills are visible; every wave is done with the buffers the next step refills
+  };
+
+  STile s_a, s_b;
+  if (threadIdx.x < 2) bad_tile[threadIdx.x] = -1;
+  if (n_it > 0) {
+    constexpr int S1 = DEEP ? 1 : 0;
+    typedef std::integral_constant<int, 0> Even;
+    typedef std::integral_constant<int, 1> Odd;
+    fetch_k(0, kpre[0]);
+    fetch_v(vpre[0]);
+    if constexpr (DEEP) fetch_k(1, kpre[1]);
+    __builtin_amdgcn_sched_barrier(0);
+    load_q();
+    __syncthreads();  // bad_tile
+    stage_k(Even{}, kpre[0]);
+    stage_v(Even{}, 0, vpre[0], seen_whole(0));
+    if constexpr (!DEEP) fetch_k(1, kpre[0]);
+    stage_k(Odd{}, kpre[S1]);
+    if constexpr (DEEP) {  // what step 0 stages at its end
+      fetch_v(vpre[1]);
+      fetch_k(2, kpre[1]);
+    }
     __syncthreads();
+    qk_tile(Even{}, s_a);
+    sched_qk(std::integral_constant<int, 0>{});
+    float alpha = mask_max(Even{}, 0, s_a);
+    __syncthreads();  // sK[0] is refilled by the first step
+    int t = 0;
+    while (true) {
+      for (; t < n_it && (F32 || CAP || t < full_from || t + 2 >= full_upto); t += 2) {
+        step(t, s_a, s_b, p_a, p_a, alpha, std::false_type{}, Even{});
+        if (t + 1 < n_it) step(t + 1, s_b, s_a, p_a, p_a, alpha, std::false_type{}, Odd{});
+      }
+      if (F32 || CAP || t >= n_it) break;
+      rescale(alpha);
+      l_head = exp_part(s_a, p_a, p_lo, J0{}, JS{});
+      for (; t + 2 < full_upto; t += 2) {
+        step(t, s_a, s_b, p_a, p_b, alpha, std::true_type{}, Even{});
+        step(t + 1, s_b, s_a, p_b, p_a, alpha, std::true_type{}, Odd{});
+      }
+      // tile t has its logits but no maximum yet, and its early slices are formed again with the others
+      alpha = mask_max(Even{}, t, s_a);
+    }
   }
 
   l_run += __shfl_xor(l_run, 32, 64);
+  {
+  const PagedParams &p = params_again();
   if (!entire) {
     if (row_ok) {
       const int64_t at = ((int64_t)slot * p.heads_kv + kvh) * kChunkRows + 32 * wave + ln;
@@ -300,31 +490,26 @@ __global__ __launch_bounds__(256, (D <= 128 && std::is_same<T, _Float16>::value)
         *(T4 *)(out + 32 * r + 8 * i4 + 4 * hl) = o;
       }
   }
+  work.next(p.sched, p.cu_new, p.kv_len);
   }
+  }
+  if (p.cuts && w < p.sched.target && kvh == 0 && threadIdx.x == 0) p.cuts[w] = cut;
 }
 
 // Merge of the parts of cut tiles: row m of a tile is sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m), in the
-// order of the parts.  The end of share b - 1 cuts at most one tile; of a tile cut more than once the
-// first cut's workgroups do the merge.  D / 4 threads share a row.
+// order of the parts.  One share begins a cut tile at most, its last one.  D / 4 threads share a row.
 template <int D, typename T>
 __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedParams p) {
   constexpr int RPB = 256 / (D / 4);
   const int R = p.sched.tile_rows, chunks = (R + RPB - 1) / RPB;
-  const int b = blockIdx.x / (chunks * p.heads_kv) + 1, kvh = blockIdx.x / chunks % p.heads_kv;
-  const PagedLine line(p.sched, p.cu_new, p.kv_len);
-  if (line.whole(p.sched) || b * line.share >= line.work) return;
-  PagedPlace it;
-  if (!sched_find(p.sched, p.cu_new, p.kv_len, false, b * line.share, it)) return;
-  if (it.start == b * line.share || it.start < (b - 1) * line.share) return;  // not cut here, or cut before
-  const int last = (int)((it.start + it.cost - 1) / line.share);               // the share the tile ends in
-  const int G = p.sched.group;
+  const int w = blockIdx.x / (chunks * p.heads_kv), kvh = blockIdx.x / chunks % p.heads_kv;
+  const PagedCut cut = p.cuts[w];
   const int lr = blockIdx.x % chunks * RPB + threadIdx.x / (D / 4), ch = threadIdx.x % (D / 4) * 4;
-  const int64_t row = (int64_t)it.tile * R + lr;
-  if (lr >= R || row >= (int64_t)(it.s.q_end - it.s.q_begin) * G) return;
-  // parts: slot 2 (b - 1) + 1, then 2 b, 2 (b + 1), .. 2 last
+  if (cut.parts == 0 || lr >= cut.rows) return;
+  const int G = p.sched.group, n = cut.parts, row = cut.row0 + lr;
+  // parts: slot 2 w + 1, then 2 (w + 1), 2 (w + 2), ..
   const int64_t step = (int64_t)p.heads_kv * R, row_at = (int64_t)kvh * R + lr;
-  auto part = [&](int i) { return (int64_t)(i == 0 ? 2 * b - 1 : 2 * (b + i - 1)) * step + row_at; };
-  const int n = last - b + 2;
+  auto part = [&](int i) { return (int64_t)(2 * (w + i) + (i == 0)) * step + row_at; };
   float m = kNegInf;
   for (int i = 0; i < n; ++i) m = fmaxf(m, p.ws_ml[part(i) * 2]);
   const float m_ref = m == kNegInf ? 0.0f : m;
@@ -339,7 +524,7 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedParams p)
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] += x[e] * f;
   }
-  T *out = (T *)p.out + (int64_t)(it.s.q_begin + row / G) * p.out_stride + (int64_t)(kvh * G + row % G) * D + ch;
+  T *out = (T *)p.out + (int64_t)(cut.q_begin + row / G) * p.out_stride + (int64_t)(kvh * G + row % G) * D + ch;
 #pragma unroll
   for (int e = 0; e < 4; ++e) out[e] = (T)(l == 0.0f ? 0.0f : o[e] / l);
 }
@@ -347,8 +532,9 @@ __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedParams p)
 template <int D, typename T>
 int launch_chunk(argus_hip_ctx *ctx, const PagedParams &p, int items, hipStream_t stream) {
   auto kern = p.softcap > 0.0f ? paged_chunk_kernel<D, T, true> : paged_chunk_kernel<D, T, false>;
-  ARGUS_HIP_CHECK(ctx, argus_raise_lds_limit(ctx, kern, ChunkTile<D>::LDS_BYTES));
-  hipLaunchKernelGGL(kern, dim3((unsigned)(items * p.heads_kv)), dim3(256), ChunkTile<D>::LDS_BYTES, stream, p);
+  constexpr int lds = ChunkTile<D, std::is_same<T, float>::value>::LDS_BYTES;
+  ARGUS_HIP_CHECK(ctx, argus_raise_lds_limit(ctx, kern, lds));
+  hipLaunchKernelGGL(kern, dim3((unsigned)(items * p.heads_kv)), dim3(256), lds, stream, p);
   ARGUS_HIP_CHECK(ctx, hipGetLastError());
   return ARGUS_HIP_OK;
 }
@@ -358,7 +544,7 @@ struct CallPlan {
   bool decode, chunk;
   PagedSched ds, cs;
   int64_t d_items, c_items, d_slots, c_slots;
-  int64_t ws_floats;  // [decode o][decode ml][chunk o][chunk ml]
+  int64_t ws_floats;  // decode, chunk: [output rows][cuts][maxima and sums]
 };
 
 int make_plan(argus_hip_ctx *ctx, int compute_units, const argus_hip_paged_attention_args *a, CallPlan &pl) {
@@ -406,7 +592,8 @@ int make_plan(argus_hip_ctx *ctx, int compute_units, const argus_hip_paged_atten
   constexpr int64_t kGrid = 0x7fffffff;
   if (pl.c_items * a->heads_kv > kGrid)
     return argus_fail(ctx, ARGUS_HIP_ERR_UNSUPPORTED, "paged_attention: %d rows are too many for one call", a->n_tokens);
-  pl.ws_floats = (pl.d_slots * kDecodeRows + pl.c_slots * kChunkRows) * a->heads_kv * (d + 2);
+  pl.ws_floats = (pl.d_slots * kDecodeRows + pl.c_slots * kChunkRows) * a->heads_kv * (d + 2) +
+                 ((pl.d_slots ? pl.ds.target : 0) + (pl.c_slots ? pl.cs.target : 0)) * (int64_t)(sizeof(PagedCut) / sizeof(float));
   return ARGUS_HIP_OK;
 }
 
@@ -511,17 +698,19 @@ ARGUS_API int argus_hip_paged_attention(argus_hip_ctx *ctx, const argus_hip_page
   if (pl.decode) {
     p.sched = pl.ds;
     p.ws_o = ws;  // output rows first: they are read and written 16 bytes at a time
-    p.ws_ml = ws + pl.d_slots * kDecodeRows * a->heads_kv * d;
+    p.cuts = pl.d_slots ? (PagedCut *)(ws + pl.d_slots * kDecodeRows * a->heads_kv * d) : nullptr;
+    p.ws_ml = (float *)(p.cuts + (pl.d_slots ? pl.ds.target : 0));
     rc = launch_paged_decode(ctx, p, d, f32, (int)pl.d_items, stream);
     if (rc == ARGUS_HIP_OK && !pl.chunk) timer.mark();
     if (rc == ARGUS_HIP_OK && pl.d_slots) rc = launch_paged_combine(ctx, p, d, f32, stream);
     if (rc != ARGUS_HIP_OK) return rc;
-    if (ws) ws += pl.d_slots * kDecodeRows * a->heads_kv * (d + 2);
+    if (pl.d_slots) ws = p.ws_ml + pl.d_slots * kDecodeRows * a->heads_kv * 2;
   }
   if (pl.chunk) {
     p.sched = pl.cs;
     p.ws_o = ws;
-    p.ws_ml = ws + pl.c_slots * kChunkRows * a->heads_kv * d;
+    p.cuts = pl.c_slots ? (PagedCut *)(ws + pl.c_slots * kChunkRows * a->heads_kv * d) : nullptr;
+    p.ws_ml = (float *)(p.cuts + (pl.c_slots ? pl.cs.target : 0));
     rc = launch_paged_chunk(ctx, p, d, f32, (int)pl.c_items, stream);
     timer.mark();
     if (rc == ARGUS_HIP_OK && pl.c_slots) rc = launch_paged_combine(ctx, p, d, f32, stream);

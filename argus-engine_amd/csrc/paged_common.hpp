@@ -44,6 +44,7 @@ struct PagedParams {
   // the begin of one that ends behind it.
   float *ws_ml;  // [slots, Hkv, tile_rows, 2]: running maximum (log2 units) and sum of a part's rows
   float *ws_o;   // [slots, Hkv, tile_rows, D]: un-normalised output rows
+  PagedCut *cuts;  // [shares]
   int64_t q_stride, out_stride;
   PoolStrides pool;  // elements
   PagedSched sched;
@@ -65,37 +66,66 @@ constexpr int chunk_align(int D) { return D <= 64 ? 64 : 32; }     // keys per t
 // dword 3 of a raw (untyped, unstrided) buffer descriptor on this target
 constexpr int kRawBuffer = 0x00020000;
 
-// Page numbers of a request's consecutive pages, 64 per register: the number of a page is a lane read,
-// not a memory access in the way of the page's rows.  `first` only moves up.
-struct PageWindow {
-  const int32_t *row;  // the request's row of the page table
-  int stride, first, now, next;
-  __device__ __forceinline__ int load(int at, int lane) const { return at + lane < stride ? row[at + lane] : -1; }
-  __device__ __forceinline__ PageWindow(const PagedParams &p, int seq, int page, int lane)
-      : row(p.page_table + (int64_t)seq * p.table_stride), stride(p.table_stride), first(page) {
-    now = load(first, lane);
-    next = load(first + 64, lane);
-  }
-  __device__ __forceinline__ void advance(int page, int lane) {  // wave-uniform; pages below `page` are not asked for again
-    if (page >= first + 64) {
-      first += 64;
-      now = next;
-      next = load(first + 64, lane);
-    }
-  }
-  __device__ __forceinline__ int number(int page) const {  // first <= page < first + 128
-    const int rel = page - first;
-    return __builtin_amdgcn_readlane(rel < 64 ? now : next, rel & 63);
+// One head's rows of the pages of a pool.
+struct PagePool {
+  const char *base;  // the head's first row in page 0
+  uint32_t bytes;    // from there to the end of the head's last row in a page
+  __device__ __forceinline__ PagePool(const _Float16 *pool, const PagedParams &p, int kvh, int D)
+      : base((const char *)(pool + kvh * p.pool.head)), bytes((uint32_t)(((1 << p.page_shift) - 1) * p.pool.row + D) * 2) {}
+  __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows(uint64_t page_off) const {
+    return __builtin_amdgcn_make_buffer_rsrc((void *)(base + page_off), 0, bytes, kRawBuffer);
   }
 };
 
-// Descriptor of one head's rows of a page that ends behind row `rows` - 1: rows past it, and every row
-// of a page whose number is none, read as zeros without touching memory.
-__device__ __forceinline__ __amdgpu_buffer_rsrc_t page_rows(const _Float16 *pool, const PagedParams &p, int number, int kvh, int rows, int D) {
-  const bool ok = (uint32_t)number < (uint32_t)p.n_pages && rows > 0;
-  const _Float16 *base = pool + (ok ? (int64_t)number * p.pool.page : 0) + (int64_t)kvh * p.pool.head;
-  const uint32_t bytes = ok ? (uint32_t)((rows - 1) * p.pool.row + D) * 2 : 0;
-  return __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, bytes, kRawBuffer);
+// Byte offsets of a request's consecutive pages, 64 per register pair: where a page lies is two lane reads,
+// not a memory access in the way of its rows.  Pages are asked for in ascending order.  A number outside the
+// pool, or a page behind the table, stands for page 0: what is read then is not specified, but is inside.
+struct PageWindow {
+  const int32_t *row;  // the request's row of the page table
+  int stride, first, next;
+  uint32_t n_pages, page_bytes, lo, hi;
+  __device__ __forceinline__ int load(int at) const {
+    const int i = at + (int)(threadIdx.x & 63);
+    const int number = i < stride ? row[i] : 0;
+    return (uint32_t)number < n_pages ? number : 0;
+  }
+  __device__ __forceinline__ void take(int numbers) {
+    const uint64_t off = (uint64_t)(uint32_t)numbers * page_bytes;
+    lo = (uint32_t)off;
+    hi = (uint32_t)(off >> 32);
+  }
+  template <int SPAN>
+  __device__ __forceinline__ void start(const PagedParams &p, int seq, int page) {
+    row = p.page_table + (int64_t)seq * p.table_stride;
+    stride = p.table_stride;
+    n_pages = (uint32_t)p.n_pages;
+    page_bytes = (uint32_t)p.pool.page * 2;
+    first = page;
+    take(load(first));
+    next = load(first + 64 - SPAN);
+  }
+  // makes pages page .. page + SPAN - 1 available; page at most 32 ahead of the last one
+  template <int SPAN>
+  __device__ __forceinline__ void advance(int page) {
+    if (page + SPAN > first + 64) {
+      first += 64 - SPAN;
+      take(next);
+      next = load(first + 64 - SPAN);
+    }
+  }
+  __device__ __forceinline__ uint64_t offset(int page) const {
+    const int l = page - first;
+    return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)hi, l) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)lo, l);
+  }
+};
+
+// The kernel's arguments read again from where they came: what is needed only after a long loop does not
+// stay in scalar registers through it.
+__device__ __forceinline__ const PagedParams &params_again() {
+  typedef const __attribute__((address_space(4))) PagedParams *const_ptr;
+  const_ptr a = (const_ptr)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(a));
+  return *(const PagedParams *)a;
 }
 
 // cap * tanh(s / cap), tanh(x) = 1 - 2 / (exp(2x) + 1); the argument is clamped where tanh is 1 in F32

@@ -59,22 +59,21 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(const PagedPa
   const int page_mask = (1 << p.page_shift) - 1;
   const uint32_t row_bytes = (uint32_t)p.pool.row * 2;
   const uint32_t k_lane = r * row_bytes + 16 * j, v_lane = 4 * j * row_bytes + 2 * VC * r;
+  const PagePool k_pool(p.k, p, kvh, D), v_pool(p.v, p, kvh, D);
   const float c = p.scale * kLog2e;
   const float inv_cap = CAP ? 1.0f / p.softcap : 0.0f;
   __shared__ float lds_m[kWaves][16], lds_l[kWaves][16];
   extern __shared__ __attribute__((aligned(16))) float lds_acc[];  // [kWaves][16][D + 4]
 
-  const PagedLine line(p.sched, p.cu_new, p.kv_len);
-  int64_t x = w * line.share;
-  const int64_t x_end = std::min<int64_t>(line.work, x + line.share);
-  while (x < x_end) {  // the requests this share touches
-  PagedPlace it;
-  if (!sched_find(p.sched, p.cu_new, p.kv_len, false, x, it)) return;
+  PagedCut cut{0, 0, 0, 0};
+  PagedShare work(p.sched, p.cu_new, p.kv_len, w);
+  while (work.found) {  // the requests this share touches
+  const PagedPlace it = work.at;
   const int rows = (it.s.q_end - it.s.q_begin) * G;  // at most 16: one tile
-  const int64_t from = x - it.start, upto = std::min<int64_t>(x_end - it.start, it.cost);
-  x = it.start + upto;
+  const int64_t from = work.from(), upto = work.upto();
   const bool entire = from == 0 && upto == it.cost;
   const int slot = 2 * w + (from == 0 ? 1 : 0);
+  if (!entire && from == 0) cut = PagedCut{(int)((it.start + it.cost - 1) / work.share) - w + 1, it.s.q_begin, 0, rows};
   const int begin = std::min<int64_t>(it.s.key_end, it.s.key_begin + from * p.sched.unit);
   const int end = std::min<int64_t>(it.s.key_end, it.s.key_begin + upto * p.sched.unit);
 
@@ -83,40 +82,37 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(const PagedPa
   const int pos = it.s.pos0 + rr / G;
   const int pos_last = it.s.pos0 + (rows - 1) / G;
 
-  PageWindow pages(p, it.seq, begin >> p.page_shift, lane);
+  PageWindow pages;
+  pages.start<TW>(p, it.seq, begin >> p.page_shift);
   half8_t kr[TW][KK];
   vpiece_t vr[TW][VSEG][4];
-  // the page of 16 keys from `key` on, ended at this part's last key (behind it: no rows at all), and the
-  // offset of the first of them
-  auto rows_at = [&](const _Float16 *pool, int key, uint32_t &soff) {
-    const bool some = key < end;
-    const int page = (some ? key : end) >> p.page_shift;
-    soff = some ? (uint32_t)(key & page_mask) * row_bytes : 0;
-    return page_rows(pool, p, pages.number(page), kvh, some ? min(end - (page << p.page_shift), page_mask + 1) : 0, D);
-  };
-  auto load_k = [&](int base) {
+  // 16 consecutive keys lie in one page: where, of the K rows requested last (the V rows follow)
+  uint64_t page_off[TW];
+  uint32_t row_off[TW];
+  auto load_k = [&](int base) {  // behind the part: its last page again
+    pages.advance<TW>(max(min(base, end - 1), begin) >> p.page_shift);
 #pragma unroll
     for (int tw = 0; tw < TW; ++tw) {
-      uint32_t soff;
-      const __amdgpu_buffer_rsrc_t rsrc = rows_at(p.k, base + 16 * tw, soff);
+      page_off[tw] = pages.offset(max(min(base + 16 * tw, end - 1), begin) >> p.page_shift);
+      row_off[tw] = (uint32_t)((base + 16 * tw) & page_mask) * row_bytes;
+      const __amdgpu_buffer_rsrc_t rsrc = k_pool.rows(page_off[tw]);
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) kr[tw][kk] = load_stream<half8_t>(rsrc, k_lane + 64 * kk, soff);
+      for (int kk = 0; kk < KK; ++kk) kr[tw][kk] = load_stream<half8_t>(rsrc, k_lane + 64 * kk, row_off[tw]);
     }
   };
-  auto load_v = [&](int base) {
+  auto load_v = [&]() {
 #pragma unroll
     for (int tw = 0; tw < TW; ++tw) {
-      uint32_t soff;
-      const __amdgpu_buffer_rsrc_t rsrc = rows_at(p.v, base + 16 * tw, soff);
+      const __amdgpu_buffer_rsrc_t rsrc = v_pool.rows(page_off[tw]);
 #pragma unroll
       for (int e = 0; e < 4; ++e)
 #pragma unroll
-        for (int sg = 0; sg < VSEG; ++sg) vr[tw][sg][e] = load_stream<vpiece_t>(rsrc, v_lane + e * row_bytes + 32 * VC * sg, soff);
+        for (int sg = 0; sg < VSEG; ++sg) vr[tw][sg][e] = load_stream<vpiece_t>(rsrc, v_lane + e * row_bytes + 32 * VC * sg, row_off[tw]);
     }
   };
   const int base0 = begin + wave * STEP;
   load_k(base0);
-  load_v(base0);
+  load_v();
 
   // Q: lane (j, r) holds chunk 4 kk + j of row r
   half8_t qh[KK], ql[F32 ? KK : 1];
@@ -152,13 +148,17 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(const PagedPa
 #pragma unroll
     for (int tw = 0; tw < TW; ++tw) {
       s[tw] = float4_t{0.0f, 0.0f, 0.0f, 0.0f};
+      float4_t low = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
       for (int kk = 0; kk < KK; ++kk) {
         s[tw] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kr[tw][kk], qh[kk], s[tw], 0, 0, 0);
-        if constexpr (F32) s[tw] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kr[tw][kk], ql[kk], s[tw], 0, 0, 0);
+        if constexpr (F32) low = __builtin_amdgcn_mfma_f32_16x16x32_f16(kr[tw][kk], ql[kk], low, 0, 0, 0);
+      }
+      if constexpr (F32) {  // an infinite logit is the high half's: the low one would add the other sign, or zero times it
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[tw][i] += __builtin_isinf(s[tw][i]) ? 0.0f : low[i];
       }
     }
-    pages.advance(base >> p.page_shift, lane);
     load_k(base + kWaves * STEP);
     // keys some row does not see: past the first token's position, in front of the last one's window, past the part
     const bool edge = base + STEP - 1 > it.s.pos0 || base + STEP > end || (window != 0x7fffffff && base <= pos_last - window);
@@ -243,6 +243,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(const PagedPa
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
                       if (sees[i]) o_acc[sg * VC + ch][i] += x;
+                  __builtin_amdgcn_sched_barrier(0);  // one value at a time: this path is rare and must not cost the common one registers
                 }
             }
 #pragma unroll
@@ -277,10 +278,11 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(const PagedPa
           if constexpr (F32) o = __builtin_amdgcn_mfma_f32_16x16x16f16(pl[0], bv, o, 0, 0, 0);
         }
       }
-    load_v(base + kWaves * STEP);
+    load_v();
   }
 
   // ---- merge: lane groups (row sum), then the waves through LDS -----------------------------------
+  const PagedParams &p = params_again();
   l_run += __shfl_xor(l_run, 16, 64);
   l_run += __shfl_xor(l_run, 32, 64);
   if (j == 0) {
@@ -321,7 +323,9 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(const PagedPa
     }
   }
   __syncthreads();  // the merge area is free for the next request
+  work.next(p.sched, p.cu_new, p.kv_len);
   }
+  if (p.cuts && kvh == 0 && threadIdx.x == 0) p.cuts[w] = cut;
 }
 
 template <int D, typename T>

@@ -108,24 +108,27 @@ inline int64_t sched_slots_bound(const PagedSched &c) { return 2 * (int64_t)c.ta
 #ifdef __HIPCC__
 #include <hip/hip_runtime.h>
 
-__device__ __forceinline__ int64_t wave_add64(int64_t x) {
-#pragma unroll
-  for (int d = 32; d; d >>= 1) x += __shfl_xor(x, d, 64);
+// Inclusive sum over the wave's lanes, in the vector ALU: within rows of 16 lanes, then the rows' ends
+// broadcast to the rows behind them.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int64_t dpp_add64(int64_t x) {
+  const int lo = __builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWS, 0xf, false);
+  const int hi = __builtin_amdgcn_update_dpp(0, (int)(x >> 32), CTRL, ROWS, 0xf, false);
+  return x + (int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo);
+}
+__device__ __forceinline__ int64_t wave_scan64(int64_t x) {
+  x = dpp_add64<0x111, 0xf>(x);  // row_shr 1, 2, 4, 8
+  x = dpp_add64<0x112, 0xf>(x);
+  x = dpp_add64<0x114, 0xf>(x);
+  x = dpp_add64<0x118, 0xf>(x);
+  x = dpp_add64<0x142, 0xa>(x);  // row_bcast 15 into rows 1 and 3
+  x = dpp_add64<0x143, 0xc>(x);  // row_bcast 31 into rows 2 and 3
   return x;
 }
-__device__ __forceinline__ int64_t wave_scan64(int64_t x, int lane) {  // inclusive
-#pragma unroll
-  for (int d = 1; d < 64; d <<= 1) {
-    const int64_t a = __shfl_up(x, d, 64);
-    if (lane >= d) x += a;
-  }
-  return x;
+__device__ __forceinline__ int lane_value(int x, int l) { return __builtin_amdgcn_readlane(x, l); }
+__device__ __forceinline__ int64_t lane_value(int64_t x, int l) {
+  return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(x >> 32), l) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)x, l));
 }
-__device__ __forceinline__ int wave_same(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ int64_t wave_same(int64_t x) {
-  return (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32) | (uint32_t)__builtin_amdgcn_readfirstlane((int)x));
-}
-
 // A tile on the line of work.
 struct PagedPlace {
   PagedSeq s;
@@ -133,80 +136,119 @@ struct PagedPlace {
   int64_t start, cost;  // of the tile, on the line
 };
 
-// The line of work of one class.  Every wave of a workgroup gets the same answers; lane l looks after
-// requests l, 64 + l, ...  Nothing but the sums stays in registers: a search looks the lengths up again.
-struct PagedLine {
-  int64_t work, tiles, share;
+// A block of 64 requests, one per lane.
+struct PagedBlock {
+  PagedSeq s;
+  PagedCost k;
+  int64_t total, inc;  // cost of this lane's request, and of the block's requests up to it
 
-  static __device__ __forceinline__ void look(const PagedSched &c, const int32_t *cu, const int32_t *kv, int i, PagedSeq &s, PagedCost &k) {
-    k = PagedCost{0, 0, 0};
-    s = PagedSeq{};
+  __device__ __forceinline__ PagedBlock(const PagedSched &c, const int32_t *cu, const int32_t *kv, int b) : s{}, k{0, 0, 0} {
+    const int i = b + (threadIdx.x & 63);
     if (i < c.n_seqs) {
       s = sched_seq(c, cu[i], cu[i + 1], kv[i]);
       k = sched_cost(c, s);
     }
+    total = sched_before(k, k.tiles);
+    inc = wave_scan64(total);
   }
-  __device__ __forceinline__ PagedLine(const PagedSched &c, const int32_t *cu, const int32_t *kv) {
-    const int lane = threadIdx.x & 63;
-    int64_t w = 0, t = 0;
-    for (int b = 0; b < c.n_seqs; b += 64) {
-      PagedSeq s;
-      PagedCost k;
-      look(c, cu, kv, b + lane, s, k);
-      w += sched_before(k, k.tiles);
-      t += k.tiles;
+  // the tile that holds position x of the line; `at`: where the block begins.  False: behind the block
+  __device__ __forceinline__ bool find(int b, int64_t at, int64_t x, PagedPlace &out) const {
+    const uint64_t past = __builtin_amdgcn_ballot_w64(at + inc > x);
+    if (!past) return false;
+    const int l = __builtin_ctzll(past);
+    PagedCost cost;
+    cost.tiles = lane_value(k.tiles, l);
+    cost.base = lane_value(k.base, l);
+    cost.slope = lane_value(k.slope, l);
+    const int64_t before = at + lane_value(inc - total, l);
+    int tile = 0, hi = cost.tiles;  // the last tile with sched_before <= x - before
+    while (hi - tile > 1) {
+      const int mid = (tile + hi) >> 1;
+      if (sched_before(cost, mid) <= x - before) tile = mid;
+      else hi = mid;
     }
-    work = wave_same(wave_add64(w));
-    tiles = wave_same(wave_add64(t));
-    share = sched_share(c, work);
+    place(b, l, cost, tile, before, out);
+    return true;
   }
-  __device__ __forceinline__ bool whole(const PagedSched &c) const { return tiles >= c.whole_from; }
+  // tile number x of the line, the last tiles of a request first
+  __device__ __forceinline__ bool find_tile(int b, int64_t at, int64_t inc_tiles, int64_t x, PagedPlace &out) const {
+    const uint64_t past = __builtin_amdgcn_ballot_w64(at + inc_tiles > x);
+    if (!past) return false;
+    const int l = __builtin_ctzll(past);
+    PagedCost cost;
+    cost.tiles = lane_value(k.tiles, l);
+    cost.base = lane_value(k.base, l);
+    cost.slope = lane_value(k.slope, l);
+    place(b, l, cost, (int)(at + lane_value(inc_tiles, l) - 1 - x), 0, out);
+    return true;
+  }
+  __device__ __forceinline__ void place(int b, int l, const PagedCost &cost, int tile, int64_t before, PagedPlace &out) const {
+    out.tile = tile;
+    out.seq = b + l;
+    out.start = before + sched_before(cost, tile);
+    out.cost = cost.base + cost.slope * tile;
+    out.s.q_begin = lane_value(s.q_begin, l);
+    out.s.q_end = lane_value(s.q_end, l);
+    out.s.pos0 = lane_value(s.pos0, l);
+    out.s.len = lane_value(s.len, l);
+    out.s.key_begin = lane_value(s.key_begin, l);
+    out.s.key_end = lane_value(s.key_end, l);
+  }
 };
 
-// The tile that holds position x of the line (by_tile: tile number x, the last tiles of a request first).
-__device__ __forceinline__ bool sched_find(const PagedSched &c, const int32_t *cu, const int32_t *kv, bool by_tile, int64_t x, PagedPlace &out) {
-  const int lane = threadIdx.x & 63;
-  int64_t at = 0;
-  for (int b = 0; b < c.n_seqs; b += 64) {
-    PagedSeq s;
-    PagedCost k;
-    PagedLine::look(c, cu, kv, b + lane, s, k);
-    const int64_t mine = by_tile ? (int64_t)k.tiles : sched_before(k, k.tiles);
-    const int64_t inc = wave_scan64(mine, lane);
-    const uint64_t past = __builtin_amdgcn_ballot_w64(at + inc > x);
-    if (past) {
-      const int l = __builtin_ctzll(past);
-      PagedCost cost;
-      cost.tiles = wave_same(__shfl(k.tiles, l, 64));
-      cost.base = wave_same(__shfl(k.base, l, 64));
-      cost.slope = wave_same(__shfl(k.slope, l, 64));
-      const int64_t before = at + wave_same(__shfl(inc - mine, l, 64));
-      int tile = 0;
-      if (by_tile) {
-        tile = cost.tiles - 1 - (int)(x - before);
-      } else if (cost.tiles > 1) {
-        int hi = cost.tiles;  // the last tile with sched_before <= x - before
-        while (hi - tile > 1) {
-          const int mid = (tile + hi) >> 1;
-          if (sched_before(cost, mid) <= x - before) tile = mid;
-          else hi = mid;
-        }
-      }
-      if (tile < 0 || tile >= cost.tiles) return false;  // lengths that are none: sums that wrapped
-      out.tile = wave_same(tile);
-      out.seq = wave_same(b + l);
-      out.start = before + sched_before(cost, tile);
-      out.cost = cost.base + cost.slope * tile;
-      out.s.q_begin = wave_same(__shfl(s.q_begin, l, 64));
-      out.s.q_end = wave_same(__shfl(s.q_end, l, 64));
-      out.s.pos0 = wave_same(__shfl(s.pos0, l, 64));
-      out.s.len = wave_same(__shfl(s.len, l, 64));
-      out.s.key_begin = wave_same(__shfl(s.key_begin, l, 64));
-      out.s.key_end = wave_same(__shfl(s.key_end, l, 64));
-      return true;
+// Share `w` of the line of work of a class, tile by tile.  Every wave of a workgroup gets the same
+// answers.  The lengths are looked up again for each further request: nothing but a few sums stays in
+// registers beside a tile's work.
+struct PagedShare {
+  int64_t x, end;    // what is left of the share
+  int64_t share;     // of every workgroup
+  bool whole;        // tiles are not cut
+  bool found;        // a tile is there
+  PagedPlace at;
+
+  __device__ __forceinline__ PagedShare(const PagedSched &c, const int32_t *cu, const int32_t *kv, int64_t w) {
+    int64_t work = 0, tiles = 0;
+    PagedBlock first(c, cu, kv, 0);
+    const int64_t first_tiles = wave_scan64(first.k.tiles);
+    work = lane_value(first.inc, 63);
+    tiles = lane_value(first_tiles, 63);
+    for (int b = 64; b < c.n_seqs; b += 64) {
+      const PagedBlock block(c, cu, kv, b);
+      work += lane_value(block.inc, 63);
+      tiles += lane_value(wave_scan64(block.k.tiles), 63);
     }
-    at += wave_same(__shfl(inc, 63, 64));
+    share = sched_share(c, work);
+    whole = tiles >= c.whole_from;
+    x = whole ? w : w * share;
+    end = whole ? tiles : work;
+    if (x + (whole ? 1 : share) < end) end = x + (whole ? 1 : share);
+    found = x < end && (whole ? first.find_tile(0, 0, first_tiles, x, at) : first.find(0, 0, x, at));
+    if (x < end && !found) search(c, cu, kv, lane_value(whole ? first_tiles : first.inc, 63), 64);
   }
-  return false;
-}
+  __device__ __forceinline__ void search(const PagedSched &c, const int32_t *cu, const int32_t *kv, int64_t before, int b) {
+    found = false;
+    for (; b < c.n_seqs && !found; b += 64) {
+      const PagedBlock block(c, cu, kv, b);
+      const int64_t inc = whole ? wave_scan64(block.k.tiles) : block.inc;
+      found = whole ? block.find_tile(b, before, inc, x, at) : block.find(b, before, x, at);
+      before += lane_value(inc, 63);
+    }
+  }
+  // part of the tile that lies in the share
+  __device__ __forceinline__ int64_t from() const { return whole ? 0 : x - at.start; }
+  __device__ __forceinline__ int64_t upto() const { return whole ? at.cost : end - at.start < at.cost ? end - at.start : at.cost; }
+  __device__ __forceinline__ void next(const PagedSched &c, const int32_t *cu, const int32_t *kv) {
+    x = whole ? end : at.start + at.cost;
+    found = false;
+    if (x < end) search(c, cu, kv, 0, 0);
+  }
+};
+
+// What the merge has to know of a tile that is cut: left in the workspace by the share it begins in.
+struct PagedCut {
+  int32_t parts;    // 0: the share ends with a tile
+  int32_t q_begin;  // row of q of its request
+  int32_t row0;     // first of its rows in the request
+  int32_t rows;
+};
 #endif

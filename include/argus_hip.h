@@ -741,9 +741,9 @@ int argus_hip_qk_norm_rope(argus_hip_ctx *ctx, const argus_hip_qk_norm_rope_args
  *   s_c = (q . k_c) * scale; softcap > 0: softcap * tanh(s_c / softcap); out = sum_c softmax(s)_c v_c
  * Rows that see nothing, or whose logits are all -inf, give zeros; a NaN logit gives a NaN row; what
  * a key the row does not see holds (NaN, infinities, rows of a page behind the last token) has no
- * influence.  Rows of q / out behind cu_new[n_seqs] are neither read nor written.  The keys of a page
- * number outside the pool, and those past table_stride pages, read as zeros: such a request's rows are
- * finite and otherwise unspecified.
+ * influence.  Rows of q / out behind cu_new[n_seqs] are neither read nor written.  A request with a page
+ * number outside the pool where its keys lie reads some page of the pool there instead, and keys past
+ * table_stride pages do not exist: its rows are not specified, no other request's are touched.
  * dtype F16: logits and sums in F32, probabilities rounded to F16 for the second product; dtype F32: q and
  * the probabilities as F16 pairs (hi + lo), so the result is that of F32 arithmetic.
  * max_new / max_kv: no request brings more new tokens / holds more tokens than this (0 = not known).
