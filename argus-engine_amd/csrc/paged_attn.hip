@@ -76,10 +76,10 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
   const int my_row = lane / (D / 8), my_col = lane % (D / 8);
   const uint32_t lane_off = my_row * row_bytes + 16 * my_col;
   const PagePool k_pool(p.k, p, kvh, D), v_pool(p.v, p, kvh, D);
-  // exponents are logit * ce - m_ref; a negative scale turns the queries round instead
+  // exponents are logit * ce - m_ref (CAP: of the capped logit); a negative scale turns the queries round instead
   const float ce = CAP ? kLog2e : __builtin_fabsf(p.scale) * kLog2e;
-  const float q_sign = !CAP && p.scale < 0.0f ? -1.0f : 1.0f;
-  const float inv_cap = CAP ? 1.0f / p.softcap : 0.0f;
+  const float q_sign = p.scale < 0.0f ? -1.0f : 1.0f;
+  const float cap = p.softcap, cap_in = CAP ? __builtin_fabsf(p.scale) / p.softcap : 0.0f;  // cap * tanh(product * cap_in)
   // V^T operand: ds_read_b64_tr_b16 gives lane i of 16 channel ch0 + i of keys key0 .. key0 + 3 when lane s
   // addresses V[key0 + s / 4][ch0 + 4 (s % 4)]; P^T holds keys 4 hl + {0..3} and 8 + 4 hl + {0..3} of 16
   const int g16 = lane >> 4, s16 = lane & 15;
@@ -123,7 +123,7 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
   half8_t kpre[SETS][CH], vpre[SETS][CH];
   uint64_t page_off[CH];  // of the K tile requested last; its V tile follows a step later
   uint32_t row_off[CH];
-  auto fetch_k = [&](int t, half8_t(&pre)[CH]) {  // behind the part: its last page again
+  auto fetch_k = [&](int t, half8_t(&pre)[CH]) __attribute__((always_inline)) {  // behind the part: its last page again
     const int base = base0 + t * BN;
     pages.advance<SPAN>(min(base, part_end - 1) >> p.page_shift);
 #pragma unroll
@@ -134,18 +134,18 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
       pre[i] = __builtin_bit_cast(half8_t, __builtin_amdgcn_raw_buffer_load_b128(k_pool.rows(page_off[i]), lane_off, row_off[i], 0));
     }
   };
-  auto fetch_v = [&](half8_t(&pre)[CH]) {  // of the K tile requested last
+  auto fetch_v = [&](half8_t(&pre)[CH]) __attribute__((always_inline)) {  // of the K tile requested last
 #pragma unroll
     for (int i = 0; i < CH; ++i)
       pre[i] = __builtin_bit_cast(half8_t, __builtin_amdgcn_raw_buffer_load_b128(v_pool.rows(page_off[i]), lane_off, row_off[i], 0));
   };
   const int stage_row = wave * RPW + my_row;
-  auto stage_k = [&](auto buf_c, half8_t(&pre)[CH]) {
+  auto stage_k = [&](auto buf_c, half8_t(&pre)[CH]) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < CH; ++i)
       *(half8_t *)(sK + stage_row * KP + 8 * my_col + (decltype(buf_c)::value * BN + 4 * RPW * i) * KP) = pre[i];
   };
-  auto stage_v = [&](auto buf_c, int t, half8_t(&pre)[CH], bool seen_whole) {  // tile t into buffer t % 2
+  auto stage_v = [&](auto buf_c, int t, half8_t(&pre)[CH], bool seen_whole) __attribute__((always_inline)) {  // tile t into buffer t % 2
     if (!seen_whole) {
       // A weight of zero does not keep an infinity or a NaN out of the product: such values of V leave the
       // tile here and are added, by themselves, to the rows that see their key.
@@ -164,11 +164,11 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
     for (int i = 0; i < CH; ++i)
       *(half8_t *)(sV + stage_row * VP + 8 * my_col + (decltype(buf_c)::value * BN + 4 * RPW * i) * VP) = pre[i];
   };
-  auto seen_whole = [&](int t) { return t >= full_from && t < full_upto; };
+  auto seen_whole = [&](int t) __attribute__((always_inline)) { return t >= full_from && t < full_upto; };
 
   // ---- Q as the B operand: lane (row ln, half hl) holds channels 16 kk + 8 hl .. + 7
   half8_t qh[KK], ql[F32 ? KK : 1];
-  auto load_q = [&]() {
+  auto load_q = [&]() __attribute__((always_inline)) {
     const T *qp = (const T *)p.q + (int64_t)(it.s.q_begin + tok) * p.q_stride + (int64_t)head * D + 8 * hl;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
@@ -199,7 +199,7 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
   typedef half8_t PTile[PS];
   // Instruction order of a phase, given once all of its code has been emitted: operand reads a few MFMAs
   // ahead, and behind every MFMA some of the other tile's exponentials (a wave issues in order).
-  auto qk_tile = [&](auto buf_c, STile &s) {
+  auto qk_tile = [&](auto buf_c, STile &s) __attribute__((always_inline)) {
     const _Float16 *kt = sK + ln * KP + 8 * hl + decltype(buf_c)::value * BN * KP;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk)
@@ -210,7 +210,7 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
         if constexpr (F32) s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[kk], s[kb], 0, 0, 0);
       }
   };
-  auto sched_qk = [&](auto nv_c) {
+  auto sched_qk = [&](auto nv_c) __attribute__((always_inline)) {
     constexpr int NV = decltype(nv_c)::value, N = KK * KB, AH = kAhead < N ? kAhead : N;
     __builtin_amdgcn_sched_group_barrier(0x100, AH, 0);
 #pragma unroll
@@ -220,7 +220,7 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
       if constexpr (NV > 0) __builtin_amdgcn_sched_group_barrier(0x402, NV, 0);
     }
   };
-  auto pv_tile = [&](auto buf_c, PTile &ph, PTile &pl) {
+  auto pv_tile = [&](auto buf_c, PTile &ph, PTile &pl) __attribute__((always_inline)) {
     const _Float16 *vt = sV + vlane_off + decltype(buf_c)::value * BN * VP;
 #pragma unroll
     for (int jn = 0; jn < PS; ++jn)
@@ -233,7 +233,7 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
         if constexpr (F32) o_acc[r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[jn], o_acc[r], 0, 0, 0);
       }
   };
-  auto sched_pv = [&](auto nv_c) {
+  auto sched_pv = [&](auto nv_c) __attribute__((always_inline)) {
     constexpr int NV = decltype(nv_c)::value, N = PS * RB, AH = kVAhead < N ? kVAhead : N;
     __builtin_amdgcn_sched_group_barrier(0x100, 2 * AH, 0);
 #pragma unroll
@@ -243,24 +243,26 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
       if constexpr (NV > 0) __builtin_amdgcn_sched_group_barrier(0x402, NV, 0);
     }
   };
-  auto row_max = [&](STile &s) {
+  auto row_max = [&](STile &s, auto raw_c) __attribute__((always_inline)) {  // raw: products of q and k, not capped yet
     float mt = kNegInf;
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[kb][i]);
-    return xor32_combine(mt, [](float a, float b) { return fmaxf(a, b); }) * ce;
+    mt = xor32_combine(mt, [](float a, float b) { return fmaxf(a, b); });
+    if constexpr (CAP && decltype(raw_c)::value) mt = soft_cap<F32>(mt, cap, cap_in);
+    return mt * ce;
   };
   constexpr float kLazy = 8.0f;
   // Cap, mask and maximum of tile t.  The reference moves where a row's maximum exceeds it by more than
   // kLazy (log2), or when the row sees its first key; the factor its sums take with it is returned.
-  auto mask_max = [&](auto buf_c, int t, STile &s) -> float {
+  auto mask_max = [&](auto buf_c, int t, STile &s) __attribute__((always_inline)) -> float {
     const int base = base0 + t * BN;
     if constexpr (CAP) {
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s[kb][i] = soft_cap(s[kb][i] * p.scale, p.softcap, inv_cap);
+        for (int i = 0; i < 16; ++i) s[kb][i] = soft_cap<F32>(s[kb][i], cap, cap_in);
     }
     if (!seen_whole(t)) {
       const int hi = min(pos, key_end - 1), lo = windowed ? pos - window : -1;
@@ -291,13 +293,13 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             float x = high[i];
-            if constexpr (CAP) x = soft_cap(x * p.scale, p.softcap, inv_cap);
+            if constexpr (CAP) x = soft_cap<F32>(x, cap, cap_in);
             if (s[kb][i] != s[kb][i] && __builtin_isinf(high[i])) s[kb][i] = x;
           }
         }
       }
     }
-    const float mt = row_max(s);
+    const float mt = row_max(s, std::false_type{});
     const bool first = m_run == kNegInf;
     const float over = mt - m_ref;
     const float delta = first ? (mt == kNegInf ? 0.0f : over) : over > kLazy ? over : 0.0f;
@@ -305,7 +307,7 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
     if (!first || mt != kNegInf) m_run = m_ref;
     return first ? 0.0f : __builtin_amdgcn_exp2f(-delta);
   };
-  auto rescale = [&](float alpha) {
+  auto rescale = [&](float alpha) __attribute__((always_inline)) {
     if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
 #pragma unroll
       for (int r = 0; r < RB; ++r)
@@ -315,14 +317,16 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
     }
   };
   // probabilities of slices [J0, J1) of a tile; returns their row sum (this half's keys)
-  auto exp_part = [&](STile &s, PTile &ph, PTile &pl, auto j0_c, auto j1_c) -> float {
+  auto exp_part = [&](STile &s, PTile &ph, PTile &pl, auto raw_c, auto j0_c, auto j1_c) __attribute__((always_inline)) -> float {
     float sum = 0.0f;
 #pragma unroll
     for (int jn = decltype(j0_c)::value; jn < decltype(j1_c)::value; ++jn) {
       typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[jn / 2][8 * (jn % 2) + e], ce, -m_ref));
+        float x = s[jn / 2][8 * (jn % 2) + e];
+        if constexpr (CAP && decltype(raw_c)::value) x = soft_cap<F32>(x, cap, cap_in);
+        x = __builtin_amdgcn_exp2f(__builtin_fmaf(x, ce, -m_ref));
         if constexpr (F32) {
           _Float16 hi, lo;
           split_f16(x, hi, lo);
@@ -348,7 +352,7 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
   typedef std::integral_constant<int, kSplit> JS;
   typedef std::integral_constant<int, PS> JN;
   // the infinities and NaN that were taken out of V tile t, to the rows that see them
-  auto add_bad = [&](int t) {
+  auto add_bad = [&](int t) __attribute__((always_inline)) {
     for (int k = 0; k < BN; ++k) {
       const int key = base0 + t * BN + k;
       if (key >= part_end) break;
@@ -373,7 +377,7 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
   float l_head = 0.0f;   // row sum of the slices formed early
   // One step: on entry s_cur holds the logits of tile t (edge steps: masked, their reference set, the sums'
   // factor in alpha; interior steps: the first slices of P formed).
-  auto step = [&](int t, STile &s_cur, STile &s_next, PTile &p_cur, PTile &p_next, float &alpha, auto interior_c, auto parity_c) {
+  auto step = [&](int t, STile &s_cur, STile &s_next, PTile &p_cur, PTile &p_next, float &alpha, auto interior_c, auto parity_c) __attribute__((always_inline)) {
     constexpr bool INTERIOR = decltype(interior_c)::value;
     typedef std::integral_constant<int, decltype(parity_c)::value> Buf;         // t % 2
     typedef std::integral_constant<int, 1 - decltype(parity_c)::value> Other;
@@ -384,23 +388,23 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
     fetch_k(t + 2 + AHEAD, kpre[FETCH]);
     qk_tile(Other{}, s_next);  // behind the last tile: of zeros, or of what is staged, and not used
     if constexpr (INTERIOR) {
-      float sum = l_head + exp_part(s_cur, p_cur, p_lo, JS{}, JN{});
+      float sum = l_head + exp_part(s_cur, p_cur, p_lo, std::true_type{}, JS{}, JN{});
       sched_qk(std::integral_constant<int, kPhaseValu>{});
       if (__builtin_amdgcn_ballot_w64(!(sum < 1e30f)) != 0) {
-        const float over = row_max(s_cur) - m_ref, delta = over > kLazy ? over : 0.0f;
+        const float over = row_max(s_cur, std::true_type{}) - m_ref, delta = over > kLazy ? over : 0.0f;
         rescale(__builtin_amdgcn_exp2f(-delta));
         m_ref += delta;
         m_run = m_ref;
-        sum = exp_part(s_cur, p_cur, p_lo, J0{}, JN{});
+        sum = exp_part(s_cur, p_cur, p_lo, std::true_type{}, J0{}, JN{});
       }
       l_run += sum;
     } else {
       sched_qk(std::integral_constant<int, 0>{});
-      l_run += exp_part(s_cur, p_cur, p_lo, J0{}, JN{});
+      l_run += exp_part(s_cur, p_cur, p_lo, std::false_type{}, J0{}, JN{});
     }
     pv_tile(Buf{}, p_cur, p_lo);
     if constexpr (INTERIOR) {
-      l_head = exp_part(s_next, p_next, p_lo, J0{}, JS{});
+      l_head = exp_part(s_next, p_next, p_lo, std::true_type{}, J0{}, JS{});
       // formed here, beside the MFMAs, and not where they are first used
 #pragma unroll
       for (int jn = 0; jn < kSplit; ++jn) asm volatile("" : "+v"(p_next[jn]));
@@ -443,13 +447,17 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
     __syncthreads();  // sK[0] is refilled by the first step
     int t = 0;
     while (true) {
-      for (; t < n_it && (F32 || CAP || t < full_from || t + 2 >= full_upto); t += 2) {
+      for (; t < n_it && (F32 || t < full_from || t + 2 >= full_upto); t += 2) {
         step(t, s_a, s_b, p_a, p_a, alpha, std::false_type{}, Even{});
         if (t + 1 < n_it) step(t + 1, s_b, s_a, p_a, p_a, alpha, std::false_type{}, Odd{});
       }
-      if (F32 || CAP || t >= n_it) break;
+      if (F32 || t >= n_it) break;
       rescale(alpha);
-      l_head = exp_part(s_a, p_a, p_lo, J0{}, JS{});
+      if constexpr (CAP) {  // an interior step starts from products
+        qk_tile(Even{}, s_a);
+        __syncthreads();
+      }
+      l_head = exp_part(s_a, p_a, p_lo, std::true_type{}, J0{}, JS{});
       for (; t + 2 < full_upto; t += 2) {
         step(t, s_a, s_b, p_a, p_b, alpha, std::true_type{}, Even{});
         step(t + 1, s_b, s_a, p_b, p_a, alpha, std::true_type{}, Odd{});
@@ -496,37 +504,60 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
   if (p.cuts && w < p.sched.target && kvh == 0 && threadIdx.x == 0) p.cuts[w] = cut;
 }
 
-// Merge of the parts of cut tiles: row m of a tile is sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m), in the
-// order of the parts.  One share begins a cut tile at most, its last one.  D / 4 threads share a row.
-template <int D, typename T>
+// Merge of the parts of cut tiles: row m of a tile is sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m).  One
+// share begins a cut tile at most, its last one.  D / 4 threads share a row's channels.  Decode tiles (PG > 1)
+// have few rows and up to hundreds of parts: a workgroup takes one row, its thread groups every PG-th part,
+// and the groups are added in LDS; chunk tiles (PG 1) have many rows of two or three parts.
+template <int D, typename T, bool DECODE>
 __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedParams p) {
-  constexpr int RPB = 256 / (D / 4);
-  const int R = p.sched.tile_rows, chunks = (R + RPB - 1) / RPB;
+  constexpr int TPR = D / 4, PG = DECODE ? 256 / TPR : 1, RPB = DECODE ? 1 : 256 / TPR;
+  constexpr int R = DECODE ? kDecodeRows : kChunkRows;
+  constexpr int chunks = R / RPB;
+  static_assert(R % RPB == 0, "whole workgroups per tile");
   const int w = blockIdx.x / (chunks * p.heads_kv), kvh = blockIdx.x / chunks % p.heads_kv;
   const PagedCut cut = p.cuts[w];
-  const int lr = blockIdx.x % chunks * RPB + threadIdx.x / (D / 4), ch = threadIdx.x % (D / 4) * 4;
-  if (cut.parts == 0 || lr >= cut.rows) return;
+  const int lr = blockIdx.x % chunks * RPB + (DECODE ? 0 : threadIdx.x / TPR), ch = threadIdx.x % TPR * 4;
+  if (cut.parts == 0 || lr >= cut.rows) return;  // DECODE: the whole workgroup
   const int G = p.sched.group, n = cut.parts, row = cut.row0 + lr;
   // parts: slot 2 w + 1, then 2 (w + 1), 2 (w + 2), ..
   const int64_t step = (int64_t)p.heads_kv * R, row_at = (int64_t)kvh * R + lr;
   auto part = [&](int i) { return (int64_t)(2 * (w + i) + (i == 0)) * step + row_at; };
-  float m = kNegInf;
-  for (int i = 0; i < n; ++i) m = fmaxf(m, p.ws_ml[part(i) * 2]);
-  const float m_ref = m == kNegInf ? 0.0f : m;
+  float m = kNegInf, l = 0.0f, m_ref;
+  if constexpr (DECODE) {  // a lane per part, every wave for itself
+    const int lane = threadIdx.x & 63;
+    for (int i = lane; i < n; i += 64) m = fmaxf(m, p.ws_ml[part(i) * 2]);
+    m = wave_allreduce_max(m);
+    m_ref = m == kNegInf ? 0.0f : m;
+    for (int i = lane; i < n; i += 64) l += p.ws_ml[part(i) * 2 + 1] * __builtin_amdgcn_exp2f(p.ws_ml[part(i) * 2] - m_ref);
+    l = wave_allreduce_sum(l);
+  } else {
+    for (int i = 0; i < n; ++i) m = fmaxf(m, p.ws_ml[part(i) * 2]);
+    m_ref = m == kNegInf ? 0.0f : m;
+    for (int i = 0; i < n; ++i) l += p.ws_ml[part(i) * 2 + 1] * __builtin_amdgcn_exp2f(p.ws_ml[part(i) * 2] - m_ref);
+  }
   float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
-  float l = 0.0f;
 #pragma unroll 4
-  for (int i = 0; i < n; ++i) {
+  for (int i = DECODE ? threadIdx.x / TPR : 0; i < n; i += PG) {
     const int64_t at = part(i);
     const float f = __builtin_amdgcn_exp2f(p.ws_ml[at * 2] - m_ref);
-    l += p.ws_ml[at * 2 + 1] * f;
     const float4_t x = *(const float4_t *)(p.ws_o + at * D + ch);
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] += x[e] * f;
   }
-  T *out = (T *)p.out + (int64_t)(cut.q_begin + row / G) * p.out_stride + (int64_t)(kvh * G + row % G) * D + ch;
+  if constexpr (DECODE) {
+    __shared__ float4_t sum[256];
+    sum[threadIdx.x] = o;
+    __syncthreads();
+    if (threadIdx.x >= TPR) return;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) out[e] = (T)(l == 0.0f ? 0.0f : o[e] / l);
+    for (int g = 1; g < PG; ++g) o += sum[g * TPR + threadIdx.x];
+  }
+  T *out = (T *)p.out + (int64_t)(cut.q_begin + row / G) * p.out_stride + (int64_t)(kvh * G + row % G) * D + ch;
+  typedef T T4 __attribute__((ext_vector_type(4)));
+  T4 y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = (T)(l == 0.0f ? 0.0f : o[e] / l);
+  *(T4 *)out = y;
 }
 
 template <int D, typename T>
@@ -560,6 +591,10 @@ int make_plan(argus_hip_ctx *ctx, int compute_units, const argus_hip_paged_atten
   pl = CallPlan{};
   pl.decode = G <= kDecodeRows && (int64_t)a->min_new * G <= kDecodeRows;
   pl.chunk = !pl.decode || a->max_new == 0 || (int64_t)a->max_new * G > kDecodeRows;
+  // A call that is nearly all chunks gives its few short requests to the chunk kernel too: each costs it at
+  // most one tile more, and the decode kernel and its merge cost two launches (8 us beside a chunk kernel of
+  // 100 us at 2 requests of 414 new tokens) whether there is a request for them or not.
+  if (pl.decode && pl.chunk && (int64_t)a->n_seqs * kChunkRows * 8 <= (int64_t)a->n_tokens * G) pl.decode = false;
   if (pl.decode) {
     PagedSched &c = pl.ds = s;
     c.rows_upto = c.tile_rows = kDecodeRows;
@@ -632,14 +667,22 @@ int launch_paged_chunk(argus_hip_ctx *ctx, const PagedParams &p, int D, bool f32
   }
 }
 
-int launch_paged_combine(argus_hip_ctx *ctx, const PagedParams &p, int D, bool f32, hipStream_t stream) {
-  const int rpb = 256 / (D / 4), chunks = (p.sched.tile_rows + rpb - 1) / rpb, cuts = p.sched.target - 1;
-  auto kern = D == 64 ? (f32 ? paged_combine_kernel<64, float> : paged_combine_kernel<64, _Float16>)
-              : D == 128 ? (f32 ? paged_combine_kernel<128, float> : paged_combine_kernel<128, _Float16>)
-                         : (f32 ? paged_combine_kernel<256, float> : paged_combine_kernel<256, _Float16>);
+template <int D, typename T>
+static int launch_combine(argus_hip_ctx *ctx, const PagedParams &p, hipStream_t stream) {
+  const bool decode = p.sched.tile_rows == kDecodeRows;
+  const int chunks = decode ? kDecodeRows : kChunkRows / (256 / (D / 4)), cuts = p.sched.target - 1;
+  auto kern = decode ? paged_combine_kernel<D, T, true> : paged_combine_kernel<D, T, false>;
   hipLaunchKernelGGL(kern, dim3((unsigned)(cuts * p.heads_kv * chunks)), dim3(256), 0, stream, p);
   ARGUS_HIP_CHECK(ctx, hipGetLastError());
   return ARGUS_HIP_OK;
+}
+
+int launch_paged_combine(argus_hip_ctx *ctx, const PagedParams &p, int D, bool f32, hipStream_t stream) {
+  switch (D) {
+    case 64: return f32 ? launch_combine<64, float>(ctx, p, stream) : launch_combine<64, _Float16>(ctx, p, stream);
+    case 128: return f32 ? launch_combine<128, float>(ctx, p, stream) : launch_combine<128, _Float16>(ctx, p, stream);
+    default: return f32 ? launch_combine<256, float>(ctx, p, stream) : launch_combine<256, _Float16>(ctx, p, stream);
+  }
 }
 
 }  // namespace argus_paged

@@ -168,7 +168,7 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(const PagedPa
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         float x = s[tw][i];
-        if constexpr (CAP) x = soft_cap(F32 ? x : x * p.scale, p.softcap, inv_cap) * kLog2e;
+        if constexpr (CAP) x = soft_cap<F32>(F32 ? x : x * p.scale, p.softcap, inv_cap) * kLog2e;
         else if constexpr (!F32) x *= c;
         if (edge) {
           const int key = base + 16 * tw + 4 * j + i;

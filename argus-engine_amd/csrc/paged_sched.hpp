@@ -86,7 +86,8 @@ ARGUS_HD PagedCost sched_cost(const PagedSched &c, const PagedSeq &s) {
 ARGUS_HD int64_t sched_before(const PagedCost &k, int t) { return k.base * t + k.slope * ((int64_t)t * (t - 1) / 2); }  // of tiles 0 .. t - 1
 
 ARGUS_HD int64_t sched_share(const PagedSched &c, int64_t work) {
-  const int64_t share = (int64_t)((double)work / c.target) + 1;  // target shares hold at least the work
+  int64_t share = (int64_t)((double)work / c.target);
+  if (share * c.target < work) ++share;  // target shares hold the work
   return share < c.min_share ? c.min_share : share;
 }
 
