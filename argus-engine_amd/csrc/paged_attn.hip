@@ -446,24 +446,23 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
     float alpha = mask_max(Even{}, 0, s_a);
     __syncthreads();  // sK[0] is refilled by the first step
     int t = 0;
-    while (true) {
-      for (; t < n_it && (F32 || t < full_from || t + 2 >= full_upto); t += 2) {
-        step(t, s_a, s_b, p_a, p_a, alpha, std::false_type{}, Even{});
-        if (t + 1 < n_it) step(t + 1, s_b, s_a, p_a, p_a, alpha, std::false_type{}, Odd{});
-      }
-      if (F32 || t >= n_it) break;
-      rescale(alpha);
+    const int n_int = full_from == 0 ? max(0, full_upto - 1) & ~1 : 0;  // steps whose tile and the next are seen whole
+    if (n_int > 0) {
       if constexpr (CAP) {  // an interior step starts from products
         qk_tile(Even{}, s_a);
         __syncthreads();
       }
       l_head = exp_part(s_a, p_a, p_lo, std::true_type{}, J0{}, JS{});
-      for (; t + 2 < full_upto; t += 2) {
+      for (; t < n_int; t += 2) {
         step(t, s_a, s_b, p_a, p_b, alpha, std::true_type{}, Even{});
         step(t + 1, s_b, s_a, p_b, p_a, alpha, std::true_type{}, Odd{});
       }
       // tile t has its logits but no maximum yet, and its early slices are formed again with the others
       alpha = mask_max(Even{}, t, s_a);
+    }
+    for (; t < n_it; t += 2) {
+      step(t, s_a, s_b, p_a, p_a, alpha, std::false_type{}, Even{});
+      if (t + 1 < n_it) step(t + 1, s_b, s_a, p_a, p_a, alpha, std::false_type{}, Odd{});
     }
   }
 
