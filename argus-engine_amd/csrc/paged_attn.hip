@@ -59,8 +59,7 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
   constexpr float kLog2e = 1.4426950408889634f;
   constexpr int kSplit = PS / 2;        // slices of P^T formed in phase B of the step before
   constexpr int kAhead = 4, kVAhead = D <= 64 ? 4 : 3;  // operand reads kept in flight
-  constexpr int kPhaseValu = D <= 64 ? 5 : 4;           // vector-ALU instructions placed behind each MFMA
-
+  
   extern __shared__ __attribute__((aligned(16))) _Float16 smem[];
   _Float16 *const sK = smem, *const sV = smem + 2 * BN * KP;  // [2][BN][KP], [2][BN][VP]
   __shared__ int bad_tile[2];  // tile whose V held infinities or NaN under a mask
@@ -115,35 +114,35 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
   const int full_from = windowed && wg_last >= window ? max(0, (wg_last - window + BN - base0) / BN) : 0;
   const int full_upto = min(n_it, max(0, min(wg_first + 1, key_end) - base0) / BN);
 
-  // ---- tiles: piece i of a thread is 16 bytes of row (threadIdx + 256 i) / (D / 8) of the tile; the rows
-  // one wave covers with a piece lie in one page
+  // ---- tiles: a wave fetches BN / 4 consecutive rows, which lie in one page, in CH pieces of 16 bytes per lane
   constexpr int SPAN = BN / 16;  // pages a tile touches at most
+  static_assert(BN / 4 <= 16, "a wave's rows of a tile lie in one page");
   PageWindow pages;
   pages.start<SPAN>(p, it.seq, base0 >> p.page_shift);
   half8_t kpre[SETS][CH], vpre[SETS][CH];
-  uint64_t page_off[CH];  // of the K tile requested last; its V tile follows a step later
-  uint32_t row_off[CH];
+  uint64_t page_off = 0;  // of the K tile requested last; its V tile follows a step later
+  uint32_t row_off = 0;
   auto fetch_k = [&](int t, half8_t(&pre)[CH]) __attribute__((always_inline)) {  // behind the part: its last page again
-    const int base = base0 + t * BN;
+    const int base = base0 + t * BN, key = base + wave * (BN / 4);
     pages.advance<SPAN>(min(base, part_end - 1) >> p.page_shift);
-#pragma unroll
-    for (int i = 0; i < CH; ++i) {
-      const int key = base + wave * RPW + 4 * RPW * i;
-      page_off[i] = pages.offset(min(key, part_end - 1) >> p.page_shift);
-      row_off[i] = (uint32_t)(key & page_mask) * row_bytes;
-      pre[i] = __builtin_bit_cast(half8_t, __builtin_amdgcn_raw_buffer_load_b128(k_pool.rows(page_off[i]), lane_off, row_off[i], 0));
-    }
-  };
-  auto fetch_v = [&](half8_t(&pre)[CH]) __attribute__((always_inline)) {  // of the K tile requested last
+    page_off = pages.offset(min(key, part_end - 1) >> p.page_shift);
+    row_off = (uint32_t)(key & page_mask) * row_bytes;
+    const __amdgpu_buffer_rsrc_t rows = k_pool.rows(page_off);
 #pragma unroll
     for (int i = 0; i < CH; ++i)
-      pre[i] = __builtin_bit_cast(half8_t, __builtin_amdgcn_raw_buffer_load_b128(v_pool.rows(page_off[i]), lane_off, row_off[i], 0));
+      pre[i] = __builtin_bit_cast(half8_t, __builtin_amdgcn_raw_buffer_load_b128(rows, lane_off, row_off + i * (RPW * row_bytes), 0));
   };
-  const int stage_row = wave * RPW + my_row;
+  auto fetch_v = [&](half8_t(&pre)[CH]) __attribute__((always_inline)) {  // of the K tile requested last
+    const __amdgpu_buffer_rsrc_t rows = v_pool.rows(page_off);
+#pragma unroll
+    for (int i = 0; i < CH; ++i)
+      pre[i] = __builtin_bit_cast(half8_t, __builtin_amdgcn_raw_buffer_load_b128(rows, lane_off, row_off + i * (RPW * row_bytes), 0));
+  };
+  const int stage_row = wave * (BN / 4) + my_row;
   auto stage_k = [&](auto buf_c, half8_t(&pre)[CH]) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < CH; ++i)
-      *(half8_t *)(sK + stage_row * KP + 8 * my_col + (decltype(buf_c)::value * BN + 4 * RPW * i) * KP) = pre[i];
+      *(half8_t *)(sK + stage_row * KP + 8 * my_col + (decltype(buf_c)::value * BN + RPW * i) * KP) = pre[i];
   };
   auto stage_v = [&](auto buf_c, int t, half8_t(&pre)[CH], bool seen_whole) __attribute__((always_inline)) {  // tile t into buffer t % 2
     if (!seen_whole) {
@@ -162,7 +161,7 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
     }
 #pragma unroll
     for (int i = 0; i < CH; ++i)
-      *(half8_t *)(sV + stage_row * VP + 8 * my_col + (decltype(buf_c)::value * BN + 4 * RPW * i) * VP) = pre[i];
+      *(half8_t *)(sV + stage_row * VP + 8 * my_col + (decltype(buf_c)::value * BN + RPW * i) * VP) = pre[i];
   };
   auto seen_whole = [&](int t) __attribute__((always_inline)) { return t >= full_from && t < full_upto; };
 
@@ -197,8 +196,6 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
 
   typedef float16_t STile[KB];
   typedef half8_t PTile[PS];
-  // Instruction order of a phase, given once all of its code has been emitted: operand reads a few MFMAs
-  // ahead, and behind every MFMA some of the other tile's exponentials (a wave issues in order).
   auto qk_tile = [&](auto buf_c, STile &s) __attribute__((always_inline)) {
     const _Float16 *kt = sK + ln * KP + 8 * hl + decltype(buf_c)::value * BN * KP;
 #pragma unroll
@@ -210,14 +207,15 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
         if constexpr (F32) s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[kk], s[kb], 0, 0, 0);
       }
   };
-  auto sched_qk = [&](auto nv_c) __attribute__((always_inline)) {
-    constexpr int NV = decltype(nv_c)::value, N = KK * KB, AH = kAhead < N ? kAhead : N;
+  // Order of a phase, given once its code has been emitted: operand reads a few MFMAs ahead.  (Placing the
+  // exponentials behind the MFMAs as well made no difference at d 128 and cost 4 % at d 256.)
+  auto sched_qk = [&]() __attribute__((always_inline)) {
+    constexpr int N = KK * KB, AH = kAhead < N ? kAhead : N;
     __builtin_amdgcn_sched_group_barrier(0x100, AH, 0);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, F32 ? 2 : 1, 0);
       if (i < N - AH) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      if constexpr (NV > 0) __builtin_amdgcn_sched_group_barrier(0x402, NV, 0);
     }
   };
   auto pv_tile = [&](auto buf_c, PTile &ph, PTile &pl) __attribute__((always_inline)) {
@@ -233,14 +231,13 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
         if constexpr (F32) o_acc[r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[jn], o_acc[r], 0, 0, 0);
       }
   };
-  auto sched_pv = [&](auto nv_c) __attribute__((always_inline)) {
-    constexpr int NV = decltype(nv_c)::value, N = PS * RB, AH = kVAhead < N ? kVAhead : N;
+  auto sched_pv = [&]() __attribute__((always_inline)) {
+    constexpr int N = PS * RB, AH = kVAhead < N ? kVAhead : N;
     __builtin_amdgcn_sched_group_barrier(0x100, 2 * AH, 0);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, F32 ? 2 : 1, 0);
       if (i < N - AH) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-      if constexpr (NV > 0) __builtin_amdgcn_sched_group_barrier(0x402, NV, 0);
     }
   };
   auto row_max = [&](STile &s, auto raw_c) __attribute__((always_inline)) {  // raw: products of q and k, not capped yet
@@ -389,7 +386,7 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
     qk_tile(Other{}, s_next);  // behind the last tile: of zeros, or of what is staged, and not used
     if constexpr (INTERIOR) {
       float sum = l_head + exp_part(s_cur, p_cur, p_lo, std::true_type{}, JS{}, JN{});
-      sched_qk(std::integral_constant<int, kPhaseValu>{});
+      sched_qk();
       if (__builtin_amdgcn_ballot_w64(!(sum < 1e30f)) != 0) {
         const float over = row_max(s_cur, std::true_type{}) - m_ref, delta = over > kLazy ? over : 0.0f;
         rescale(__builtin_amdgcn_exp2f(-delta));
@@ -399,7 +396,7 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
       }
       l_run += sum;
     } else {
-      sched_qk(std::integral_constant<int, 0>{});
+      sched_qk();
       l_run += exp_part(s_cur, p_cur, p_lo, std::false_type{}, J0{}, JN{});
     }
     pv_tile(Buf{}, p_cur, p_lo);
@@ -409,9 +406,9 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
 #pragma unroll
       for (int jn = 0; jn < kSplit; ++jn) asm volatile("" : "+v"(p_next[jn]));
       asm volatile("" : "+v"(l_head));
-      sched_pv(std::integral_constant<int, kPhaseValu>{});
+      sched_pv();
     } else {
-      sched_pv(std::integral_constant<int, 0>{});
+      sched_pv();
       if (!seen_whole(t) && bad_tile[Buf::value] == t) add_bad(t);
       if (t + 1 < n_it) alpha = mask_max(Other{}, t + 1, s_next);
     }
@@ -442,7 +439,7 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
     }
     __syncthreads();
     qk_tile(Even{}, s_a);
-    sched_qk(std::integral_constant<int, 0>{});
+    sched_qk();
     float alpha = mask_max(Even{}, 0, s_a);
     __syncthreads();  // sK[0] is refilled by the first step
     int t = 0;
@@ -600,13 +597,14 @@ int make_plan(argus_hip_ctx *ctx, int compute_units, const argus_hip_paged_atten
     c.align = decode_align(d);
     c.unit = 4 * c.align;
     c.min_share = 2;
-    c.whole_from = 0x7fffffff;
+    c.cut_cost = 2;  // 10 us; a unit of 128 keys is 5 us at d 128 with the device full
     // resident workgroups, and no more shares than the longest lengths make
     const int64_t tiles = sched_tiles_bound(c, a->min_new);
     const int64_t most = tiles * std::max<int64_t>(1, (longest + 2 * c.align) / c.unit + 1);
     c.target = (int)std::min<int64_t>(std::max(1, compute_units * 2 / a->heads_kv), std::max<int64_t>(1, most / c.min_share));
-    pl.d_items = c.target;
-    pl.d_slots = c.target > 1 ? sched_slots_bound(c) : 0;
+    if (c.target == 1) c.cut_cost = -1;
+    pl.d_items = sched_items_bound(c, tiles);
+    pl.d_slots = c.cut_cost >= 0 ? sched_slots_bound(c) : 0;
   }
   if (pl.chunk) {
     PagedSched &c = pl.cs = s;
@@ -617,11 +615,11 @@ int make_plan(argus_hip_ctx *ctx, int compute_units, const argus_hip_paged_atten
     c.min_share = 512;
     const int64_t tiles = sched_tiles_bound(c, a->min_new);
     c.target = std::max(1, compute_units * 2 / a->heads_kv);
-    c.whole_from = 4 * c.target;
-    if (longest + 96 <= c.min_share / 2) c.whole_from = 0;  // tiles too short to be cut
-    if (tiles == 0) pl.chunk = false;                       // too few rows for any request of this class
+    c.cut_cost = d == 64 ? 900 : 500;                    // keys a workgroup gets through in 15 us
+    if (longest + 96 <= c.min_share) c.cut_cost = -1;    // tiles too short to be cut
+    if (tiles == 0) pl.chunk = false;                    // too few rows for any request of this class
     pl.c_items = sched_items_bound(c, tiles);
-    pl.c_slots = c.whole_from > 0 && pl.chunk ? sched_slots_bound(c) : 0;
+    pl.c_slots = c.cut_cost >= 0 && pl.chunk ? sched_slots_bound(c) : 0;
   }
   constexpr int64_t kGrid = 0x7fffffff;
   if (pl.c_items * a->heads_kv > kGrid)

@@ -6,8 +6,9 @@
 // as many units as it sees keys.  The tiles of all requests, laid end to end, are one line of work that
 // is cut into equal shares, one per workgroup and KV head: a share ends in the middle of a tile where it
 // falls there, and the tile's parts are merged afterwards.  So a call fills the device whatever its
-// lengths are, and no workgroup carries more than another.  A call of very many tiles is not cut: every
-// workgroup takes one tile, the tiles of a request that see most keys first.
+// lengths are, and no workgroup carries more than another.  Where whole tiles fill it as well -- what the
+// rounds of workgroups take, or the longest tile, is not more than the shares and what the cutting costs --
+// every workgroup takes one tile, the tiles of a request that see most keys first.
 #pragma once
 
 #include <cstdint>
@@ -26,7 +27,7 @@ struct PagedSched {
   int32_t align;                 // key ranges start on a multiple of this
   int32_t min_share;             // a share is not smaller than this
   int32_t target;                // shares per KV head
-  int32_t whole_from;            // from this many tiles per KV head on every tile is a share
+  int32_t cut_cost;              // what cutting costs a call: further starts, partial results, the merge; < 0: no tile is cut
   int32_t window, max_len;       // max_len: keys the page table has room for
 };
 
@@ -91,6 +92,14 @@ ARGUS_HD int64_t sched_share(const PagedSched &c, int64_t work) {
   return share < c.min_share ? c.min_share : share;
 }
 
+// Are the tiles taken whole?  tiles, work, longest: over the class.
+ARGUS_HD bool sched_whole(const PagedSched &c, int64_t tiles, int64_t work, int64_t longest) {
+  if (c.cut_cost < 0 || tiles == 0) return true;
+  const double rounds = (double)((tiles + c.target - 1) / c.target) * ((double)work / (double)tiles);
+  const double whole = rounds > (double)longest ? rounds : (double)longest;
+  return whole <= (double)work / c.target + c.cut_cost;
+}
+
 // Bounds the host can give: tiles of a class, workgroups per KV head, and partial results (two per share:
 // the end of a tile begun before it and the begin of one that ends behind it).
 inline int64_t sched_tiles_bound(const PagedSched &c, int min_new) {
@@ -101,9 +110,7 @@ inline int64_t sched_tiles_bound(const PagedSched &c, int min_new) {
   if (c.rows_upto <= c.tile_rows) return seqs;
   return seqs ? rows / c.tile_rows + seqs : 0;
 }
-inline int64_t sched_items_bound(const PagedSched &c, int64_t tiles) {
-  return tiles >= c.whole_from ? tiles : (int64_t)c.target < (int64_t)c.whole_from ? c.target : c.whole_from;
-}
+inline int64_t sched_items_bound(const PagedSched &c, int64_t tiles) { return c.cut_cost >= 0 && tiles < c.target ? c.target : tiles; }
 inline int64_t sched_slots_bound(const PagedSched &c) { return 2 * (int64_t)c.target; }
 
 #ifdef __HIPCC__
@@ -125,6 +132,19 @@ __device__ __forceinline__ int64_t wave_scan64(int64_t x) {
   x = dpp_add64<0x142, 0xa>(x);  // row_bcast 15 into rows 1 and 3
   x = dpp_add64<0x143, 0xc>(x);  // row_bcast 31 into rows 2 and 3
   return x;
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ int dpp_max(int x) {
+  const int y = __builtin_amdgcn_update_dpp(x, x, CTRL, ROWS, 0xf, false);
+  return y > x ? y : x;
+}
+__device__ __forceinline__ int wave_max(int x) {  // in lane 63
+  x = dpp_max<0x111, 0xf>(x);
+  x = dpp_max<0x112, 0xf>(x);
+  x = dpp_max<0x114, 0xf>(x);
+  x = dpp_max<0x118, 0xf>(x);
+  x = dpp_max<0x142, 0xa>(x);
+  return dpp_max<0x143, 0xc>(x);
 }
 __device__ __forceinline__ int lane_value(int x, int l) { return __builtin_amdgcn_readlane(x, l); }
 __device__ __forceinline__ int64_t lane_value(int64_t x, int l) {
@@ -151,6 +171,10 @@ struct PagedBlock {
     }
     total = sched_before(k, k.tiles);
     inc = wave_scan64(total);
+  }
+  __device__ __forceinline__ int longest() const {
+    const int64_t last = k.tiles > 0 ? k.base + k.slope * (k.tiles - 1) : 0;
+    return lane_value(wave_max(last > 0x7fffffff ? 0x7fffffff : (int)last), 63);
   }
   // the tile that holds position x of the line; `at`: where the block begins.  False: behind the block
   __device__ __forceinline__ bool find(int b, int64_t at, int64_t x, PagedPlace &out) const {
@@ -213,13 +237,16 @@ struct PagedShare {
     const int64_t first_tiles = wave_scan64(first.k.tiles);
     work = lane_value(first.inc, 63);
     tiles = lane_value(first_tiles, 63);
+    int longest = first.longest();
     for (int b = 64; b < c.n_seqs; b += 64) {
       const PagedBlock block(c, cu, kv, b);
       work += lane_value(block.inc, 63);
       tiles += lane_value(wave_scan64(block.k.tiles), 63);
+      const int l = block.longest();
+      longest = l > longest ? l : longest;
     }
     share = sched_share(c, work);
-    whole = tiles >= c.whole_from;
+    whole = sched_whole(c, tiles, work, longest);
     x = whole ? w : w * share;
     end = whole ? tiles : work;
     if (x + (whole ? 1 : share) < end) end = x + (whole ? 1 : share);
