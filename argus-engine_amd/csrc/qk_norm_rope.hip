@@ -3,9 +3,9 @@
 //
 //   y = x * rsqrt(mean(x^2) + eps) * (w + b);   (a, b) -> (a cos - b sin, b cos + a sin)
 //
-// D / 8 lanes share a head; a lane holds the two groups of four channels that rotate into each other
-// (4i .. 4i+3 and rot/2 + 4i .., or 8i .. 8i+7 with adjacent pairs), so the rotation needs no exchange
-// and the norm one reduction over the head's lanes.  Bound by HBM for many tokens, by the launch for few.
+// A lane holds the two groups of W channels that rotate into each other (W i .. and rot/2 + W i .., or
+// 2 W i .. 2 W i + 2 W - 1 with adjacent pairs), so the rotation needs no exchange and the norm one
+// reduction over the head's lanes; W = 8, or 4 where alignment or rot_dim asks for it.  Bound by HBM for many tokens, by the launch for few.
 #include "paged_common.hpp"
 
 #include <type_traits>
@@ -24,124 +24,150 @@ struct QkNormRopeParams {
   float eps, weight_bias;
 };
 
-__device__ __forceinline__ void load4(const float *p, float (&x)[4]) {
-  const float4_t v = *(const float4_t *)p;
+// W consecutive channels (4, or 8 from two loads of a 4-byte type) as F32
+template <int W>
+__device__ __forceinline__ void load(const float *p, float (&x)[W]) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) x[e] = v[e];
-}
-__device__ __forceinline__ void load4(const _Float16 *p, float (&x)[4]) {
-  const half4_t v = *(const half4_t *)p;
+  for (int i = 0; i < W; i += 4) {
+    const float4_t v = *(const float4_t *)(p + i);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) x[e] = (float)v[e];
+    for (int e = 0; e < 4; ++e) x[i + e] = v[e];
+  }
 }
-__device__ __forceinline__ void store4(float *p, const float (&x)[4]) { *(float4_t *)p = float4_t{x[0], x[1], x[2], x[3]}; }
-__device__ __forceinline__ void store4(_Float16 *p, const float (&x)[4]) {
-  *(half4_t *)p = half4_t{(_Float16)x[0], (_Float16)x[1], (_Float16)x[2], (_Float16)x[3]};
+template <int W>
+__device__ __forceinline__ void load(const _Float16 *p, float (&x)[W]) {
+  typedef _Float16 half_w __attribute__((ext_vector_type(W)));
+  const half_w v = *(const half_w *)p;
+#pragma unroll
+  for (int e = 0; e < W; ++e) x[e] = (float)v[e];
+}
+template <int W>
+__device__ __forceinline__ void store(float *p, const float (&x)[W]) {
+#pragma unroll
+  for (int i = 0; i < W; i += 4) *(float4_t *)(p + i) = float4_t{x[i], x[i + 1], x[i + 2], x[i + 3]};
+}
+template <int W>
+__device__ __forceinline__ void store(_Float16 *p, const float (&x)[W]) {
+  typedef _Float16 half_w __attribute__((ext_vector_type(W)));
+  half_w v;
+#pragma unroll
+  for (int e = 0; e < W; ++e) v[e] = (_Float16)x[e];
+  *(half_w *)p = v;
 }
 
-template <int D, typename IN, typename OUT>
+// W: channels per group; a lane holds two groups, D / (2 W) lanes a head.
+template <int D, int W, typename IN, typename OUT>
 __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const QkNormRopeParams p) {
-  constexpr int LPH = D / 8;            // lanes per head
-  constexpr int HPB = 256 / LPH;        // heads per workgroup
+  constexpr int LPH = D / (2 * W);      // lanes per head
+  constexpr int HPB = 256 / LPH;        // heads per workgroup and turn
   const int token = blockIdx.x / p.chunks, chunk = blockIdx.x % p.chunks;
-  const int u = chunk * HPB + threadIdx.x / LPH;  // query heads, key heads, value heads
   const int i = threadIdx.x % LPH;
   const int pos = p.positions ? p.positions[token] : 0;
   if (pos < 0 || (p.rot_dim > 0 && pos >= p.n_positions)) return;  // padding
-  if (u >= p.heads_q + 2 * p.heads_kv) return;                     // whole heads: no lane of a head's reduction is missing
-  const bool is_q = u < p.heads_q, is_v = u >= p.heads_q + p.heads_kv;
-  const int h = is_q ? u : is_v ? u - p.heads_q - p.heads_kv : u - p.heads_q;
 
   // channels of this lane
   const int half = p.rot_dim / 2;
   int c0, c1;
   bool turn;
   if (p.interleaved) {
-    c0 = 8 * i, c1 = c0 + 4;
+    c0 = 2 * W * i, c1 = c0 + W;
     turn = c0 < p.rot_dim;
   } else {
-    turn = 4 * i < half;
-    c0 = turn ? 4 * i : 8 * i;  // lanes past half / 4: the channels behind rot_dim, eight in a row
-    c1 = turn ? c0 + half : c0 + 4;
+    turn = W * i < half;
+    c0 = turn ? W * i : 2 * W * i;  // lanes past half / W: the channels behind rot_dim, 2 W in a row
+    c1 = turn ? c0 + half : c0 + W;
   }
-  const IN *src = is_q ? (const IN *)p.q + token * p.q_stride : is_v ? (const IN *)p.v + token * p.v_stride : (const IN *)p.k + token * p.k_stride;
-  src += (int64_t)h * D;
-  float a[4], b[4];
-  load4(src + c0, a);
-  load4(src + c1, b);
-
-  if (!is_v) {
-    const float *w = is_q ? p.q_weight : p.k_weight;
-    if (w) {
-      float sq = 0.0f;
+  float cs[W], sn[W];
+  if (turn) {
+    const float *row = p.cos_sin + (int64_t)pos * p.rot_dim + W * i;
+    load<W>(row, cs);
+    load<W>(row + half, sn);
+  }
+  const int units = p.heads_q + 2 * p.heads_kv;  // query heads, key heads, value heads
+  for (int u = chunk * HPB + threadIdx.x / LPH; u < units; u += p.chunks * HPB) {  // whole heads: no lane of a head's sum is missing
+    const bool is_q = u < p.heads_q, is_v = u >= p.heads_q + p.heads_kv;
+    const int h = is_q ? u : is_v ? u - p.heads_q - p.heads_kv : u - p.heads_q;
+    const IN *src = is_q ? (const IN *)p.q + token * p.q_stride : is_v ? (const IN *)p.v + token * p.v_stride : (const IN *)p.k + token * p.k_stride;
+    src += (int64_t)h * D;
+    float a[W], b[W];
+    load<W>(src + c0, a);
+    load<W>(src + c1, b);
+    if (!is_v) {
+      const float *w = is_q ? p.q_weight : p.k_weight;
+      if (w) {
+        float sq = 0.0f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) sq += a[e] * a[e] + b[e] * b[e];
-      sq = group_allreduce_sum<LPH>(sq);
-      const float inv = 1.0f / sqrtf(sq * (1.0f / D) + p.eps);
-      float wa[4], wb[4];
-      load4(w + c0, wa);
-      load4(w + c1, wb);
+        for (int e = 0; e < W; ++e) sq += a[e] * a[e] + b[e] * b[e];
+        sq = group_allreduce_sum<LPH>(sq);
+        const float inv = 1.0f / sqrtf(sq * (1.0f / D) + p.eps);
+        float wa[W], wb[W];
+        load<W>(w + c0, wa);
+        load<W>(w + c1, wb);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        a[e] = a[e] * inv * (wa[e] + p.weight_bias);
-        b[e] = b[e] * inv * (wb[e] + p.weight_bias);
-      }
-    }
-    if (turn) {
-      const float *row = p.cos_sin + (int64_t)pos * p.rot_dim;
-      const int j = 4 * i;  // first of this lane's four angles
-      float cs[4], sn[4];
-      load4(row + j, cs);
-      load4(row + half + j, sn);
-      if (p.interleaved) {
-        float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float r = x[2 * e] * cs[e] - x[2 * e + 1] * sn[e], s = x[2 * e + 1] * cs[e] + x[2 * e] * sn[e];
-          x[2 * e] = r;
-          x[2 * e + 1] = s;
-        }
-#pragma unroll
-        for (int e = 0; e < 4; ++e) a[e] = x[e], b[e] = x[4 + e];
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float r = a[e] * cs[e] - b[e] * sn[e], s = b[e] * cs[e] + a[e] * sn[e];
-          a[e] = r;
-          b[e] = s;
+        for (int e = 0; e < W; ++e) {
+          a[e] = a[e] * inv * (wa[e] + p.weight_bias);
+          b[e] = b[e] * inv * (wb[e] + p.weight_bias);
         }
       }
+      if (turn) {
+        if (p.interleaved) {
+          float x[2 * W];
+#pragma unroll
+          for (int e = 0; e < W; ++e) x[e] = a[e], x[W + e] = b[e];
+#pragma unroll
+          for (int e = 0; e < W; ++e) {
+            const float r = x[2 * e] * cs[e] - x[2 * e + 1] * sn[e], s = x[2 * e + 1] * cs[e] + x[2 * e] * sn[e];
+            x[2 * e] = r;
+            x[2 * e + 1] = s;
+          }
+#pragma unroll
+          for (int e = 0; e < W; ++e) a[e] = x[e], b[e] = x[W + e];
+        } else {
+#pragma unroll
+          for (int e = 0; e < W; ++e) {
+            const float r = a[e] * cs[e] - b[e] * sn[e], s = b[e] * cs[e] + a[e] * sn[e];
+            a[e] = r;
+            b[e] = s;
+          }
+        }
+      }
     }
-  }
-  if (is_q) {
-    OUT *dst = (OUT *)p.q_out + token * p.q_out_stride + (int64_t)h * D;
-    store4(dst + c0, a);
-    store4(dst + c1, b);
-  } else {
-    const int slot = p.slots[token];
-    if ((uint32_t)slot >= (uint32_t)p.n_slots) return;
-    const int page = slot >> p.page_shift, row = slot & ((1 << p.page_shift) - 1);
-    _Float16 *dst = (_Float16 *)(is_v ? p.v_cache : p.k_cache) + page * p.pool.page + h * p.pool.head + row * p.pool.row;
-    store4(dst + c0, a);
-    store4(dst + c1, b);
+    if (is_q) {
+      OUT *dst = (OUT *)p.q_out + token * p.q_out_stride + (int64_t)h * D;
+      store<W>(dst + c0, a);
+      store<W>(dst + c1, b);
+    } else {
+      const int slot = p.slots[token];
+      if ((uint32_t)slot >= (uint32_t)p.n_slots) continue;
+      const int page = slot >> p.page_shift, row = slot & ((1 << p.page_shift) - 1);
+      _Float16 *dst = (_Float16 *)(is_v ? p.v_cache : p.k_cache) + page * p.pool.page + h * p.pool.head + row * p.pool.row;
+      store<W>(dst + c0, a);
+      store<W>(dst + c1, b);
+    }
   }
 }
 
-template <int D, typename IN>
-int launch(argus_hip_ctx *ctx, QkNormRopeParams &p, int tokens, bool out_f16, hipStream_t stream) {
-  constexpr int HPB = 256 / (D / 8);
-  p.chunks = (p.heads_q + 2 * p.heads_kv + HPB - 1) / HPB;
+template <int D, int W, typename IN, typename OUT>
+int launch(argus_hip_ctx *ctx, QkNormRopeParams &p, int tokens, hipStream_t stream) {
+  constexpr int HPB = 256 / (D / (2 * W));
+  const int chunks = (p.heads_q + 2 * p.heads_kv + HPB - 1) / HPB;
+  p.chunks = (int64_t)tokens * chunks <= (int64_t)ctx->compute_units * 8 ? chunks : 1;
   const int64_t grid = (int64_t)tokens * p.chunks;
   if (grid > 0x7fffffff) return argus_fail(ctx, ARGUS_HIP_ERR_UNSUPPORTED, "qk_norm_rope: too many tokens");
-  if (out_f16) hipLaunchKernelGGL((qk_norm_rope_kernel<D, IN, _Float16>), dim3((unsigned)grid), dim3(256), 0, stream, p);
-  else hipLaunchKernelGGL((qk_norm_rope_kernel<D, IN, float>), dim3((unsigned)grid), dim3(256), 0, stream, p);
+  hipLaunchKernelGGL((qk_norm_rope_kernel<D, W, IN, OUT>), dim3((unsigned)grid), dim3(256), 0, stream, p);
   ARGUS_HIP_CHECK(ctx, hipGetLastError());
   return ARGUS_HIP_OK;
 }
 
+template <int D, typename IN>
+int launch(argus_hip_ctx *ctx, QkNormRopeParams &p, int tokens, bool wide, bool out_f16, hipStream_t stream) {
+  if (wide) return out_f16 ? launch<D, 8, IN, _Float16>(ctx, p, tokens, stream) : launch<D, 8, IN, float>(ctx, p, tokens, stream);
+  return out_f16 ? launch<D, 4, IN, _Float16>(ctx, p, tokens, stream) : launch<D, 4, IN, float>(ctx, p, tokens, stream);
+}
+
 template <int D>
-int launch(argus_hip_ctx *ctx, QkNormRopeParams &p, int tokens, bool in_f16, bool out_f16, hipStream_t stream) {
-  return in_f16 ? launch<D, _Float16>(ctx, p, tokens, out_f16, stream) : launch<D, float>(ctx, p, tokens, out_f16, stream);
+int launch(argus_hip_ctx *ctx, QkNormRopeParams &p, int tokens, bool wide, bool in_f16, bool out_f16, hipStream_t stream) {
+  return in_f16 ? launch<D, _Float16>(ctx, p, tokens, wide, out_f16, stream) : launch<D, float>(ctx, p, tokens, wide, out_f16, stream);
 }
 
 }  // namespace
@@ -190,9 +216,12 @@ ARGUS_API int argus_hip_qk_norm_rope(argus_hip_ctx *ctx, const argus_hip_qk_norm
   p.eps = a->eps, p.weight_bias = a->weight_bias;
   const bool in_f16 = a->in_dtype == ARGUS_HIP_F16, out_f16 = a->out_dtype == ARGUS_HIP_F16;
   const hipStream_t stream = (hipStream_t)a->stream;
+  // groups of eight channels (16-byte accesses of F16) where the rotation's halves and every row allow it
+  const bool wide = a->rot_dim % 16 == 0 && (p.q_stride | p.k_stride | p.v_stride | p.q_out_stride) % 8 == 0 &&
+                    (((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v | (uintptr_t)a->q_out) & 15) == 0;
   switch (d) {
-    case 64: return launch<64>(ctx, p, a->tokens, in_f16, out_f16, stream);
-    case 128: return launch<128>(ctx, p, a->tokens, in_f16, out_f16, stream);
-    default: return launch<256>(ctx, p, a->tokens, in_f16, out_f16, stream);
+    case 64: return launch<64>(ctx, p, a->tokens, wide, in_f16, out_f16, stream);
+    case 128: return launch<128>(ctx, p, a->tokens, wide, in_f16, out_f16, stream);
+    default: return launch<256>(ctx, p, a->tokens, wide, in_f16, out_f16, stream);
   }
 }
