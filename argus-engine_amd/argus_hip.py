@@ -447,36 +447,31 @@ def _refuse(what, device, t, dtype):
     raise ValueError(what + ": lengths, tables, weights, pools and workspaces are contiguous")
 
 
-def _packed(what, device, dtype, *tensors):
-    """Their addresses (0 for None): contiguous tensors of one dtype on the context's device."""
-    found = []
-    for t in tensors:
-        if t is None:
-            found.append(0)
-            continue
-        if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
-            _refuse(what, device, t, dtype)
-        found.append(t.data_ptr())
-    return found
+def _packed(what, device, dtype, t):
+    """The address of a contiguous tensor of `dtype` on the context's device."""
+    if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
+        _refuse(what, device, t, dtype)
+    return t.data_ptr()
 
 
-def _heads(what, device, dtype, heads, d, t):
+def _heads(what, device, dtype, tokens, heads, d, t):
     """(address, elements between tokens) of [tokens, heads, d] with packed heads."""
     if t.dtype is not dtype or t.get_device() != device:
         _refuse(what, device, t, dtype)
     token, head, one = t.stride()
     if (one != 1 and d > 1) or (head != d and heads > 1):
         raise ValueError(what + ": the heads of a token must be packed")
-    return t.data_ptr(), token if t.shape[0] > 1 else heads * d
+    return t.data_ptr(), token if tokens > 1 else heads * d
 
 
 def _pool(what, device, k, v, layout, hkv, d):
-    """(addresses, n_pages, page_size) of a pair of page pools."""
-    n, a, b, e = k.shape
+    """(addresses of the two, n_pages, KV heads, page_size) of a pair of page pools; hkv 0: any."""
+    shape = k.shape
+    n, a, b, e = shape
     heads, size = (a, b) if layout == HEAD_MAJOR else (b, a)
-    if k.shape != v.shape or e != d or (hkv is not None and heads != hkv):
+    if v.shape != shape or e != d or (hkv and heads != hkv):
         raise ValueError(what + ": the pools belong to other heads")
-    return _packed(what, device, torch.float16, k, v), n, heads, size
+    return _packed(what, device, torch.float16, k), _packed(what, device, torch.float16, v), n, heads, size
 
 
 _FLOATS = {torch.float32: F32, torch.float16: F16}
@@ -754,7 +749,8 @@ class Context:
         """Device int32 tensors: past_len, new_len, kv_len [n], free_pages [f], page_table [n, c] (in place), cu_new [n + 1],
         positions and slots [token_capacity], counts [3]."""
         dev = self.device
-        ptrs = _packed("page_plan", dev, torch.int32, past_len, new_len, free_pages, page_table, cu_new, kv_len, positions, slots, counts)
+        ptrs = [0 if x is None else _packed("page_plan", dev, torch.int32, x)
+                for x in (past_len, new_len, free_pages, page_table, cu_new, kv_len, positions, slots, counts)]
         n, tokens = past_len.numel(), positions.numel()
         rows, width = page_table.shape
         if (new_len.numel() != n or kv_len.numel() != n or cu_new.numel() != n + 1 or counts.numel() != 3 or rows != n
@@ -769,41 +765,53 @@ class Context:
         argus_hip.h; cos_sin [n_positions, rot_dim] F32 or None (no rotation); positions, slots [t] int32."""
         what, dev, ty = "qk_norm_rope", self.device, q.dtype
         in_dtype, out_dtype = _float(what, q), _float(what, q_out)
-        t, hq, d = q.shape
-        hkv = k.shape[1]
-        pools, n_pages, _, page_size = _pool(what, dev, k_cache, v_cache, layout, hkv, d)
-        if k.shape != (t, hkv, d) or v.shape != k.shape or q_out.shape != q.shape:
+        shape, kv_shape = q.shape, k.shape
+        t, hq, d = shape
+        hkv = kv_shape[1]
+        kc, vc, n_pages, _, page_size = _pool(what, dev, k_cache, v_cache, layout, hkv, d)
+        if kv_shape[0] != t or kv_shape[2] != d or v.shape != kv_shape or q_out.shape != shape:
             raise ValueError("qk_norm_rope: shapes do not belong together")
-        (qp, qs), (kp, ks), (vp, vs) = _heads(what, dev, ty, hq, d, q), _heads(what, dev, ty, hkv, d, k), _heads(what, dev, ty, hkv, d, v)
-        op, os_ = _heads(what, dev, q_out.dtype, hq, d, q_out)
-        wq, wk, cs = _packed(what, dev, torch.float32, q_weight, k_weight, cos_sin)
-        pos, slot = _packed(what, dev, torch.int32, positions, slots)
+        qp, qs = _heads(what, dev, ty, t, hq, d, q)
+        kp, ks = _heads(what, dev, ty, t, hkv, d, k)
+        vp, vs = _heads(what, dev, ty, t, hkv, d, v)
+        op, os_ = _heads(what, dev, q_out.dtype, t, hq, d, q_out)
+        wq = 0 if q_weight is None else _packed(what, dev, torch.float32, q_weight)
+        wk = 0 if k_weight is None else _packed(what, dev, torch.float32, k_weight)
+        slot = _packed(what, dev, torch.int32, slots)
+        pos = 0 if positions is None else _packed(what, dev, torch.int32, positions)
         if slots.numel() != t or (pos and positions.numel() != t):
             raise ValueError("qk_norm_rope: one position and one slot per token")
         if (wq and q_weight.numel() != d) or (wk and k_weight.numel() != d):
             raise ValueError("qk_norm_rope: a weight has head_dim elements")
-        n_pos, rot = (0, 0) if cos_sin is None else cos_sin.shape
+        cs = n_pos = rot = 0
+        if cos_sin is not None:
+            cs = _packed(what, dev, torch.float32, cos_sin)
+            n_pos, rot = cos_sin.shape
         return self._check(_qk_norm_rope(
-            self.handle, _raw_stream(dev), qp, kp, vp, wq, wk, cs, pos, slot, op, pools[0], pools[1], qs, ks, vs, os_, t, hq, hkv, d, rot,
+            self.handle, _raw_stream(dev), qp, kp, vp, wq, wk, cs, pos, slot, op, kc, vc, qs, ks, vs, os_, t, hq, hkv, d, rot,
             1 if interleaved else 0, n_pos, n_pages, page_size, layout, in_dtype, out_dtype, eps, weight_bias), check)
 
     def _paged(self, fn, q, k_cache, v_cache, page_table, cu_new, kv_len, out, max_new, max_kv, min_new, softcap, scale, window, layout,
                workspace, check):
-        what, dev = "paged_attention", self.device
+        what, dev, ty = "paged_attention", self.device, q.dtype
         dtype = _float(what, q)
-        t, hq, d = q.shape
-        pools, n_pages, hkv, page_size = _pool(what, dev, k_cache, v_cache, layout, None, d)
-        table, cu, kv = _packed(what, dev, torch.int32, page_table, cu_new, kv_len)
-        (qp, qs), (op, os_) = _heads(what, dev, q.dtype, hq, d, q), _heads(what, dev, q.dtype, hq, d, out)
+        shape = q.shape
+        t, hq, d = shape
+        kc, vc, n_pages, hkv, page_size = _pool(what, dev, k_cache, v_cache, layout, 0, d)
+        table = _packed(what, dev, torch.int32, page_table)
+        cu = _packed(what, dev, torch.int32, cu_new)
+        kv = _packed(what, dev, torch.int32, kv_len)
+        qp, qs = _heads(what, dev, ty, t, hq, d, q)
+        op, os_ = _heads(what, dev, ty, t, hq, d, out)
         n = kv_len.numel()
         rows, width = page_table.shape
-        if cu_new.numel() != n + 1 or rows != n or out.shape != q.shape:
+        if cu_new.numel() != n + 1 or rows != n or out.shape != shape:
             raise ValueError("paged_attention: shapes do not belong together")
-        ws, ws_bytes = 0, 0
+        ws = ws_bytes = 0
         if workspace is not None:
-            (ws,), ws_bytes = _packed(what, dev, workspace.dtype, workspace), workspace.numel() * workspace.element_size()
-        return self._check(fn(self.handle, _raw_stream(dev), qp, pools[0], pools[1], table, cu, kv, op, ws, ws_bytes, qs, os_, n, t, hq, hkv,
-                              d, n_pages, page_size, width, layout, dtype, min_new, max_new, max_kv, window, softcap, scale), check)
+            ws, ws_bytes = _packed(what, dev, workspace.dtype, workspace), workspace.numel() * workspace.element_size()
+        return self._check(fn(self.handle, _raw_stream(dev), qp, kc, vc, table, cu, kv, op, ws, ws_bytes, qs, os_, n, t, hq, hkv, d, n_pages,
+                              page_size, width, layout, dtype, min_new, max_new, max_kv, window, softcap, scale), check)
 
     def paged_attention(self, q, k_cache, v_cache, page_table, cu_new, kv_len, out, max_new=0, max_kv=0, min_new=0, softcap=0.0,
                         scale=0.0, window=0, layout=HEAD_MAJOR, workspace=None, check=True):

@@ -42,7 +42,7 @@ __device__ __forceinline__ half4_t load_stream<half4_t>(__amdgpu_buffer_rsrc_t r
 }
 
 template <int D, typename T, bool CAP>
-__global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(const PagedParams p) {
+__global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(const PagedParams p) {
   using SH = DecodeShape<D>;
   constexpr int KK = SH::KK, VC = SH::VC, VSEG = SH::VSEG, NACC = SH::NACC, TW = SH::TW;
   constexpr int STEP = 16 * TW;
@@ -110,33 +110,41 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(const PagedPa
         for (int sg = 0; sg < VSEG; ++sg) vr[tw][sg][e] = load_stream<vpiece_t>(rsrc, v_lane + e * row_bytes + 32 * VC * sg, row_off[tw]);
     }
   };
+  // Q: lane (j, r) holds chunk 4 kk + j of row r.  Requested ahead of the first keys and waited for ahead of
+  // the loop: a wait for the query inside it would be one for everything requested since.
+  half8_t qh[KK], ql[F32 ? KK : 1];
+  const T *qp = (const T *)p.q + (int64_t)(it.s.q_begin + rr / G) * p.q_stride + (int64_t)(kvh * G + rr % G) * D + 8 * j;
+  float qx[F32 ? KK : 1][8];
+#pragma unroll
+  for (int kk = 0; kk < KK; ++kk) {
+    if constexpr (F32) {
+      const float4_t a = *(const float4_t *)(qp + 32 * kk), b = *(const float4_t *)(qp + 32 * kk + 4);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) qx[kk][e] = e < 4 ? a[e] : b[e - 4];
+    } else {
+      qh[kk] = *(const half8_t *)(qp + 32 * kk);
+    }
+  }
+  __builtin_amdgcn_sched_barrier(0);
   const int base0 = begin + wave * STEP;
   load_k(base0);
   load_v();
-
-  // Q: lane (j, r) holds chunk 4 kk + j of row r
-  half8_t qh[KK], ql[F32 ? KK : 1];
-  {
-    const T *qp = (const T *)p.q + (int64_t)(it.s.q_begin + rr / G) * p.q_stride + (int64_t)(kvh * G + rr % G) * D;
+  __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      if constexpr (F32) {
-        float x[8];
+  for (int kk = 0; kk < KK; ++kk) {
+    if constexpr (F32) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = qp[(4 * kk + j) * 8 + e];
-        loaded8(x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          _Float16 hi, lo;
-          split_f16(CAP ? x[e] * p.scale : x[e] * c, hi, lo);
-          qh[kk][e] = hi;
-          ql[kk][e] = lo;
-        }
-      } else {
-        qh[kk] = *(const half8_t *)(qp + (4 * kk + j) * 8);
+      for (int e = 0; e < 8; ++e) {
+        _Float16 hi, lo;
+        split_f16(CAP ? qx[kk][e] * p.scale : qx[kk][e] * c, hi, lo);
+        qh[kk][e] = hi;
+        ql[kk][e] = lo;
       }
+    } else {
+      asm volatile("" : "+v"(qh[kk]));
     }
   }
+
 
   float4_t o_acc[NACC];
 #pragma unroll
@@ -162,21 +170,28 @@ __global__ __launch_bounds__(64 * kWaves) void paged_decode_kernel(const PagedPa
     load_k(base + kWaves * STEP);
     // keys some row does not see: past the first token's position, in front of the last one's window, past the part
     const bool edge = base + STEP - 1 > it.s.pos0 || base + STEP > end || (window != 0x7fffffff && base <= pos_last - window);
-    float mt = kNegInf;
 #pragma unroll
     for (int tw = 0; tw < TW; ++tw)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float x = s[tw][i];
-        if constexpr (CAP) x = soft_cap<F32>(F32 ? x : x * p.scale, p.softcap, inv_cap) * kLog2e;
-        else if constexpr (!F32) x *= c;
-        if (edge) {
-          const int key = base + 16 * tw + 4 * j + i;
-          if (key > pos || key >= end || (window != 0x7fffffff && key <= pos - window)) x = kNegInf;
-        }
-        s[tw][i] = x;
-        mt = fmaxf(mt, x);
+        if constexpr (CAP) s[tw][i] = soft_cap<F32>(F32 ? s[tw][i] : s[tw][i] * p.scale, p.softcap, inv_cap) * kLog2e;
+        else if constexpr (!F32) s[tw][i] *= c;
       }
+    if (edge) {
+      const int hi = min(pos, end - 1), lo = window != 0x7fffffff ? pos - window : -1;
+#pragma unroll
+      for (int tw = 0; tw < TW; ++tw)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = base + 16 * tw + 4 * j + i;
+          s[tw][i] = key <= hi && key > lo ? s[tw][i] : kNegInf;
+        }
+    }
+    float mt = kNegInf;
+#pragma unroll
+    for (int tw = 0; tw < TW; ++tw)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) mt = fmaxf(mt, s[tw][i]);
     mt = rows_allreduce_max(mt);
     const float m_new = fmaxf(m_run, mt);
     const float m_ref = m_new == kNegInf ? 0.0f : m_new;
