@@ -118,7 +118,7 @@ __global__ __launch_bounds__(kThreads) void page_plan_kernel(const PagePlanParam
           p.cu_new[s] = at_t;
           p.kv_len[s] = len;
           const int64_t room = (int64_t)p.table_stride << p.page_shift;
-          shorts += fresh[i] > 0 && (len > room || (need[i] > 0 && sat_add(at_p, need[i]) > p.n_free));
+          shorts += fresh[i] > 0 && (len > room || (need[i] > 0 && new_page(p, sat_add(at_p, need[i]) - 1) < 0));
         }
       }
       at_t = sat_add(at_t, fresh[i]);

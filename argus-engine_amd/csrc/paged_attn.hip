@@ -614,8 +614,13 @@ int make_plan(argus_hip_ctx *ctx, int compute_units, const argus_hip_paged_atten
     c.align = chunk_align(d);
     c.min_share = 512;
     const int64_t tiles = sched_tiles_bound(c, a->min_new);
-    c.target = std::max(1, compute_units * 2 / a->heads_kv);
-    c.cut_cost = d == 64 ? 900 : 500;                    // keys a workgroup gets through in 15 us
+    const int resident = d <= 128 ? 2 : 1;               // workgroups per compute unit
+    c.target = std::max(1, compute_units * resident / a->heads_kv);
+    c.alone = resident == 2 ? compute_units / a->heads_kv : 0;
+    // in keys a workgroup gets through meanwhile.  Measured over prompts of 512 to 8192 tokens and chunks of
+    // 64 to 700 behind up to 8192: half or twice as much lose up to 30 % somewhere (700 tokens behind 2300 at
+    // d 64 37 -> 49 us with 1800, 2048 tokens at d 128 66 -> 77 us with 500, at d 256 64 -> 100 us with 1600).
+    c.cut_cost = d == 64 ? 1300 : d == 128 ? 1100 : 700;
     if (longest + 96 <= c.min_share) c.cut_cost = -1;    // tiles too short to be cut
     if (tiles == 0) pl.chunk = false;                    // too few rows for any request of this class
     pl.c_items = sched_items_bound(c, tiles);

@@ -27,6 +27,7 @@ struct PagedSched {
   int32_t align;                 // key ranges start on a multiple of this
   int32_t min_share;             // a share is not smaller than this
   int32_t target;                // shares per KV head
+  int32_t alone;                 // up to this many shares per KV head run without another on their compute unit: ~0.6 of the time
   int32_t cut_cost;              // what cutting costs a call: further starts, partial results, the merge; < 0: no tile is cut
   int32_t window, max_len;       // max_len: keys the page table has room for
 };
@@ -96,7 +97,8 @@ ARGUS_HD int64_t sched_share(const PagedSched &c, int64_t work) {
 ARGUS_HD bool sched_whole(const PagedSched &c, int64_t tiles, int64_t work, int64_t longest) {
   if (c.cut_cost < 0 || tiles == 0) return true;
   const double rounds = (double)((tiles + c.target - 1) / c.target) * ((double)work / (double)tiles);
-  const double whole = rounds > (double)longest ? rounds : (double)longest;
+  double whole = rounds > (double)longest ? rounds : (double)longest;
+  if (tiles <= c.alone) whole *= 0.6;
   return whole <= (double)work / c.target + c.cut_cost;
 }
 
@@ -153,8 +155,9 @@ __device__ __forceinline__ int64_t lane_value(int64_t x, int l) {
 // A tile on the line of work.
 struct PagedPlace {
   PagedSeq s;
-  int32_t seq, tile;
-  int64_t start, cost;  // of the tile, on the line
+  int32_t seq, tile, left;  // left: further tiles of the request
+  int64_t start, cost;      // of the tile, on the line
+  int64_t slope;            // cost of the request's next tile above this one's
 };
 
 // A block of 64 requests, one per lane.
@@ -210,6 +213,8 @@ struct PagedBlock {
   __device__ __forceinline__ void place(int b, int l, const PagedCost &cost, int tile, int64_t before, PagedPlace &out) const {
     out.tile = tile;
     out.seq = b + l;
+    out.left = cost.tiles - 1 - tile;
+    out.slope = cost.slope;
     out.start = before + sched_before(cost, tile);
     out.cost = cost.base + cost.slope * tile;
     out.s.q_begin = lane_value(s.q_begin, l);
@@ -267,8 +272,16 @@ struct PagedShare {
   __device__ __forceinline__ int64_t upto() const { return whole ? at.cost : end - at.start < at.cost ? end - at.start : at.cost; }
   __device__ __forceinline__ void next(const PagedSched &c, const int32_t *cu, const int32_t *kv) {
     x = whole ? end : at.start + at.cost;
-    found = false;
-    if (x < end) search(c, cu, kv, 0, 0);
+    if (x >= end) {
+      found = false;
+    } else if (at.left > 0) {
+      ++at.tile;
+      --at.left;
+      at.start = x;
+      at.cost += at.slope;
+    } else {
+      search(c, cu, kv, 0, 0);
+    }
   }
 };
 

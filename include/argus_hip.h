@@ -659,7 +659,8 @@ int argus_hip_kv_scatter_f32_batch(argus_hip_ctx *ctx, void *stream, const float
 /* One step of a scheduler over n_seqs requests, request s bringing new_len[s] tokens (0: idle this
  * step) behind past_len[s] cached ones.  Rows of page_table hold ceil(past_len / page_size) pages on
  * entry; the pages the new tokens need are taken from the front of free_pages in request order and
- * appended (-1 where the list is exhausted).  With need_s the pages of request s:
+ * appended (-1 where the list is exhausted).  A list of fixed size ends with -1s, or other numbers outside
+ * the pool: they are no pages.  With the pages appended:
  *   cu_new[s] = sum of new_len before s (cu_new[n_seqs] = total), kv_len[s] = past_len[s] + new_len[s];
  *   token t = cu_new[s] + i: positions[t] = past_len[s] + i,
  *     slots[t] = page * page_size + position % page_size, -1 for a token without a page;

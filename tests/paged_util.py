@@ -21,7 +21,7 @@ def plan(past, new, free, table, page, n_pages, capacity):
         for i in range(need):
             f = int(free[taken + i]) if taken + i < len(free) else -1
             table[s, had + i] = f if 0 <= f < n_pages else -1
-        short += bool(y and (x + y > width * page or (need and taken + need > len(free))))
+        short += bool(y and (x + y > width * page or (need and table[s, had + need - 1] < 0)))
         taken += need
         kv.append(x + y)
         for i in range(y):
