@@ -1,570 +1,15 @@
 // Causal GQA attention of the new tokens of many requests over their pages (include/argus_hip.h,
-// argus_hip_paged_attention): the chunk kernel, the merge of requests cut along their length, and the
-// entry point.  Requests of at most 16 rows (tokens x heads of a group) take the decode kernel of
-// paged_decode.hip.
+// argus_hip_paged_attention): checks, the plan of a call, and the entry points.  Kernels: paged_launch.hpp.
 //
 //   s_c = cap((q . k_c) * scale) for the visible keys c of a row;  out = sum_c softmax(s)_c v_c
-//
-// Chunk kernel: one workgroup = 128 rows of one KV head, four waves of 32.  A row is a (token, head of the
-// group) pair, so the whole group shares each K / V tile and a short chunk fills its rows with heads.
-// v_mfma_f32_32x32x16_f16 in the transposed form
-//     S^T = K . Q^T  (A = K rows from LDS, B = Q rows in registers)
-//     O^T = V^T . P^T (A = V^T through a transposing LDS read, B = the S^T accumulators' own layout)
-// a lane owns one row: the softmax is in-lane plus one exchange between the wave's halves, the running
-// maximum and sum are F32, and P never goes through LDS.
 #include "paged_common.hpp"
 
 #include <algorithm>
 #include <cmath>
-#include <type_traits>
 
 namespace argus_paged {
 
 namespace {
-
-typedef float float16_t __attribute__((ext_vector_type(16)));
-
-__device__ __forceinline__ half4_t lds_read_tr16(const _Float16 *p) {
-  typedef short short4_t __attribute__((ext_vector_type(4)));
-  typedef __attribute__((address_space(3))) short4_t lds_short4_t;
-  return __builtin_bit_cast(half4_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4_t *)p));
-}
-
-template <int D, bool F32>
-struct ChunkTile {
-  static constexpr int BN = chunk_align(D);            // keys per tile
-  static constexpr int KP = D + 8, VP = D + 32;        // row pitches (halfs): no bank is hit twice by one read
-  static constexpr int LDS_BYTES = 2 * BN * (KP + VP) * 2;  // two buffers each of K and V tiles
-  static constexpr bool DEEP = !F32 && D <= 128;       // tiles are requested a step earlier (registers allow a second set)
-  static constexpr int WAVES_PER_SIMD = D <= 128 ? 2 : 1;
-};
-
-// Software pipeline of a wave, as the logits of tile t + 1 are formed while tile t is exponentiated:
-//   phase A   S(t+1) = K . Q^T on the matrix cores  beside  the second half of tile t's exponentials
-//   phase B   O += V . P(t)                         beside  the first half of tile t + 1's
-// K tiles are staged in LDS two steps ahead, V tiles one; one barrier per step.  Interior steps -- every row
-// of the workgroup sees all of tiles t and t + 1 -- carry no masks and take no maximum: their exponents
-// stand against a reference some earlier tile of the row set, and a probability only leaves F16's range
-// where a logit exceeds it by 16 (log2), which shows in the row sum.
-template <int D, typename T, bool CAP>
-__global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::WAVES_PER_SIMD)) void paged_chunk_kernel(const PagedParams p) {
-  constexpr bool F32 = std::is_same<T, float>::value;
-  using TL = ChunkTile<D, F32>;
-  constexpr int BN = TL::BN, KP = TL::KP, VP = TL::VP;
-  constexpr int KK = D / 16, KB = BN / 32, RB = D / 32, PS = BN / 16;  // logits MFMAs per 32 keys, row blocks of S^T and O^T, P^T slices
-  constexpr int CH = BN * D / 8 / 256;  // 16-byte pieces of a K (or V) tile per thread
-  constexpr int RPW = 64 / (D / 8);     // rows of a piece that one wave covers
-  constexpr bool DEEP = TL::DEEP;
-  constexpr int SETS = DEEP ? 2 : 1;
-  constexpr float kLog2e = 1.4426950408889634f;
-  constexpr int kSplit = PS / 2;        // slices of P^T formed in phase B of the step before
-  constexpr int kAhead = 4, kVAhead = D <= 64 ? 4 : 3;  // operand reads kept in flight
-  
-  extern __shared__ __attribute__((aligned(16))) _Float16 smem[];
-  _Float16 *const sK = smem, *const sV = smem + 2 * BN * KP;  // [2][BN][KP], [2][BN][VP]
-  __shared__ int bad_tile[2];  // tile whose V held infinities or NaN under a mask
-
-  const int kvh = blockIdx.x % p.heads_kv, w = blockIdx.x / p.heads_kv;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int ln = lane & 31, hl = lane >> 5;
-  const int G = p.sched.group;
-  const bool windowed = p.sched.window > 0;
-  const int window = p.sched.window;
-  const int page_mask = (1 << p.page_shift) - 1;
-  const uint32_t row_bytes = (uint32_t)p.pool.row * 2;
-  const int my_row = lane / (D / 8), my_col = lane % (D / 8);
-  const uint32_t lane_off = my_row * row_bytes + 16 * my_col;
-  const PagePool k_pool(p.k, p, kvh, D), v_pool(p.v, p, kvh, D);
-  // exponents are logit * ce - m_ref (CAP: of the capped logit); a negative scale turns the queries round instead
-  const float ce = CAP ? kLog2e : __builtin_fabsf(p.scale) * kLog2e;
-  const float q_sign = p.scale < 0.0f ? -1.0f : 1.0f;
-  const float cap = p.softcap, cap_in = CAP ? __builtin_fabsf(p.scale) / p.softcap : 0.0f;  // cap * tanh(product * cap_in)
-  // V^T operand: ds_read_b64_tr_b16 gives lane i of 16 channel ch0 + i of keys key0 .. key0 + 3 when lane s
-  // addresses V[key0 + s / 4][ch0 + 4 (s % 4)]; P^T holds keys 4 hl + {0..3} and 8 + 4 hl + {0..3} of 16
-  const int g16 = lane >> 4, s16 = lane & 15;
-  const int vlane_off = (4 * (g16 >> 1) + (s16 >> 2)) * VP + 16 * (g16 & 1) + 4 * (s16 & 3);
-
-  PagedCut cut{0, 0, 0, 0};
-  PagedShare work(p.sched, p.cu_new, p.kv_len, w);
-  while (work.found) {  // the tiles this share touches
-  const PagedPlace it = work.at;
-  const int64_t from = work.from(), upto = work.upto();
-  const bool entire = from == 0 && upto == it.cost;
-  const int slot = 2 * w + (from == 0 ? 1 : 0);
-  const int n_rows = (int)std::min<int64_t>((int64_t)(it.s.q_end - it.s.q_begin) * G, 0x7fffffff);
-  const int row0 = it.tile * kChunkRows;
-  const int row_last = min(n_rows, row0 + kChunkRows) - 1;
-  if (!entire && from == 0) cut = PagedCut{(int)((it.start + it.cost - 1) / work.share) - w + 1, it.s.q_begin, row0, row_last + 1 - row0};
-
-  const int row = row0 + 32 * wave + ln;
-  const bool row_ok = row < n_rows;
-  const int rr = min(row, row_last);  // rows past the last one repeat it and are not stored
-  const int tok = rr / G, head = kvh * G + rr % G;
-  const int pos = it.s.pos0 + tok;
-  const int wg_first = it.s.pos0 + row0 / G, wg_last = it.s.pos0 + row_last / G;  // positions of the workgroup's rows
-
-  // keys the tile's rows see, and this part of them
-  const int key_end = min(it.s.len, max(wg_last, -1) + 1);
-  const int key_begin = windowed && wg_first >= window ? (wg_first - window + 1) / BN * BN : 0;
-  const int n_tiles = key_end > key_begin ? (key_end - key_begin + BN - 1) / BN : 0;
-  const int t0 = (int)((double)from * n_tiles / it.cost), n_it = (int)((double)upto * n_tiles / it.cost) - t0;
-  const int base0 = key_begin + t0 * BN;
-  const int part_end = min(key_end, base0 + n_it * BN);
-  // key tiles that every row sees whole
-  const int full_from = windowed && wg_last >= window ? max(0, (wg_last - window + BN - base0) / BN) : 0;
-  const int full_upto = min(n_it, max(0, min(wg_first + 1, key_end) - base0) / BN);
-
-  // ---- tiles: a wave fetches BN / 4 consecutive rows, which lie in one page, in CH pieces of 16 bytes per lane
-  constexpr int SPAN = BN / 16;  // pages a tile touches at most
-  static_assert(BN / 4 <= 16, "a wave's rows of a tile lie in one page");
-  PageWindow pages;
-  pages.start<SPAN>(p, it.seq, base0 >> p.page_shift);
-  half8_t kpre[SETS][CH], vpre[SETS][CH];
-  uint64_t page_off = 0;  // of the K tile requested last; its V tile follows a step later
-  uint32_t row_off = 0;
-  auto fetch_k = [&](int t, half8_t(&pre)[CH]) __attribute__((always_inline)) {  // behind the part: its last page again
-    const int base = base0 + t * BN, key = base + wave * (BN / 4);
-    pages.advance<SPAN>(min(base, part_end - 1) >> p.page_shift);
-    page_off = pages.offset(min(key, part_end - 1) >> p.page_shift);
-    row_off = (uint32_t)(key & page_mask) * row_bytes;
-    const __amdgpu_buffer_rsrc_t rows = k_pool.rows(page_off);
-#pragma unroll
-    for (int i = 0; i < CH; ++i)
-      pre[i] = __builtin_bit_cast(half8_t, __builtin_amdgcn_raw_buffer_load_b128(rows, lane_off, row_off + i * (RPW * row_bytes), 0));
-  };
-  auto fetch_v = [&](half8_t(&pre)[CH]) __attribute__((always_inline)) {  // of the K tile requested last
-    const __amdgpu_buffer_rsrc_t rows = v_pool.rows(page_off);
-#pragma unroll
-    for (int i = 0; i < CH; ++i)
-      pre[i] = __builtin_bit_cast(half8_t, __builtin_amdgcn_raw_buffer_load_b128(rows, lane_off, row_off + i * (RPW * row_bytes), 0));
-  };
-  const int stage_row = wave * (BN / 4) + my_row;
-  auto stage_k = [&](auto buf_c, half8_t(&pre)[CH]) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < CH; ++i)
-      *(half8_t *)(sK + stage_row * KP + 8 * my_col + (decltype(buf_c)::value * BN + RPW * i) * KP) = pre[i];
-  };
-  auto stage_v = [&](auto buf_c, int t, half8_t(&pre)[CH], bool seen_whole) __attribute__((always_inline)) {  // tile t into buffer t % 2
-    if (!seen_whole) {
-      // A weight of zero does not keep an infinity or a NaN out of the product: such values of V leave the
-      // tile here and are added, by themselves, to the rows that see their key.
-      bool bad = false;
-#pragma unroll
-      for (int i = 0; i < CH; ++i)
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-          if (not_finite(pre[i][e])) {
-            bad = true;
-            pre[i][e] = (_Float16)0.0f;
-          }
-      if (bad) bad_tile[decltype(buf_c)::value] = t;
-    }
-#pragma unroll
-    for (int i = 0; i < CH; ++i)
-      *(half8_t *)(sV + stage_row * VP + 8 * my_col + (decltype(buf_c)::value * BN + RPW * i) * VP) = pre[i];
-  };
-  auto seen_whole = [&](int t) __attribute__((always_inline)) { return t >= full_from && t < full_upto; };
-
-  // ---- Q as the B operand: lane (row ln, half hl) holds channels 16 kk + 8 hl .. + 7
-  half8_t qh[KK], ql[F32 ? KK : 1];
-  auto load_q = [&]() __attribute__((always_inline)) {
-    const T *qp = (const T *)p.q + (int64_t)(it.s.q_begin + tok) * p.q_stride + (int64_t)head * D + 8 * hl;
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-      if constexpr (F32) {
-        const float4_t a = *(const float4_t *)(qp + 16 * kk), b = *(const float4_t *)(qp + 16 * kk + 4);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          _Float16 hi, lo;
-          split_f16((e < 4 ? a[e] : b[e - 4]) * q_sign, hi, lo);
-          qh[kk][e] = hi;
-          ql[kk][e] = lo;
-        }
-      } else {
-        qh[kk] = *(const half8_t *)(qp + 16 * kk);
-        if (q_sign < 0.0f) qh[kk] = -qh[kk];
-      }
-    }
-  };
-
-  float16_t o_acc[RB];
-#pragma unroll
-  for (int r = 0; r < RB; ++r)
-#pragma unroll
-    for (int i = 0; i < 16; ++i) o_acc[r][i] = 0.0f;
-  float m_run = kNegInf, m_ref = 0.0f, l_run = 0.0f;  // m_ref: what exponents stand against; m_run the same, -inf while no key was seen
-
-  typedef float16_t STile[KB];
-  typedef half8_t PTile[PS];
-  auto qk_tile = [&](auto buf_c, STile &s) __attribute__((always_inline)) {
-    const _Float16 *kt = sK + ln * KP + 8 * hl + decltype(buf_c)::value * BN * KP;
-#pragma unroll
-    for (int kk = 0; kk < KK; ++kk)
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb) {
-        const half8_t a = *(const half8_t *)(kt + 32 * kb * KP + 16 * kk);
-        s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qh[kk], kk == 0 ? float16_t{0.0f} : s[kb], 0, 0, 0);
-        if constexpr (F32) s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ql[kk], s[kb], 0, 0, 0);
-      }
-  };
-  // Order of a phase, given once its code has been emitted: operand reads a few MFMAs ahead.  (Placing the
-  // exponentials behind the MFMAs as well made no difference at d 128 and cost 4 % at d 256.)
-  auto sched_qk = [&]() __attribute__((always_inline)) {
-    constexpr int N = KK * KB, AH = kAhead < N ? kAhead : N;
-    __builtin_amdgcn_sched_group_barrier(0x100, AH, 0);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, F32 ? 2 : 1, 0);
-      if (i < N - AH) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-    }
-  };
-  auto pv_tile = [&](auto buf_c, PTile &ph, PTile &pl) __attribute__((always_inline)) {
-    const _Float16 *vt = sV + vlane_off + decltype(buf_c)::value * BN * VP;
-#pragma unroll
-    for (int jn = 0; jn < PS; ++jn)
-#pragma unroll
-      for (int r = 0; r < RB; ++r) {
-        const _Float16 *vp = vt + 16 * jn * VP + 32 * r;
-        const half4_t lo = lds_read_tr16(vp), hi = lds_read_tr16(vp + 8 * VP);
-        const half8_t a = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-        o_acc[r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, ph[jn], o_acc[r], 0, 0, 0);
-        if constexpr (F32) o_acc[r] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, pl[jn], o_acc[r], 0, 0, 0);
-      }
-  };
-  auto sched_pv = [&]() __attribute__((always_inline)) {
-    constexpr int N = PS * RB, AH = kVAhead < N ? kVAhead : N;
-    __builtin_amdgcn_sched_group_barrier(0x100, 2 * AH, 0);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      __builtin_amdgcn_sched_group_barrier(0x008, F32 ? 2 : 1, 0);
-      if (i < N - AH) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
-    }
-  };
-  auto row_max = [&](STile &s, auto raw_c) __attribute__((always_inline)) {  // raw: products of q and k, not capped yet
-    float mt = kNegInf;
-#pragma unroll
-    for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) mt = fmaxf(mt, s[kb][i]);
-    mt = xor32_combine(mt, [](float a, float b) { return fmaxf(a, b); });
-    if constexpr (CAP && decltype(raw_c)::value) mt = soft_cap<F32>(mt, cap, cap_in);
-    return mt * ce;
-  };
-  constexpr float kLazy = 8.0f;
-  // Cap, mask and maximum of tile t.  The reference moves where a row's maximum exceeds it by more than
-  // kLazy (log2), or when the row sees its first key; the factor its sums take with it is returned.
-  auto mask_max = [&](auto buf_c, int t, STile &s) __attribute__((always_inline)) -> float {
-    const int base = base0 + t * BN;
-    if constexpr (CAP) {
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[kb][i] = soft_cap<F32>(s[kb][i], cap, cap_in);
-    }
-    if (!seen_whole(t)) {
-      const int hi = min(pos, key_end - 1), lo = windowed ? pos - window : -1;
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = base + 32 * kb + 8 * (i / 4) + 4 * hl + (i % 4);
-          s[kb][i] = key <= hi && key > lo ? s[kb][i] : kNegInf;
-        }
-    }
-    if constexpr (F32) {
-      // An infinite key times the two halves of a query is infinity minus infinity, or infinity times zero:
-      // where a logit is NaN, the high half alone says whether it is infinite.
-      float any = 0.0f;
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) any += s[kb][i];
-      if (__builtin_amdgcn_ballot_w64(any != any) != 0) {
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-          float16_t high = {0.0f};
-#pragma unroll
-          for (int kk = 0; kk < KK; ++kk)
-            high = __builtin_amdgcn_mfma_f32_32x32x16_f16(
-                *(const half8_t *)(sK + ln * KP + 8 * hl + (decltype(buf_c)::value * BN + 32 * kb) * KP + 16 * kk), qh[kk], high, 0, 0, 0);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float x = high[i];
-            if constexpr (CAP) x = soft_cap<F32>(x, cap, cap_in);
-            if (s[kb][i] != s[kb][i] && __builtin_isinf(high[i])) s[kb][i] = x;
-          }
-        }
-      }
-    }
-    const float mt = row_max(s, std::false_type{});
-    const bool first = m_run == kNegInf;
-    const float over = mt - m_ref;
-    const float delta = first ? (mt == kNegInf ? 0.0f : over) : over > kLazy ? over : 0.0f;
-    m_ref += delta;
-    if (!first || mt != kNegInf) m_run = m_ref;
-    return first ? 0.0f : __builtin_amdgcn_exp2f(-delta);
-  };
-  auto rescale = [&](float alpha) __attribute__((always_inline)) {
-    if (__builtin_amdgcn_ballot_w64(alpha != 1.0f) != 0) {
-#pragma unroll
-      for (int r = 0; r < RB; ++r)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o_acc[r][i] *= alpha;
-      l_run *= alpha;
-    }
-  };
-  // probabilities of slices [J0, J1) of a tile; returns their row sum (this half's keys)
-  auto exp_part = [&](STile &s, PTile &ph, PTile &pl, auto raw_c, auto j0_c, auto j1_c) __attribute__((always_inline)) -> float {
-    float sum = 0.0f;
-#pragma unroll
-    for (int jn = decltype(j0_c)::value; jn < decltype(j1_c)::value; ++jn) {
-      typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        float x = s[jn / 2][8 * (jn % 2) + e];
-        if constexpr (CAP && decltype(raw_c)::value) x = soft_cap<F32>(x, cap, cap_in);
-        x = __builtin_amdgcn_exp2f(__builtin_fmaf(x, ce, -m_ref));
-        if constexpr (F32) {
-          _Float16 hi, lo;
-          split_f16(x, hi, lo);
-          ph[jn][e] = hi;
-          pl[jn][e] = lo;
-          sum += x;
-        } else {
-          ph[jn][e] = (_Float16)x;
-        }
-      }
-      if constexpr (!F32) {
-        // the sum takes the rounded weights the matrix cores consume
-#pragma unroll
-        for (int e = 0; e < 8; e += 2) {
-          const half2_t pr = {ph[jn][e], ph[jn][e + 1]}, one = {(_Float16)1.0f, (_Float16)1.0f};
-          sum = __builtin_amdgcn_fdot2(pr, one, sum, false);
-        }
-      }
-    }
-    return sum;
-  };
-  typedef std::integral_constant<int, 0> J0;
-  typedef std::integral_constant<int, kSplit> JS;
-  typedef std::integral_constant<int, PS> JN;
-  // the infinities and NaN that were taken out of V tile t, to the rows that see them
-  auto add_bad = [&](int t) __attribute__((always_inline)) {
-    for (int k = 0; k < BN; ++k) {
-      const int key = base0 + t * BN + k;
-      if (key >= part_end) break;
-      const int number = pages.row[key >> p.page_shift];  // key < key_end <= the table's room
-      if ((uint32_t)number >= pages.n_pages) continue;
-      const _Float16 *vrow = (const _Float16 *)(v_pool.base + (uint64_t)(uint32_t)number * pages.page_bytes + (uint32_t)(key & page_mask) * row_bytes);
-      const bool sees = key <= pos && !(windowed && key <= pos - window);
-#pragma unroll
-      for (int r = 0; r < RB; ++r)
-#pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4) {
-          const half4_t x = *(const half4_t *)(vrow + 32 * r + 8 * i4 + 4 * hl);
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (sees && not_finite(x[e])) o_acc[r][4 * i4 + e] += (float)x[e];
-          __builtin_amdgcn_sched_barrier(0);  // a few conditions at a time: this path is rare and must not cost the common one registers
-        }
-    }
-  };
-
-  PTile p_a, p_b, p_lo;
-  float l_head = 0.0f;   // row sum of the slices formed early
-  // One step: on entry s_cur holds the logits of tile t (edge steps: masked, their reference set, the sums'
-  // factor in alpha; interior steps: the first slices of P formed).
-  auto step = [&](int t, STile &s_cur, STile &s_next, PTile &p_cur, PTile &p_next, float &alpha, auto interior_c, auto parity_c) __attribute__((always_inline)) {
-    constexpr bool INTERIOR = decltype(interior_c)::value;
-    typedef std::integral_constant<int, decltype(parity_c)::value> Buf;         // t % 2
-    typedef std::integral_constant<int, 1 - decltype(parity_c)::value> Other;
-    constexpr int FETCH = DEEP ? Buf::value : 0, STAGE = DEEP ? Other::value : 0;
-    constexpr int AHEAD = DEEP ? 1 : 0;
-    if constexpr (!INTERIOR) rescale(alpha);
-    fetch_v(vpre[FETCH]);                  // tile t + 1 + AHEAD
-    fetch_k(t + 2 + AHEAD, kpre[FETCH]);
-    qk_tile(Other{}, s_next);  // behind the last tile: of zeros, or of what is staged, and not used
-    if constexpr (INTERIOR) {
-      float sum = l_head + exp_part(s_cur, p_cur, p_lo, std::true_type{}, JS{}, JN{});
-      sched_qk();
-      if (__builtin_amdgcn_ballot_w64(!(sum < 1e30f)) != 0) {
-        const float over = row_max(s_cur, std::true_type{}) - m_ref, delta = over > kLazy ? over : 0.0f;
-        rescale(__builtin_amdgcn_exp2f(-delta));
-        m_ref += delta;
-        m_run = m_ref;
-        sum = exp_part(s_cur, p_cur, p_lo, std::true_type{}, J0{}, JN{});
-      }
-      l_run += sum;
-    } else {
-      sched_qk();
-      l_run += exp_part(s_cur, p_cur, p_lo, std::false_type{}, J0{}, JN{});
-    }
-    pv_tile(Buf{}, p_cur, p_lo);
-    if constexpr (INTERIOR) {
-      l_head = exp_part(s_next, p_next, p_lo, std::true_type{}, J0{}, JS{});
-      // formed here, beside the MFMAs, and not where they are first used
-#pragma unroll
-      for (int jn = 0; jn < kSplit; ++jn) asm volatile("" : "+v"(p_next[jn]));
-      asm volatile("" : "+v"(l_head));
-      sched_pv();
-    } else {
-      sched_pv();
-      if (!seen_whole(t) && bad_tile[Buf::value] == t) add_bad(t);
-      if (t + 1 < n_it) alpha = mask_max(Other{}, t + 1, s_next);
-    }
-    stage_k(Buf{}, kpre[STAGE]);
-    stage_v(Other{}, t + 1, vpre[STAGE], INTERIOR || seen_whole(t + 1));
-    __syncthreads();  // fills are visible; every wave is done with the buffers the next step refills
-  };
-
-  STile s_a, s_b;
-  if (threadIdx.x < 2) bad_tile[threadIdx.x] = -1;
-  if (n_it > 0) {
-    constexpr int S1 = DEEP ? 1 : 0;
-    typedef std::integral_constant<int, 0> Even;
-    typedef std::integral_constant<int, 1> Odd;
-    fetch_k(0, kpre[0]);
-    fetch_v(vpre[0]);
-    if constexpr (DEEP) fetch_k(1, kpre[1]);
-    __builtin_amdgcn_sched_barrier(0);
-    load_q();
-    __syncthreads();  // bad_tile
-    stage_k(Even{}, kpre[0]);
-    stage_v(Even{}, 0, vpre[0], seen_whole(0));
-    if constexpr (!DEEP) fetch_k(1, kpre[0]);
-    stage_k(Odd{}, kpre[S1]);
-    if constexpr (DEEP) {  // what step 0 stages at its end
-      fetch_v(vpre[1]);
-      fetch_k(2, kpre[1]);
-    }
-    __syncthreads();
-    qk_tile(Even{}, s_a);
-    sched_qk();
-    float alpha = mask_max(Even{}, 0, s_a);
-    __syncthreads();  // sK[0] is refilled by the first step
-    int t = 0;
-    const int n_int = full_from == 0 ? max(0, full_upto - 1) & ~1 : 0;  // steps whose tile and the next are seen whole
-    if (n_int > 0) {
-      if constexpr (CAP) {  // an interior step starts from products
-        qk_tile(Even{}, s_a);
-        __syncthreads();
-      }
-      l_head = exp_part(s_a, p_a, p_lo, std::true_type{}, J0{}, JS{});
-      for (; t < n_int; t += 2) {
-        step(t, s_a, s_b, p_a, p_b, alpha, std::true_type{}, Even{});
-        step(t + 1, s_b, s_a, p_b, p_a, alpha, std::true_type{}, Odd{});
-      }
-      // tile t has its logits but no maximum yet, and its early slices are formed again with the others
-      alpha = mask_max(Even{}, t, s_a);
-    }
-    for (; t < n_it; t += 2) {
-      step(t, s_a, s_b, p_a, p_a, alpha, std::false_type{}, Even{});
-      if (t + 1 < n_it) step(t + 1, s_b, s_a, p_a, p_a, alpha, std::false_type{}, Odd{});
-    }
-  }
-
-  l_run += __shfl_xor(l_run, 32, 64);
-  {
-  const PagedParams &p = params_again();
-  if (!entire) {
-    if (row_ok) {
-      const int64_t at = ((int64_t)slot * p.heads_kv + kvh) * kChunkRows + 32 * wave + ln;
-      float *o = p.ws_o + at * D;
-#pragma unroll
-      for (int r = 0; r < RB; ++r)
-#pragma unroll
-        for (int i4 = 0; i4 < 4; ++i4)
-          *(float4_t *)(o + 32 * r + 8 * i4 + 4 * hl) = float4_t{o_acc[r][4 * i4], o_acc[r][4 * i4 + 1], o_acc[r][4 * i4 + 2], o_acc[r][4 * i4 + 3]};
-      if (hl == 0) {
-        p.ws_ml[at * 2] = m_run;
-        p.ws_ml[at * 2 + 1] = l_run;
-      }
-    }
-  } else if (row_ok) {
-    const float inv = l_run == 0.0f ? 0.0f : 1.0f / l_run;
-    T *out = (T *)p.out + (int64_t)(it.s.q_begin + tok) * p.out_stride + (int64_t)head * D;
-#pragma unroll
-    for (int r = 0; r < RB; ++r)
-#pragma unroll
-      for (int i4 = 0; i4 < 4; ++i4) {
-        typedef T T4 __attribute__((ext_vector_type(4)));
-        T4 o;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = (T)(l_run == 0.0f ? 0.0f : o_acc[r][4 * i4 + e] * inv);
-        *(T4 *)(out + 32 * r + 8 * i4 + 4 * hl) = o;
-      }
-  }
-  work.next(p.sched, p.cu_new, p.kv_len);
-  }
-  }
-  if (p.cuts && w < p.sched.target && kvh == 0 && threadIdx.x == 0) p.cuts[w] = cut;
-}
-
-// Merge of the parts of cut tiles: row m of a tile is sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m).  One
-// share begins a cut tile at most, its last one.  D / 4 threads share a row's channels.  Decode tiles (PG > 1)
-// have few rows and up to hundreds of parts: a workgroup takes one row, its thread groups every PG-th part,
-// and the groups are added in LDS; chunk tiles (PG 1) have many rows of two or three parts.
-template <int D, typename T, bool DECODE>
-__global__ __launch_bounds__(256) void paged_combine_kernel(const PagedParams p) {
-  constexpr int TPR = D / 4, PG = DECODE ? 256 / TPR : 1, RPB = DECODE ? 1 : 256 / TPR;
-  constexpr int R = DECODE ? kDecodeRows : kChunkRows;
-  constexpr int chunks = R / RPB;
-  static_assert(R % RPB == 0, "whole workgroups per tile");
-  const int w = blockIdx.x / (chunks * p.heads_kv), kvh = blockIdx.x / chunks % p.heads_kv;
-  const PagedCut cut = p.cuts[w];
-  const int lr = blockIdx.x % chunks * RPB + (DECODE ? 0 : threadIdx.x / TPR), ch = threadIdx.x % TPR * 4;
-  if (cut.parts == 0 || lr >= cut.rows) return;  // DECODE: the whole workgroup
-  const int G = p.sched.group, n = cut.parts, row = cut.row0 + lr;
-  // parts: slot 2 w + 1, then 2 (w + 1), 2 (w + 2), ..
-  const int64_t step = (int64_t)p.heads_kv * R, row_at = (int64_t)kvh * R + lr;
-  auto part = [&](int i) { return (int64_t)(2 * (w + i) + (i == 0)) * step + row_at; };
-  float m = kNegInf, l = 0.0f, m_ref;
-  if constexpr (DECODE) {  // a lane per part, every wave for itself
-    const int lane = threadIdx.x & 63;
-    for (int i = lane; i < n; i += 64) m = fmaxf(m, p.ws_ml[part(i) * 2]);
-    m = wave_allreduce_max(m);
-    m_ref = m == kNegInf ? 0.0f : m;
-    for (int i = lane; i < n; i += 64) l += p.ws_ml[part(i) * 2 + 1] * __builtin_amdgcn_exp2f(p.ws_ml[part(i) * 2] - m_ref);
-    l = wave_allreduce_sum(l);
-  } else {
-    for (int i = 0; i < n; ++i) m = fmaxf(m, p.ws_ml[part(i) * 2]);
-    m_ref = m == kNegInf ? 0.0f : m;
-    for (int i = 0; i < n; ++i) l += p.ws_ml[part(i) * 2 + 1] * __builtin_amdgcn_exp2f(p.ws_ml[part(i) * 2] - m_ref);
-  }
-  float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-  for (int i = DECODE ? threadIdx.x / TPR : 0; i < n; i += PG) {
-    const int64_t at = part(i);
-    const float f = __builtin_amdgcn_exp2f(p.ws_ml[at * 2] - m_ref);
-    const float4_t x = *(const float4_t *)(p.ws_o + at * D + ch);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] += x[e] * f;
-  }
-  if constexpr (DECODE) {
-    __shared__ float4_t sum[256];
-    sum[threadIdx.x] = o;
-    __syncthreads();
-    if (threadIdx.x >= TPR) return;
-#pragma unroll
-    for (int g = 1; g < PG; ++g) o += sum[g * TPR + threadIdx.x];
-  }
-  T *out = (T *)p.out + (int64_t)(cut.q_begin + row / G) * p.out_stride + (int64_t)(kvh * G + row % G) * D + ch;
-  typedef T T4 __attribute__((ext_vector_type(4)));
-  T4 y;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) y[e] = (T)(l == 0.0f ? 0.0f : o[e] / l);
-  *(T4 *)out = y;
-}
-
-template <int D, typename T>
-int launch_chunk(argus_hip_ctx *ctx, const PagedParams &p, int items, hipStream_t stream) {
-  auto kern = p.softcap > 0.0f ? paged_chunk_kernel<D, T, true> : paged_chunk_kernel<D, T, false>;
-  constexpr int lds = ChunkTile<D, std::is_same<T, float>::value>::LDS_BYTES;
-  ARGUS_HIP_CHECK(ctx, argus_raise_lds_limit(ctx, kern, lds));
-  hipLaunchKernelGGL(kern, dim3((unsigned)(items * p.heads_kv)), dim3(256), lds, stream, p);
-  ARGUS_HIP_CHECK(ctx, hipGetLastError());
-  return ARGUS_HIP_OK;
-}
 
 // How a call is cut: which kernels run, with how many workgroups, and where their partial results lie.
 struct CallPlan {
@@ -598,10 +43,11 @@ int make_plan(argus_hip_ctx *ctx, int compute_units, const argus_hip_paged_atten
     c.unit = 4 * c.align;
     c.min_share = 2;
     c.cut_cost = 2;  // 10 us; a unit of 128 keys is 5 us at d 128 with the device full
-    // resident workgroups, and no more shares than the longest lengths make
+    // Resident workgroups (beside the chunk form half of them, so that chunk shares begin at once: 60 single
+    // tokens and a chunk of 64 at d 128 124 -> 115 us), and no more shares than the longest lengths make.
     const int64_t tiles = sched_tiles_bound(c, a->min_new);
     const int64_t most = tiles * std::max<int64_t>(1, (longest + 2 * c.align) / c.unit + 1);
-    c.target = (int)std::min<int64_t>(std::max(1, compute_units * 2 / a->heads_kv), std::max<int64_t>(1, most / c.min_share));
+    c.target = (int)std::min<int64_t>(std::max(1, compute_units * (pl.chunk ? 1 : 2) / a->heads_kv), std::max<int64_t>(1, most / c.min_share));
     if (c.target == 1) c.cut_cost = -1;
     pl.d_items = sched_items_bound(c, tiles);
     pl.d_slots = c.cut_cost >= 0 ? sched_slots_bound(c) : 0;
@@ -627,7 +73,7 @@ int make_plan(argus_hip_ctx *ctx, int compute_units, const argus_hip_paged_atten
     pl.c_slots = c.cut_cost >= 0 && pl.chunk ? sched_slots_bound(c) : 0;
   }
   constexpr int64_t kGrid = 0x7fffffff;
-  if (pl.c_items * a->heads_kv > kGrid)
+  if ((pl.d_items + pl.c_items) * a->heads_kv > kGrid)
     return argus_fail(ctx, ARGUS_HIP_ERR_UNSUPPORTED, "paged_attention: %d rows are too many for one call", a->n_tokens);
   pl.ws_floats = (pl.d_slots * kDecodeRows + pl.c_slots * kChunkRows) * a->heads_kv * (d + 2) +
                  ((pl.d_slots ? pl.ds.target : 0) + (pl.c_slots ? pl.cs.target : 0)) * (int64_t)(sizeof(PagedCut) / sizeof(float));
@@ -660,32 +106,6 @@ int check(argus_hip_ctx *ctx, const argus_hip_paged_attention_args *a) {
 }
 
 }  // namespace
-
-int launch_paged_chunk(argus_hip_ctx *ctx, const PagedParams &p, int D, bool f32, int items, hipStream_t stream) {
-  switch (D) {
-    case 64: return f32 ? launch_chunk<64, float>(ctx, p, items, stream) : launch_chunk<64, _Float16>(ctx, p, items, stream);
-    case 128: return f32 ? launch_chunk<128, float>(ctx, p, items, stream) : launch_chunk<128, _Float16>(ctx, p, items, stream);
-    default: return f32 ? launch_chunk<256, float>(ctx, p, items, stream) : launch_chunk<256, _Float16>(ctx, p, items, stream);
-  }
-}
-
-template <int D, typename T>
-static int launch_combine(argus_hip_ctx *ctx, const PagedParams &p, hipStream_t stream) {
-  const bool decode = p.sched.tile_rows == kDecodeRows;
-  const int chunks = decode ? kDecodeRows : kChunkRows / (256 / (D / 4)), cuts = p.sched.target - 1;
-  auto kern = decode ? paged_combine_kernel<D, T, true> : paged_combine_kernel<D, T, false>;
-  hipLaunchKernelGGL(kern, dim3((unsigned)(cuts * p.heads_kv * chunks)), dim3(256), 0, stream, p);
-  ARGUS_HIP_CHECK(ctx, hipGetLastError());
-  return ARGUS_HIP_OK;
-}
-
-int launch_paged_combine(argus_hip_ctx *ctx, const PagedParams &p, int D, bool f32, hipStream_t stream) {
-  switch (D) {
-    case 64: return f32 ? launch_combine<64, float>(ctx, p, stream) : launch_combine<64, _Float16>(ctx, p, stream);
-    case 128: return f32 ? launch_combine<128, float>(ctx, p, stream) : launch_combine<128, _Float16>(ctx, p, stream);
-    default: return f32 ? launch_combine<256, float>(ctx, p, stream) : launch_combine<256, _Float16>(ctx, p, stream);
-  }
-}
 
 }  // namespace argus_paged
 
@@ -739,26 +159,24 @@ ARGUS_API int argus_hip_paged_attention(argus_hip_ctx *ctx, const argus_hip_page
   p.pool = argus_pool_strides(a->layout, a->heads_kv, a->page_size, d);
   p.heads_kv = a->heads_kv, p.n_pages = a->n_pages, p.page_shift = argus_log2(a->page_size), p.table_stride = a->table_stride;
   p.softcap = a->softcap, p.scale = a->scale != 0.0f ? a->scale : 1.0f / std::sqrt((float)d);
-  KernelTimer timer(ctx, stream);
-  if (pl.decode) {
-    p.sched = pl.ds;
-    p.ws_o = ws;  // output rows first: they are read and written 16 bytes at a time
-    p.cuts = pl.d_slots ? (PagedCut *)(ws + pl.d_slots * kDecodeRows * a->heads_kv * d) : nullptr;
-    p.ws_ml = (float *)(p.cuts + (pl.d_slots ? pl.ds.target : 0));
-    rc = launch_paged_decode(ctx, p, d, f32, (int)pl.d_items, stream);
-    if (rc == ARGUS_HIP_OK && !pl.chunk) timer.mark();
-    if (rc == ARGUS_HIP_OK && pl.d_slots) rc = launch_paged_combine(ctx, p, d, f32, stream);
-    if (rc != ARGUS_HIP_OK) return rc;
-    if (pl.d_slots) ws = p.ws_ml + pl.d_slots * kDecodeRows * a->heads_kv * 2;
+  // a form's part of the workspace: output rows (read and written 16 bytes at a time), cuts, maxima and sums
+  auto form = [&](const PagedSched &sched, int64_t items, int64_t slots) {
+    PagedParams f = p;
+    f.sched = sched;
+    f.items = (int)items;
+    if (slots) {
+      f.ws_o = ws;
+      f.cuts = (PagedCut *)(ws + slots * sched.tile_rows * a->heads_kv * d);
+      f.ws_ml = (float *)(f.cuts + sched.target);
+      ws = f.ws_ml + slots * sched.tile_rows * a->heads_kv * 2;
+    }
+    return f;
+  };
+  const PagedParams dp = form(pl.ds, pl.decode ? pl.d_items : 0, pl.d_slots), cp = form(pl.cs, pl.chunk ? pl.c_items : 0, pl.c_slots);
+  const bool cap = a->softcap > 0.0f;
+  switch (d) {
+    case 64: return launch_paged_64(ctx, dp, cp, f32, cap, stream);
+    case 128: return launch_paged_128(ctx, dp, cp, f32, cap, stream);
+    default: return launch_paged_256(ctx, dp, cp, f32, cap, stream);
   }
-  if (pl.chunk) {
-    p.sched = pl.cs;
-    p.ws_o = ws;
-    p.cuts = pl.c_slots ? (PagedCut *)(ws + pl.c_slots * kChunkRows * a->heads_kv * d) : nullptr;
-    p.ws_ml = (float *)(p.cuts + (pl.c_slots ? pl.cs.target : 0));
-    rc = launch_paged_chunk(ctx, p, d, f32, (int)pl.c_items, stream);
-    timer.mark();
-    if (rc == ARGUS_HIP_OK && pl.c_slots) rc = launch_paged_combine(ctx, p, d, f32, stream);
-  }
-  return rc;
 }

@@ -48,6 +48,7 @@ struct PagedParams {
   int64_t q_stride, out_stride;
   PoolStrides pool;  // elements
   PagedSched sched;
+  int32_t items;  // workgroups per KV head
   int32_t heads_kv, n_pages, page_shift, table_stride;
   float scale, softcap;
 };
@@ -56,9 +57,10 @@ struct PagedParams {
 constexpr int kDecodeRows = 16;  // requests of at most this many rows (tokens x heads of a group) take the decode kernel
 constexpr int kChunkRows = 128;  // rows per workgroup of the chunk kernel
 
-int launch_paged_decode(argus_hip_ctx *ctx, const PagedParams &p, int D, bool f32, int items, hipStream_t stream);
-int launch_paged_chunk(argus_hip_ctx *ctx, const PagedParams &p, int D, bool f32, int items, hipStream_t stream);
-int launch_paged_combine(argus_hip_ctx *ctx, const PagedParams &p, int D, bool f32, hipStream_t stream);
+// dp, cp: parameters of the decode and the chunk form (items 0: not in this call)
+int launch_paged_64(argus_hip_ctx *ctx, const PagedParams &dp, const PagedParams &cp, bool f32, bool cap, hipStream_t stream);
+int launch_paged_128(argus_hip_ctx *ctx, const PagedParams &dp, const PagedParams &cp, bool f32, bool cap, hipStream_t stream);
+int launch_paged_256(argus_hip_ctx *ctx, const PagedParams &dp, const PagedParams &cp, bool f32, bool cap, hipStream_t stream);
 constexpr int decode_align(int D) { return D <= 128 ? 32 : 16; }   // keys per wave step of the decode kernel
 constexpr int chunk_align(int D) { return D <= 64 ? 64 : 32; }     // keys per tile of the chunk kernel
 
@@ -121,9 +123,10 @@ struct PageWindow {
 
 // The kernel's arguments read again from where they came: what is needed only after a long loop does not
 // stay in scalar registers through it.
+template <int ARG>  // the kernel's arguments are PagedParams only: which of them
 __device__ __forceinline__ const PagedParams &params_again() {
   typedef const __attribute__((address_space(4))) PagedParams *const_ptr;
-  const_ptr a = (const_ptr)__builtin_amdgcn_kernarg_segment_ptr();
+  const_ptr a = (const_ptr)__builtin_amdgcn_kernarg_segment_ptr() + ARG;
   asm volatile("" : "+s"(a));
   return *(const PagedParams *)a;
 }

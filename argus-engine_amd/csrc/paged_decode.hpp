@@ -11,6 +11,8 @@
 // scale is applied to the F32 logit) and probabilities are rounded to F16, as the output will be; F32
 // queries and the probabilities of their rows are held as F16 pairs, hi + lo, in two MFMAs each, which
 // leaves F32's error.  Bound by HBM: every key is read once per KV head for all rows.
+#pragma once
+
 #include "paged_common.hpp"
 
 #include <algorithm>
@@ -28,7 +30,7 @@ struct DecodeShape {
   static constexpr int NACC = VC * VSEG;
   static constexpr int TW = D <= 128 ? 2 : 1;    // blocks of 16 keys per wave step
 };
-constexpr int kWaves = 4;
+constexpr int kWaves = 4;  // of a workgroup, each taking every fourth step of the keys
 
 template <typename T>
 __device__ __forceinline__ T load_stream(__amdgpu_buffer_rsrc_t rsrc, uint32_t voff, uint32_t soff);
@@ -41,8 +43,12 @@ __device__ __forceinline__ half4_t load_stream<half4_t>(__amdgpu_buffer_rsrc_t r
   return __builtin_bit_cast(half4_t, __builtin_amdgcn_raw_buffer_load_b64(rsrc, voff, soff, 2));
 }
 
-template <int D, typename T, bool CAP>
-__global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(const PagedParams p) {
+template <int D>
+constexpr int kDecodeLds = kWaves * 16 * (D + 4) * (int)sizeof(float);  // merge of the waves
+
+// Share `w` of KV head `kvh`; ARG: which of the kernel's PagedParams arguments `p` is.
+template <int D, typename T, bool CAP, int ARG>
+__device__ __forceinline__ void decode_share(const PagedParams &p, PagedShare work, int w, int kvh, float *lds_acc) {  // lds_acc: [kWaves][16][D + 4]
   using SH = DecodeShape<D>;
   constexpr int KK = SH::KK, VC = SH::VC, VSEG = SH::VSEG, NACC = SH::NACC, TW = SH::TW;
   constexpr int STEP = 16 * TW;
@@ -51,7 +57,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(const Page
   typedef typename std::conditional<VC == 8, half8_t, half4_t>::type vpiece_t;
   constexpr float kLog2e = 1.4426950408889634f;
 
-  const int kvh = blockIdx.x % p.heads_kv, w = blockIdx.x / p.heads_kv;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int j = lane >> 4, r = lane & 15;
   const int G = p.sched.group;
@@ -63,10 +68,8 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(const Page
   const float c = p.scale * kLog2e;
   const float inv_cap = CAP ? 1.0f / p.softcap : 0.0f;
   __shared__ float lds_m[kWaves][16], lds_l[kWaves][16];
-  extern __shared__ __attribute__((aligned(16))) float lds_acc[];  // [kWaves][16][D + 4]
 
   PagedCut cut{0, 0, 0, 0};
-  PagedShare work(p.sched, p.cu_new, p.kv_len, w);
   while (work.found) {  // the requests this share touches
   const PagedPlace it = work.at;
   const int rows = (it.s.q_end - it.s.q_begin) * G;  // at most 16: one tile
@@ -297,7 +300,7 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(const Page
   }
 
   // ---- merge: lane groups (row sum), then the waves through LDS -----------------------------------
-  const PagedParams &p = params_again();
+  const PagedParams &p = params_again<ARG>();
   l_run += __shfl_xor(l_run, 16, 64);
   l_run += __shfl_xor(l_run, 32, 64);
   if (j == 0) {
@@ -343,24 +346,6 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_decode_kernel(const Page
   if (p.cuts && kvh == 0 && threadIdx.x == 0) p.cuts[w] = cut;
 }
 
-template <int D, typename T>
-int launch(argus_hip_ctx *ctx, const PagedParams &p, int items, hipStream_t stream) {
-  constexpr size_t lds = (size_t)kWaves * 16 * (D + 4) * sizeof(float);
-  auto kern = p.softcap > 0.0f ? paged_decode_kernel<D, T, true> : paged_decode_kernel<D, T, false>;
-  ARGUS_HIP_CHECK(ctx, argus_raise_lds_limit(ctx, kern, (int)lds));
-  hipLaunchKernelGGL(kern, dim3((unsigned)(items * p.heads_kv)), dim3(64 * kWaves), lds, stream, p);
-  ARGUS_HIP_CHECK(ctx, hipGetLastError());
-  return ARGUS_HIP_OK;
-}
-
 }  // namespace
-
-int launch_paged_decode(argus_hip_ctx *ctx, const PagedParams &p, int D, bool f32, int items, hipStream_t stream) {
-  switch (D) {
-    case 64: return f32 ? launch<64, float>(ctx, p, items, stream) : launch<64, _Float16>(ctx, p, items, stream);
-    case 128: return f32 ? launch<128, float>(ctx, p, items, stream) : launch<128, _Float16>(ctx, p, items, stream);
-    default: return f32 ? launch<256, float>(ctx, p, items, stream) : launch<256, _Float16>(ctx, p, items, stream);
-  }
-}
 
 }  // namespace argus_paged
