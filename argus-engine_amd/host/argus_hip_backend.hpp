@@ -323,6 +323,153 @@ struct HipKvCache {
   }
 };
 
+// A paged F16 cache shared by many requests: page pools of every layer, the requests' page tables and
+// lengths, and the three calls of a step.  No counterpart in the reference, whose KV containers hold one
+// sequence; written in its manner (Status, Result, device tensors of the backend).
+//
+//   begin_step(new_len)            one argus_hip_page_plan: positions, write slots, page tables
+//   write(layer, q, k, v, ...)     argus_hip_qk_norm_rope into that layer's pools
+//   attend(layer, q, out, ...)     argus_hip_paged_attention over them
+//   end_step()                     the new tokens count as cached
+//   release(seq)                   the request's pages are free again
+// Page numbers are handed out by the device from the list the host uploads; the host repeats the rule (pages in
+// request order from the front of the list) to know who holds what, and reads nothing back.
+class HipPagedKvCache {
+ public:
+  struct Config {
+    size_t layers = 1, heads_q = 0, heads_kv = 0, head_dim = 0;
+    size_t page_size = 16, n_pages = 0, max_seqs = 0, max_pages_per_seq = 0, max_tokens = 0;  // max_tokens: new ones per step
+    bool head_major = true;
+  };
+  static Result<std::shared_ptr<HipPagedKvCache>> create(HipBackend &be, const Config &c) {
+    typedef Result<std::shared_ptr<HipPagedKvCache>> R;
+    if (!c.layers || !c.heads_q || !c.heads_kv || !c.n_pages || !c.max_seqs || !c.max_pages_per_seq || !c.max_tokens) return R::Err("paged cache: a size is zero");
+    std::shared_ptr<HipPagedKvCache> p(new HipPagedKvCache(be, c));
+    const size_t pool = c.n_pages * c.heads_kv * c.page_size * c.head_dim * 2;
+    auto get = [&](size_t bytes, void **out) {
+      auto r = be.alloc(bytes);
+      if (!r.ok()) return false;
+      *out = r.value();
+      p->owned_.push_back(*out);
+      return true;
+    };
+    p->pools_.resize(2 * c.layers);
+    bool ok = true;
+    for (void *&x : p->pools_) ok = ok && get(pool, &x);
+    const size_t i32 = sizeof(int32_t);
+    ok = ok && get(c.max_seqs * i32, (void **)&p->past_) && get(c.max_seqs * i32, (void **)&p->new_) && get(c.n_pages * i32, (void **)&p->free_) &&
+         get(c.max_seqs * c.max_pages_per_seq * i32, (void **)&p->table_) && get((c.max_seqs + 1) * i32, (void **)&p->cu_) &&
+         get(c.max_seqs * i32, (void **)&p->kv_) && get(c.max_tokens * i32, (void **)&p->pos_) && get(c.max_tokens * i32, (void **)&p->slots_) &&
+         get(3 * i32, (void **)&p->counts_);
+    if (!ok) return R::Err("paged cache: " + be.last_error());
+    return R::Ok(p);
+  }
+  ~HipPagedKvCache() {
+    for (void *x : owned_) (void)be_.free(x);
+  }
+  HipPagedKvCache(const HipPagedKvCache &) = delete;
+  HipPagedKvCache &operator=(const HipPagedKvCache &) = delete;
+
+  size_t cached(size_t seq) const { return (size_t)past_len_[seq]; }
+  size_t free_pages() const { return free_list_.size(); }
+  size_t new_tokens() const { return tokens_; }
+
+  // new_len[s] tokens of request s join this step (0: idle).  Refused, with nothing changed, when a request
+  // would outgrow its table, the pages run out, or the step holds more than max_tokens.
+  Status begin_step(const std::vector<int32_t> &new_len) {
+    if (tokens_) return Status::Err("paged cache: a step is open");
+    if (new_len.size() != c_.max_seqs) return Status::Err("paged cache: one length per request slot");
+    size_t tokens = 0, need = 0;
+    int32_t most = 0;
+    for (size_t s = 0; s < c_.max_seqs; ++s) {
+      if (new_len[s] < 0) return Status::Err("paged cache: negative length");
+      const size_t want = pages((size_t)past_len_[s] + (size_t)new_len[s]);
+      if (want > c_.max_pages_per_seq) return Status::Err("paged cache: request " + std::to_string(s) + " outgrows its page table");
+      need += want - pages((size_t)past_len_[s]);
+      tokens += (size_t)new_len[s];
+      most = std::max(most, new_len[s]);
+    }
+    if (need > free_list_.size()) return Status::Err("paged cache: " + std::to_string(need) + " pages needed, " + std::to_string(free_list_.size()) + " free");
+    if (tokens > c_.max_tokens) return Status::Err("paged cache: too many new tokens");
+    if (!tokens) return OkStatus();
+    const size_t i32 = sizeof(int32_t);
+    Status st = be_.write_buffer(past_, past_len_.data(), c_.max_seqs * i32);
+    if (st.ok()) st = be_.write_buffer(new_, new_len.data(), c_.max_seqs * i32);
+    if (st.ok() && need) st = be_.write_buffer(free_, free_list_.data(), need * i32);
+    if (!st.ok()) return st;
+    argus_hip_page_plan_args a{};
+    a.past_len = past_, a.new_len = new_, a.free_pages = free_, a.page_table = table_, a.cu_new = cu_, a.kv_len = kv_;
+    a.positions = pos_, a.slots = slots_, a.counts = counts_;
+    a.n_seqs = (int32_t)c_.max_seqs, a.n_free = (int32_t)need, a.n_pages = (int32_t)c_.n_pages, a.page_size = (int32_t)c_.page_size;
+    a.table_stride = (int32_t)c_.max_pages_per_seq, a.token_capacity = (int32_t)c_.max_tokens;
+    st = be_.wrap(argus_hip_page_plan(be_.ctx(), &a));
+    if (!st.ok()) return st;
+    size_t taken = 0;
+    for (size_t s = 0; s < c_.max_seqs; ++s)
+      while (held_[s].size() < pages((size_t)past_len_[s] + (size_t)new_len[s])) held_[s].push_back(free_list_[taken++]);
+    free_list_.erase(free_list_.begin(), free_list_.begin() + (long)taken);
+    new_len_ = new_len;
+    tokens_ = tokens;
+    max_new_ = most;
+    return OkStatus();
+  }
+  // q [tokens, heads_q, head_dim], k / v [tokens, heads_kv, head_dim] of one dtype, packed; q_out like q, F32 or
+  // F16; cos_sin F32 [n_positions, rot_dim] (rot_dim 0: none); norm weights F32 [head_dim] or null.
+  Status write(size_t layer, const Tensor &q, const Tensor &k, const Tensor &v, Tensor &q_out, const float *q_weight, const float *k_weight, float eps,
+               const float *cos_sin, size_t n_positions, size_t rot_dim, bool interleaved = false, float weight_bias = 0.0f) {
+    if (layer >= c_.layers || !tokens_) return Status::Err("paged cache: no such layer, or no step is open");
+    if (k.dtype != q.dtype || v.dtype != q.dtype) return Status::Err("paged cache: q, k and v have one dtype");
+    argus_hip_qk_norm_rope_args a{};
+    a.q = q.ptr, a.k = k.ptr, a.v = v.ptr, a.q_weight = q_weight, a.k_weight = k_weight, a.cos_sin = cos_sin;
+    a.positions = pos_, a.slots = slots_, a.q_out = q_out.ptr, a.k_cache = pools_[2 * layer], a.v_cache = pools_[2 * layer + 1];
+    a.tokens = (int32_t)tokens_, a.heads_q = (int32_t)c_.heads_q, a.heads_kv = (int32_t)c_.heads_kv, a.head_dim = (int32_t)c_.head_dim;
+    a.rot_dim = (int32_t)rot_dim, a.interleaved = interleaved ? 1 : 0, a.n_positions = (int32_t)n_positions;
+    a.n_pages = (int32_t)c_.n_pages, a.page_size = (int32_t)c_.page_size, a.layout = layout();
+    a.in_dtype = (int32_t)q.dtype, a.out_dtype = (int32_t)q_out.dtype, a.eps = eps, a.weight_bias = weight_bias;
+    return be_.wrap(argus_hip_qk_norm_rope(be_.ctx(), &a));
+  }
+  Status attend(size_t layer, const Tensor &q, Tensor &out, size_t window = 0, float softcap = 0.0f, float scale = 0.0f) {
+    if (layer >= c_.layers || !tokens_) return Status::Err("paged cache: no such layer, or no step is open");
+    if (q.dtype != out.dtype) return Status::Err("paged cache: q and out have one dtype");
+    argus_hip_paged_attention_args a{};
+    a.q = q.ptr, a.k_cache = pools_[2 * layer], a.v_cache = pools_[2 * layer + 1], a.page_table = table_, a.cu_new = cu_, a.kv_len = kv_, a.out = out.ptr;
+    a.n_seqs = (int32_t)c_.max_seqs, a.n_tokens = (int32_t)tokens_, a.heads_q = (int32_t)c_.heads_q, a.heads_kv = (int32_t)c_.heads_kv;
+    a.head_dim = (int32_t)c_.head_dim, a.n_pages = (int32_t)c_.n_pages, a.page_size = (int32_t)c_.page_size;
+    a.table_stride = (int32_t)c_.max_pages_per_seq, a.layout = layout(), a.dtype = (int32_t)q.dtype, a.max_new = max_new_;
+    a.window = (int32_t)window, a.softcap = softcap, a.scale = scale;
+    return be_.wrap(argus_hip_paged_attention(be_.ctx(), &a));
+  }
+  Status end_step() {
+    for (size_t s = 0; s < c_.max_seqs && tokens_; ++s) past_len_[s] += new_len_[s];
+    tokens_ = 0;
+    return OkStatus();
+  }
+  Status release(size_t seq) {
+    if (tokens_) return Status::Err("paged cache: a step is open");
+    if (seq >= c_.max_seqs) return Status::Err("paged cache: no such request");
+    free_list_.insert(free_list_.end(), held_[seq].begin(), held_[seq].end());
+    held_[seq].clear();
+    past_len_[seq] = 0;
+    return OkStatus();
+  }
+
+ private:
+  HipPagedKvCache(HipBackend &be, const Config &c) : be_(be), c_(c), past_len_(c.max_seqs, 0), new_len_(c.max_seqs, 0), held_(c.max_seqs) {
+    for (size_t p = 0; p < c.n_pages; ++p) free_list_.push_back((int32_t)p);
+  }
+  size_t pages(size_t tokens) const { return (tokens + c_.page_size - 1) / c_.page_size; }
+  int32_t layout() const { return c_.head_major ? ARGUS_HIP_HEAD_MAJOR : ARGUS_HIP_SEQ_MAJOR; }
+  HipBackend &be_;
+  Config c_;
+  std::vector<void *> owned_, pools_;  // pools_: K and V of every layer
+  int32_t *past_ = nullptr, *new_ = nullptr, *free_ = nullptr, *table_ = nullptr, *cu_ = nullptr, *kv_ = nullptr, *pos_ = nullptr, *slots_ = nullptr,
+          *counts_ = nullptr;
+  std::vector<int32_t> past_len_, new_len_, free_list_;
+  std::vector<std::vector<int32_t>> held_;
+  size_t tokens_ = 0;  // of the open step
+  int32_t max_new_ = 0;
+};
+
 class HipScoreReduceBackend {
  public:
   explicit HipScoreReduceBackend(argus_hip_ctx *ctx) : ctx_(ctx) {}
