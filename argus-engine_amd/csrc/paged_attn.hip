@@ -49,7 +49,8 @@ int make_plan(argus_hip_ctx *ctx, int compute_units, const argus_hip_paged_atten
     const int64_t most = tiles * std::max<int64_t>(1, (longest + 2 * c.align) / c.unit + 1);
     c.target = (int)std::min<int64_t>(std::max(1, compute_units * (pl.chunk ? 1 : 2) / a->heads_kv), std::max<int64_t>(1, most / c.min_share));
     if (c.target == 1) c.cut_cost = -1;
-    pl.d_items = sched_items_bound(c, tiles);
+    pl.d_items = c.cut_cost < 0 ? tiles : c.target;  // more requests than shares: a share takes several
+    c.rooms = (int)pl.d_items;
     pl.d_slots = c.cut_cost >= 0 ? sched_slots_bound(c) : 0;
   }
   if (pl.chunk) {
@@ -69,7 +70,9 @@ int make_plan(argus_hip_ctx *ctx, int compute_units, const argus_hip_paged_atten
     c.cut_cost = d == 64 ? 1300 : d == 128 ? 1100 : 700;
     if (longest + 96 <= c.min_share) c.cut_cost = -1;    // tiles too short to be cut
     if (tiles == 0) pl.chunk = false;                    // too few rows for any request of this class
-    pl.c_items = sched_items_bound(c, tiles);
+    pl.c_items = c.cut_cost < 0 ? tiles : std::max<int64_t>(tiles, c.target);
+    if (!pl.chunk) pl.c_items = 0;
+    c.rooms = (int)std::min<int64_t>(pl.c_items, 0x7fffffff);
     pl.c_slots = c.cut_cost >= 0 && pl.chunk ? sched_slots_bound(c) : 0;
   }
   constexpr int64_t kGrid = 0x7fffffff;
@@ -96,7 +99,7 @@ int check(argus_hip_ctx *ctx, const argus_hip_paged_attention_args *a) {
     return argus_fail(ctx, ARGUS_HIP_ERR_INVALID, "paged_attention: layout %d", a->layout);
   if (a->dtype != ARGUS_HIP_F32 && a->dtype != ARGUS_HIP_F16)
     return argus_fail(ctx, ARGUS_HIP_ERR_UNSUPPORTED, "paged_attention: dtype %d", a->dtype);
-  if (a->window < 0 || a->min_new < 0 || a->max_new < 0 || a->max_kv < 0 || !(a->softcap >= 0.0f) || !(a->softcap < __builtin_huge_valf()) ||
+  if (a->window < 0 || a->min_new < 0 || a->max_new < 0 || a->max_kv < 0 || !(a->softcap == 0.0f || a->softcap >= 1.17549435e-38f) || !(a->softcap < __builtin_huge_valf()) ||
       !(a->scale > -__builtin_huge_valf() && a->scale < __builtin_huge_valf()))
     return argus_fail(ctx, ARGUS_HIP_ERR_INVALID, "paged_attention: window %d min_new %d max_new %d max_kv %d softcap %g scale %g", a->window,
                       a->min_new, a->max_new, a->max_kv, a->softcap, a->scale);

@@ -72,9 +72,10 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
   const uint32_t lane_off = my_row * row_bytes + 16 * my_col;
   const PagePool k_pool(p.k, p, kvh, D), v_pool(p.v, p, kvh, D);
   // exponents are logit * ce - m_ref (CAP: of the capped logit); a negative scale turns the queries round instead
-  const float ce = CAP ? kLog2e : __builtin_fabsf(p.scale) * kLog2e;
+  float ce = CAP ? kLog2e : __builtin_fabsf(p.scale) * kLog2e;
   const float q_sign = p.scale < 0.0f ? -1.0f : 1.0f;
-  const float cap = p.softcap, cap_in = CAP ? __builtin_fabsf(p.scale) / p.softcap : 0.0f;  // cap * tanh(product * cap_in)
+  const float cap = p.softcap;
+  float cap_in = CAP ? __builtin_fabsf(p.scale) / p.softcap : 0.0f;  // cap * tanh(product * cap_in)
   // V^T operand: ds_read_b64_tr_b16 gives lane i of 16 channel ch0 + i of keys key0 .. key0 + 3 when lane s
   // addresses V[key0 + s / 4][ch0 + 4 (s % 4)]; P^T holds keys 4 hl + {0..3} and 8 + 4 hl + {0..3} of 16
   const int g16 = lane >> 4, s16 = lane & 15;
@@ -164,6 +165,20 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
   half8_t qh[KK], ql[F32 ? KK : 1];
   auto load_q = [&]() __attribute__((always_inline)) {
     const T *qp = (const T *)p.q + (int64_t)(it.s.q_begin + tok) * p.q_stride + (int64_t)head * D + 8 * hl;
+    int shift = 0;
+    if constexpr (F32) {
+      float largest = 0.0f;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        const float4_t a = *(const float4_t *)(qp + 16 * kk), b = *(const float4_t *)(qp + 16 * kk + 4);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) largest = fmaxf(largest, __builtin_fabsf(e < 4 ? a[e] : b[e - 4]));
+      }
+      shift = row_shift(xor32_combine(largest, [](float a, float b) { return fmaxf(a, b); }));
+      if constexpr (CAP) cap_in = __builtin_ldexpf(__builtin_fabsf(p.scale) / cap, -shift);
+      else ce = __builtin_ldexpf(__builtin_fabsf(p.scale) * kLog2e, -shift);
+      asm volatile("" : "+v"(qp));  // read again rather than held
+    }
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
       if constexpr (F32) {
@@ -171,7 +186,7 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           _Float16 hi, lo;
-          split_f16((e < 4 ? a[e] : b[e - 4]) * q_sign, hi, lo);
+          split_f16(__builtin_ldexpf((e < 4 ? a[e] : b[e - 4]) * q_sign, shift), hi, lo);
           qh[kk][e] = hi;
           ql[kk][e] = lo;
         }

@@ -148,6 +148,13 @@ __device__ __forceinline__ float soft_cap(float s, float cap, float inv_cap) {
   return cap * t;
 }
 
+// F32 queries enter the products as F16 pairs, hi + lo.  A row is brought to 2^14 .. 2^15 by a power of two
+// first, which the factor of its logits takes back: so the pair holds 22 bits of it whatever its size is.
+__device__ __forceinline__ int row_shift(float largest) {
+  const int shift = 15 - __builtin_amdgcn_frexp_expf(largest);
+  return shift < 100 ? shift : 100;  // the factor stays a normal number
+}
+
 __device__ __forceinline__ bool not_finite(_Float16 x) { return (__builtin_bit_cast(uint16_t, x) & 0x7c00) == 0x7c00; }
 #endif
 

@@ -7,8 +7,8 @@
 //   O[row][channel] = P . V   A = the lane's own probabilities (keys 4j .. 4j + 3 of each 16), B = V rows
 //                             transposed 4 x 8 in registers
 //
-// Nothing goes through LDS in the key loop.  F16 queries are held as they are (the products are exact, the
-// scale is applied to the F32 logit) and probabilities are rounded to F16, as the output will be; F32
+// Nothing goes through LDS in the key loop.  The scale is applied to the F32 logit, so F16 queries enter as
+// they are and their products are exact; probabilities are rounded to F16, as the output will be.  F32
 // queries and the probabilities of their rows are held as F16 pairs, hi + lo, in two MFMAs each, which
 // leaves F32's error.  Bound by HBM: every key is read once per KV head for all rows.
 #pragma once
@@ -65,7 +65,6 @@ __device__ __forceinline__ void decode_share(const PagedParams &p, PagedShare wo
   const uint32_t row_bytes = (uint32_t)p.pool.row * 2;
   const uint32_t k_lane = r * row_bytes + 16 * j, v_lane = 4 * j * row_bytes + 2 * VC * r;
   const PagePool k_pool(p.k, p, kvh, D), v_pool(p.v, p, kvh, D);
-  const float c = p.scale * kLog2e;
   const float inv_cap = CAP ? 1.0f / p.softcap : 0.0f;
   __shared__ float lds_m[kWaves][16], lds_l[kWaves][16];
 
@@ -133,13 +132,23 @@ __device__ __forceinline__ void decode_share(const PagedParams &p, PagedShare wo
   load_k(base0);
   load_v();
   __builtin_amdgcn_sched_barrier(0);
+  int shift = 0;
+  if constexpr (F32) {
+    float largest = 0.0f;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) largest = fmaxf(largest, __builtin_fabsf(qx[kk][e]));
+    shift = row_shift(rows_allreduce_max(largest));
+  }
+  const float c = __builtin_ldexpf(CAP ? p.scale : p.scale * kLog2e, -shift);  // of row r: products to logits (CAP) or exponents
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) {
     if constexpr (F32) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         _Float16 hi, lo;
-        split_f16(CAP ? qx[kk][e] * p.scale : qx[kk][e] * c, hi, lo);
+        split_f16(__builtin_ldexpf(qx[kk][e], shift), hi, lo);
         qh[kk][e] = hi;
         ql[kk][e] = lo;
       }
@@ -177,8 +186,8 @@ __device__ __forceinline__ void decode_share(const PagedParams &p, PagedShare wo
     for (int tw = 0; tw < TW; ++tw)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        if constexpr (CAP) s[tw][i] = soft_cap<F32>(F32 ? s[tw][i] : s[tw][i] * p.scale, p.softcap, inv_cap) * kLog2e;
-        else if constexpr (!F32) s[tw][i] *= c;
+        if constexpr (CAP) s[tw][i] = soft_cap<F32>(s[tw][i] * c, p.softcap, inv_cap) * kLog2e;
+        else s[tw][i] *= c;
       }
     if (edge) {
       const int hi = min(pos, end - 1), lo = window != 0x7fffffff ? pos - window : -1;

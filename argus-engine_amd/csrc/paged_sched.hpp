@@ -28,6 +28,7 @@ struct PagedSched {
   int32_t min_share;             // a share is not smaller than this
   int32_t target;                // shares per KV head
   int32_t alone;                 // up to this many shares per KV head run without another on their compute unit: ~0.6 of the time
+  int32_t rooms;                 // workgroups per KV head there are: no more tiles than that are taken whole
   int32_t cut_cost;              // what cutting costs a call: further starts, partial results, the merge; < 0: no tile is cut
   int32_t window, max_len;       // max_len: keys the page table has room for
 };
@@ -96,6 +97,7 @@ ARGUS_HD int64_t sched_share(const PagedSched &c, int64_t work) {
 // Are the tiles taken whole?  tiles, work, longest: over the class.
 ARGUS_HD bool sched_whole(const PagedSched &c, int64_t tiles, int64_t work, int64_t longest) {
   if (c.cut_cost < 0 || tiles == 0) return true;
+  if (tiles > c.rooms) return false;
   const double rounds = (double)((tiles + c.target - 1) / c.target) * ((double)work / (double)tiles);
   double whole = rounds > (double)longest ? rounds : (double)longest;
   if (tiles <= c.alone) whole *= 0.6;
@@ -112,7 +114,6 @@ inline int64_t sched_tiles_bound(const PagedSched &c, int min_new) {
   if (c.rows_upto <= c.tile_rows) return seqs;
   return seqs ? rows / c.tile_rows + seqs : 0;
 }
-inline int64_t sched_items_bound(const PagedSched &c, int64_t tiles) { return c.cut_cost >= 0 && tiles < c.target ? c.target : tiles; }
 inline int64_t sched_slots_bound(const PagedSched &c) { return 2 * (int64_t)c.target; }
 
 #ifdef __HIPCC__
@@ -156,6 +157,7 @@ __device__ __forceinline__ int64_t lane_value(int64_t x, int l) {
 struct PagedPlace {
   PagedSeq s;
   int32_t seq, tile, left;  // left: further tiles of the request
+  int64_t block;            // where the requests' block of 64 begins
   int64_t start, cost;      // of the tile, on the line
   int64_t slope;            // cost of the request's next tile above this one's
 };
@@ -196,6 +198,7 @@ struct PagedBlock {
       else hi = mid;
     }
     place(b, l, cost, tile, before, out);
+    out.block = at;
     return true;
   }
   // tile number x of the line, the last tiles of a request first
@@ -208,6 +211,7 @@ struct PagedBlock {
     cost.base = lane_value(k.base, l);
     cost.slope = lane_value(k.slope, l);
     place(b, l, cost, (int)(at + lane_value(inc_tiles, l) - 1 - x), 0, out);
+    out.block = 0;  // not used: a share is one tile then
     return true;
   }
   __device__ __forceinline__ void place(int b, int l, const PagedCost &cost, int tile, int64_t before, PagedPlace &out) const {
@@ -243,6 +247,7 @@ struct PagedShare {
     work = lane_value(first.inc, 63);
     tiles = lane_value(first_tiles, 63);
     int longest = first.longest();
+#pragma unroll 4
     for (int b = 64; b < c.n_seqs; b += 64) {
       const PagedBlock block(c, cu, kv, b);
       work += lane_value(block.inc, 63);
@@ -280,7 +285,7 @@ struct PagedShare {
       at.start = x;
       at.cost += at.slope;
     } else {
-      search(c, cu, kv, 0, 0);
+      search(c, cu, kv, at.block, at.seq & ~63);
     }
   }
 };

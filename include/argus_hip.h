@@ -746,7 +746,8 @@ int argus_hip_qk_norm_rope(argus_hip_ctx *ctx, const argus_hip_qk_norm_rope_args
  * number outside the pool where its keys lie reads some page of the pool there instead, and keys past
  * table_stride pages do not exist: its rows are not specified, no other request's are touched.
  * dtype F16: logits and sums in F32, probabilities rounded to F16 for the second product; dtype F32: q and
- * the probabilities as F16 pairs (hi + lo), so the result is that of F32 arithmetic.
+ * the probabilities as F16 pairs (hi + lo), so the result is that of F32 arithmetic,
+ * whatever the size of the queries is.
  * max_new / max_kv: no request brings more new tokens / holds more tokens than this (0 = not known).
  * They choose kernels, and rows of a request that brings more than max_new may be left unwritten.
  * min_new: no request with any new token brings fewer (0 = not known).

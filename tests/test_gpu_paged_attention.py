@@ -47,11 +47,11 @@ def check(st, got, softcap=0.0, window=0, scale=None, only=None):
     assert (got[cu[-1]:] == -9.0).all(), "rows behind the last request were written"
 
 
-HEADS = {"llama": (8, 2, 128), "qwen": (14, 2, 64), "gemma": (4, 2, 256), "mha": (3, 3, 64), "wide": (24, 1, 128), "one": (1, 1, 256)}
+HEADS = {"llama": (8, 2, 128), "qwen": (14, 2, 64), "gemma": (4, 2, 256), "mha": (3, 3, 64), "wide": (24, 1, 128), "one": (1, 1, 256), "huge": (200, 1, 64)}
 
 
 @pytest.mark.parametrize("ty", ["f16", "f32"])
-@pytest.mark.parametrize("heads", ["llama", "qwen", "gemma", "mha", "wide", "one"])
+@pytest.mark.parametrize("heads", ["llama", "qwen", "gemma", "mha", "wide", "one", "huge"])
 @pytest.mark.parametrize("past,new", [
     ([0], [1]), ([1], [1]), ([15], [1]), ([16], [1]), ([700], [1]),
     ([300, 0, 33, 64, 999], [1, 1, 1, 1, 1]),              # single tokens
@@ -92,6 +92,29 @@ def test_many_requests():
     st = setup(5, [int(x) for x in past], [int(x) for x in new], 2, 1, 64, 16, "f16")
     check(st, call(st))
     check(st, call(st, hints=False))
+
+
+def test_thousands_of_requests_and_a_few_long_ones_among_them():
+    """More requests than workgroups, in blocks of 64 with long, empty and idle ones at their borders."""
+    rng = np.random.default_rng(1)
+    past, new = rng.integers(0, 20, 3001), rng.integers(0, 2, 3001)
+    for at, p, n in ((0, 900, 1), (63, 500, 2), (64, 700, 30), (1500, 0, 40), (2944, 300, 1), (3000, 1500, 3)):
+        past[at], new[at] = p, n
+    st = setup(15, [int(x) for x in past], [int(x) for x in new], 2, 1, 64, 16, "f16")
+    check(st, call(st))
+    st["q"] = st["q"].astype(np.float32)
+    check(st, call(st, hints=False))
+    one = setup(16, [int(x) for x in past], [1] * 3001, 2, 1, 64, 16, "f16")
+    check(one, call(one))
+
+
+@pytest.mark.parametrize("size,ty", [(1e-4, "f32"), (300.0, "f32"), (60000.0, "f32"), (1e-30, "f32"), (1e30, "f32"), (1e-4, "f16"), (60000.0, "f16")])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_queries_of_any_size(size, ty, d):
+    st = setup(17, [50, 9], [1, 40], 8, 2, d, 16, "f32", gain=1.0)
+    st["q"] = (st["q"] * np.float32(size / 4.5)).astype(NP[ty])
+    check(st, call(st, scale=0.08 / size), scale=0.08 / size)
+    check(st, call(st, softcap=3.0, scale=0.08 / size), softcap=3.0, scale=0.08 / size)
 
 
 def test_hints_do_not_change_what_is_computed():
@@ -287,7 +310,7 @@ def test_refusals():
     assert go(kc=f(3, 2, 24, 64)) == A.ERR_UNSUPPORTED and go(kc=f(3, 2, 2048, 64)) == A.ERR_UNSUPPORTED
     assert go(q=f(4, 4, 96), kc=f(3, 2, 16, 96)) == A.ERR_UNSUPPORTED
     assert go(kc=f(3, 3, 16, 64)) == A.ERR_INVALID  # 4 heads over 3
-    assert go(window=-1) == A.ERR_INVALID and go(softcap=-1.0) == A.ERR_INVALID and go(softcap=float("nan")) == A.ERR_INVALID
+    assert go(window=-1) == A.ERR_INVALID and go(softcap=-1.0) == A.ERR_INVALID and go(softcap=float("nan")) == A.ERR_INVALID and go(softcap=1e-40) == A.ERR_INVALID
     assert go(scale=float("inf")) == A.ERR_INVALID and go(max_new=-1) == A.ERR_INVALID
     odd = f(4 * 4 * 64 + 4)[4:].view(4, 4, 64)
     assert go(q=odd, out=f(4, 4, 64)) == A.ERR_INVALID and go(out=odd) == A.ERR_INVALID

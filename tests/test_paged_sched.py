@@ -31,6 +31,7 @@ int main(int argc, char **argv) {
     c.min_share = decode ? 2 : 512;
     c.target = pick(1, 96);
     c.alone = c.target / 2;
+    c.rooms = decode ? c.target : 1 << 30;
     c.cut_cost = pick(0, 3) ? pick(0, 1300) : -1;
     c.window = pick(0, 2) ? 0 : pick(1, 500);
     c.max_len = pick(1, 1 << 14);
@@ -81,10 +82,11 @@ int main(int argc, char **argv) {
     CHECK(share >= 1 && share * c.target >= work);
     const bool whole = sched_whole(c, tiles, work, longest);
     if (c.cut_cost < 0) CHECK(whole);
+    else CHECK(!whole || tiles <= c.rooms);
     if (wild) continue;
     const int64_t bound = sched_tiles_bound(c, 0);
     CHECK(tiles <= bound);
-    CHECK((whole ? tiles : (work + share - 1) / share) <= sched_items_bound(c, bound));
+    if (!whole) CHECK((work + share - 1) / share <= c.target);
     // a share begins at most one tile that it does not end: its parts have distinct slots
     if (!whole) {
       std::vector<int> used(sched_slots_bound(c), 0);
