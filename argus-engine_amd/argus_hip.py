@@ -461,6 +461,8 @@ def _heads(what, device, dtype, tokens, heads, d, t):
     token, head, one = t.stride()
     if (one != 1 and d > 1) or (head != d and heads > 1):
         raise ValueError(what + ": the heads of a token must be packed")
+    if token == 0 and tokens > 1:  # 0 is "packed" to the library
+        raise ValueError(what + ": tokens must not share a row")
     return t.data_ptr(), token if tokens > 1 else heads * d
 
 

@@ -180,6 +180,13 @@ ARGUS_API int argus_hip_page_plan(argus_hip_ctx *ctx, const argus_hip_page_plan_
   if (!a->cu_new || !a->counts || (a->n_seqs && (!a->past_len || !a->new_len || !a->page_table || !a->kv_len)) ||
       (a->token_capacity && (!a->positions || !a->slots)) || (a->n_free && !a->free_pages))
     return argus_fail(ctx, ARGUS_HIP_ERR_INVALID, "page_plan: null pointer");
+  // every workgroup reads the lengths, in its own time
+  const auto meet = [&](const int32_t *in, const int32_t *out, int n_out) {
+    return (uintptr_t)in < (uintptr_t)(out + n_out) && (uintptr_t)out < (uintptr_t)(in + a->n_seqs);
+  };
+  for (const int32_t *in : {a->past_len, a->new_len})
+    if (a->n_seqs && (meet(in, a->kv_len, a->n_seqs) || meet(in, a->cu_new, a->n_seqs + 1)))
+      return argus_fail(ctx, ARGUS_HIP_ERR_INVALID, "page_plan: kv_len and cu_new lie in the lengths they are computed from");
   const DeviceGuard guard(ctx);
   PagePlanParams p{a->past_len, a->new_len, a->free_pages, a->page_table, a->cu_new, a->kv_len, a->positions, a->slots, a->counts,
                    a->n_seqs, a->n_free, a->n_pages, argus_log2(a->page_size), a->table_stride, a->token_capacity};

@@ -88,6 +88,9 @@ int check(argus_hip_ctx *ctx, const argus_hip_paged_attention_args *a) {
       a->table_stride <= 0)
     return argus_fail(ctx, ARGUS_HIP_ERR_INVALID, "paged_attention: n_seqs %d n_tokens %d heads %d / %d n_pages %d table_stride %d", a->n_seqs,
                       a->n_tokens, a->heads_q, a->heads_kv, a->n_pages, a->table_stride);
+  if ((int64_t)a->n_tokens * (a->heads_q / a->heads_kv) > 0x7fffffff)
+    return argus_fail(ctx, ARGUS_HIP_ERR_UNSUPPORTED, "paged_attention: %d tokens of %d heads per KV head are more than 2^31 - 1 rows", a->n_tokens,
+                      a->heads_q / a->heads_kv);
   if (a->head_dim != 64 && a->head_dim != 128 && a->head_dim != 256)
     return argus_fail(ctx, ARGUS_HIP_ERR_UNSUPPORTED, "paged_attention: head_dim %d is not 64, 128 or 256", a->head_dim);
   if (!argus_page_size_ok(a->page_size))
@@ -99,7 +102,8 @@ int check(argus_hip_ctx *ctx, const argus_hip_paged_attention_args *a) {
     return argus_fail(ctx, ARGUS_HIP_ERR_INVALID, "paged_attention: layout %d", a->layout);
   if (a->dtype != ARGUS_HIP_F32 && a->dtype != ARGUS_HIP_F16)
     return argus_fail(ctx, ARGUS_HIP_ERR_UNSUPPORTED, "paged_attention: dtype %d", a->dtype);
-  if (a->window < 0 || a->min_new < 0 || a->max_new < 0 || a->max_kv < 0 || !(a->softcap == 0.0f || a->softcap >= 1.17549435e-38f) || !(a->softcap < __builtin_huge_valf()) ||
+  if (a->window < 0 || a->min_new < 0 || a->max_new < 0 || a->max_kv < 0 ||
+      !(a->softcap == 0.0f || a->softcap >= __FLT_MIN__) || !(a->softcap < __builtin_huge_valf()) ||
       !(a->scale > -__builtin_huge_valf() && a->scale < __builtin_huge_valf()))
     return argus_fail(ctx, ARGUS_HIP_ERR_INVALID, "paged_attention: window %d min_new %d max_new %d max_kv %d softcap %g scale %g", a->window,
                       a->min_new, a->max_new, a->max_kv, a->softcap, a->scale);

@@ -419,6 +419,7 @@ class HipPagedKvCache {
                const float *cos_sin, size_t n_positions, size_t rot_dim, bool interleaved = false, float weight_bias = 0.0f) {
     if (layer >= c_.layers || !tokens_) return Status::Err("paged cache: no such layer, or no step is open");
     if (k.dtype != q.dtype || v.dtype != q.dtype) return Status::Err("paged cache: q, k and v have one dtype");
+    if (!holds(q, c_.heads_q) || !holds(k, c_.heads_kv) || !holds(v, c_.heads_kv) || !holds(q_out, c_.heads_q)) return Status::Err("paged cache: a tensor is too small for the step's tokens");
     argus_hip_qk_norm_rope_args a{};
     a.q = q.ptr, a.k = k.ptr, a.v = v.ptr, a.q_weight = q_weight, a.k_weight = k_weight, a.cos_sin = cos_sin;
     a.positions = pos_, a.slots = slots_, a.q_out = q_out.ptr, a.k_cache = pools_[2 * layer], a.v_cache = pools_[2 * layer + 1];
@@ -431,6 +432,7 @@ class HipPagedKvCache {
   Status attend(size_t layer, const Tensor &q, Tensor &out, size_t window = 0, float softcap = 0.0f, float scale = 0.0f) {
     if (layer >= c_.layers || !tokens_) return Status::Err("paged cache: no such layer, or no step is open");
     if (q.dtype != out.dtype) return Status::Err("paged cache: q and out have one dtype");
+    if (!holds(q, c_.heads_q) || !holds(out, c_.heads_q)) return Status::Err("paged cache: a tensor is too small for the step's tokens");
     argus_hip_paged_attention_args a{};
     a.q = q.ptr, a.k_cache = pools_[2 * layer], a.v_cache = pools_[2 * layer + 1], a.page_table = table_, a.cu_new = cu_, a.kv_len = kv_, a.out = out.ptr;
     a.n_seqs = (int32_t)c_.max_seqs, a.n_tokens = (int32_t)tokens_, a.heads_q = (int32_t)c_.heads_q, a.heads_kv = (int32_t)c_.heads_kv;
@@ -458,6 +460,11 @@ class HipPagedKvCache {
     for (size_t p = 0; p < c.n_pages; ++p) free_list_.push_back((int32_t)p);
   }
   size_t pages(size_t tokens) const { return (tokens + c_.page_size - 1) / c_.page_size; }
+  bool holds(const Tensor &t, size_t heads) const {
+    size_t n = 1;
+    for (size_t x : t.dims) n *= x;
+    return n >= tokens_ * heads * c_.head_dim;
+  }
   int32_t layout() const { return c_.head_major ? ARGUS_HIP_HEAD_MAJOR : ARGUS_HIP_SEQ_MAJOR; }
   HipBackend &be_;
   Config c_;

@@ -668,7 +668,8 @@ int argus_hip_kv_scatter_f32_batch(argus_hip_ctx *ctx, void *stream, const float
  *   counts = { total tokens, pages needed, requests that ran short of free pages or of table_stride }.
  * Negative lengths count as 0, sums saturate at 2^31 - 1, tokens past token_capacity are left out (the
  * caller sees counts[0] > token_capacity).  Everything is written in place and depends on the inputs
- * alone: the same call again gives the same tables.  n_seqs at most 16384. */
+ * alone: the same call again gives the same tables.  Outputs do not overlap the inputs (kv_len is not
+ * past_len: ARGUS_HIP_ERR_INVALID).  n_seqs at most 16384. */
 typedef struct argus_hip_page_plan_args {
   void *stream;
   const int32_t *past_len;   /* device [n_seqs] */
@@ -696,8 +697,8 @@ int argus_hip_page_plan(argus_hip_ctx *ctx, const argus_hip_page_plan_args *args
  *     (a, b) -> (a cos - b sin, b cos + a sin)
  * in F32, rounded once.  q goes to q_out, k and v (v only converted) to row slots[t] of the pools.
  * A token whose slot lies outside the pool leaves the pool alone (its q_out row is written); a token
- * whose position lies outside [0, n_positions) is padding: nothing is written for it.  Two tokens with
- * the same slot leave one of the two rows there.  q_out may be q itself (same type and stride).
+ * whose position lies outside [0, n_positions) is padding: nothing is written for it.  Two tokens
+ * must not have the same slot (its row would hold pieces of either).  q_out may be q itself (same type and stride).
  * rot_dim is a multiple of 8, at most head_dim, or 0: no rotation, cos_sin and positions may be NULL
  * (positions that are given mark padding by being negative).
  * Row strides are in elements between tokens, multiples of 4, 0 = packed; rows are 16-byte (F32) or
@@ -749,11 +750,13 @@ int argus_hip_qk_norm_rope(argus_hip_ctx *ctx, const argus_hip_qk_norm_rope_args
  * the probabilities as F16 pairs (hi + lo), so the result is that of F32 arithmetic,
  * whatever the size of the queries is.
  * max_new / max_kv: no request brings more new tokens / holds more tokens than this (0 = not known).
- * They choose kernels, and rows of a request that brings more than max_new may be left unwritten.
  * min_new: no request with any new token brings fewer (0 = not known).
+ * They choose kernels; where max_new or min_new does not hold, rows may be left unwritten.  out does not
+ * overlap the inputs.
  * The partial results of requests cut along their length need a workspace: the caller's
  * (argus_hip_paged_attention_workspace bytes at least, 256-byte aligned, one per stream at a time), or
- * with workspace NULL the context's, which grows with a device synchronisation -- a call under stream
+ * with workspace NULL the context's, which serves one stream at a time and grows with a device
+ * synchronisation -- a call under stream
  * capture has to bring its own (ARGUS_HIP_ERR_INVALID otherwise). */
 typedef struct argus_hip_paged_attention_args {
   void *stream;

@@ -111,6 +111,10 @@ def test_refusals():
     assert call(n_pages=0) == A.ERR_INVALID and call(n_pages=1 << 27) == A.ERR_INVALID
     assert call(n=16385) == A.ERR_UNSUPPORTED and "16384" in ctx().last_error()
     assert call(table=z(2, 0)) == A.ERR_INVALID
+    past = z(2)
+    assert ctx().page_plan(past, z(2), z(4), z(2, 3), 16, 64, z(3), past, z(6), z(6), z(3), check=False) == A.ERR_INVALID
+    whole = z(4)
+    assert ctx().page_plan(z(2), whole[2:], z(4), z(2, 3), 16, 64, whole[:3], z(2), z(6), z(6), z(3), check=False) == A.ERR_INVALID
     with pytest.raises(ValueError):
         call(table=z(3, 3))
     with pytest.raises(TypeError):

@@ -38,7 +38,7 @@ def attention_args(**kw):
     (dict(n_seqs=-1), -1), (dict(n_tokens=-1), -1), (dict(heads_kv=3), -1), (dict(heads_q=0), -1), (dict(n_pages=0), -1),
     (dict(table_stride=0), -1), (dict(layout=2), -1), (dict(window=-1), -1), (dict(softcap=float("inf")), -1), (dict(scale=float("nan")), -1),
     (dict(min_new=-1), -1), (dict(max_kv=-1), -1), (dict(q_stride=1028), -1), (dict(out_stride=-8), -1),
-    (dict(head_dim=96), -2), (dict(page_size=15), -2), (dict(page_size=2048), -2), (dict(dtype=2), -2)])
+    (dict(softcap=1e-40), -1), (dict(n_tokens=2 ** 30, heads_q=8, heads_kv=2), -2), (dict(head_dim=96), -2), (dict(page_size=15), -2), (dict(page_size=2048), -2), (dict(dtype=2), -2)])
 def test_paged_attention_checks_its_arguments_without_a_device(kw, code):
     # the workspace query makes the checks of the call; without a context it assumes 256 compute units
     import argus_hip as A
@@ -66,6 +66,20 @@ def test_tensors_in_host_memory_are_refused():
         c.qk_norm_rope(f(2, 4, 64), f(2, 2, 64), f(2, 2, 64), i(2), torch.zeros(5, 64), f(2, 4, 64), f(3, 2, 16, 64), f(3, 2, 16, 64), i(2))
     with pytest.raises(ValueError):
         c.paged_attention(f(2, 4, 64), f(3, 2, 16, 64), f(3, 2, 16, 64), i(2, 3), i(3), i(2), f(2, 4, 64))
+
+
+def test_rows_shared_by_tokens_are_refused():
+    import argus_hip as A
+    import torch
+    c = A.Context.__new__(A.Context)
+    c.handle, c.device = None, -1  # host tensors pass for the context's: the refusal comes before the library
+    i = lambda *s: torch.zeros(s, dtype=torch.int32)  # noqa: E731
+    f = lambda *s: torch.zeros(s, dtype=torch.float16)  # noqa: E731
+    one = f(1, 4, 64).expand(2, 4, 64)
+    with pytest.raises(ValueError, match="share"):
+        c.paged_attention(one, f(3, 2, 16, 64), f(3, 2, 16, 64), i(2, 3), i(3), i(2), f(2, 4, 64))
+    with pytest.raises(ValueError, match="share"):
+        c.qk_norm_rope(one, f(2, 2, 64), f(2, 2, 64), i(2), torch.zeros(5, 64), f(2, 4, 64), f(3, 2, 16, 64), f(3, 2, 16, 64), i(2))
 
 
 # ---- the references --------------------------------------------------------------------------------
