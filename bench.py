@@ -272,6 +272,35 @@ def bench_prefill(ctx, steps, warmup, hq=32, hkv=8, d=64, s=2048, batch=1, f16_i
                 tflops_wall=round(flops / wall / 1e12, 1))
 
 
+def bench_paged(steps, warmup, only=None):
+    """The paged-cache operators on the cases of perf/operators.py (tables, lengths and sizes stand there): per
+    case the time of a call in a stream of calls over three sets of tensors, and the rates of the bytes and
+    operations the case cannot do without.  No kernel brackets: the calls are short."""
+    import importlib.util
+    import torch
+    spec = importlib.util.spec_from_file_location("paged_operators", os.path.join(ROOT, "perf", "operators.py"))
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    mod.own = True
+    res = {}
+    for case in mod.listed():
+        if only and case["name"] != only:
+            continue
+        sets = [mod.prepare(case, seed) for seed in range(3)]
+        turn = [0]
+
+        def step():
+            turn[0] += 1
+            mod.run(sets[turn[0] % 3])
+
+        t = time_region(step, steps, warmup)
+        w = mod.work(case)
+        res[case["name"]] = dict(us_per_call=round(t * 1e6, 2), gbps=round(w["bytes"] / t / 1e9, 1), tflops=round(w["flops"] / t / 1e12, 2))
+        del sets, step
+        torch.cuda.empty_cache()
+    return res
+
+
 def bench_aux(ctx, steps, warmup):
     """The data-movement kernels either side of the attention calls, each at a size of the benchmark
     configurations: microseconds per call (torch events on the current stream, `steps` calls back to
@@ -487,8 +516,9 @@ def main():
     ap.add_argument("--no-cpu", action="store_true", help="skip the CPU baseline leg")
     ap.add_argument("--workload", default="primary",
                     choices=["primary", "decode_b1", "prefill", "prefill_d128", "kivi_q4", "kivi_q8", "cfg5", "q4_0", "q4_0_b1", "primary_scores_stats",
-                             "q8_0", "q4_0_d64", "copy_calib", "aux", "layers", "primary_scores", "cfg5_b64", "prefill_d64_16k"],
+                             "q8_0", "q4_0_d64", "copy_calib", "aux", "layers", "primary_scores", "cfg5_b64", "prefill_d64_16k", "paged"],
                     help="run one secondary workload alone (for profiling) instead of the primary line")
+    ap.add_argument("--case", default=None, help="one case of --workload paged")
     args = ap.parse_args()
     if args.gpus != 1:
         print("bench.py: this build measures one GPU only (every box has one GPU; the path shards by "
@@ -515,6 +545,8 @@ def main():
             res = {"bytes_read": src.numel() * 4, "bytes_written": src.numel() * 4}
         elif w == "aux":
             res = bench_aux(ctx, args.steps, args.warmup)
+        elif w == "paged":
+            res = bench_paged(args.steps, args.warmup, args.case)
         elif w == "layers":
             res = bench_layer_loop(ctx, args.steps, args.warmup)
         elif w == "primary_scores":
