@@ -42,63 +42,109 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
 }
 
 // Merge of the parts of cut tiles: row m of a tile is sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m).  One
-// share begins a cut tile at most, its last one.  D / 4 threads share a row's channels.  Decode tiles (PG > 1)
-// have few rows and up to hundreds of parts: a workgroup takes one row, its thread groups every PG-th part,
-// and the groups are added in LDS; chunk tiles (PG 1) have many rows of two or three parts.
-template <int D, typename T, bool DECODE>
-__device__ __forceinline__ void combine_cut(const PagedParams &p, int block) {
-  constexpr int TPR = D / 4, PG = DECODE ? 256 / TPR : 1, RPB = DECODE ? 1 : 256 / TPR;
-  constexpr int R = DECODE ? kDecodeRows : kChunkRows;
-  constexpr int chunks = R / RPB;
-  static_assert(R % RPB == 0, "whole workgroups per tile");
-  const int w = block / (chunks * p.heads_kv), kvh = block / chunks % p.heads_kv;
-  const PagedCut cut = p.cuts[w];
-  const int lr = block % chunks * RPB + (DECODE ? 0 : threadIdx.x / TPR), ch = threadIdx.x % TPR * 4;
-  if (cut.parts == 0 || lr >= cut.rows) return;  // DECODE: the whole workgroup
-  const int G = p.sched.group, n = cut.parts, row = cut.row0 + lr;
-  // parts: slot 2 w + 1, then 2 (w + 1), 2 (w + 2), ..
-  const int64_t step = (int64_t)p.heads_kv * R, row_at = (int64_t)kvh * R + lr;
-  auto part = [&](int i) { return (int64_t)(2 * (w + i) + (i == 0)) * step + row_at; };
-  float m = kNegInf, l = 0.0f, m_ref;
-  if constexpr (DECODE) {  // a lane per part, every wave for itself
-    const int lane = threadIdx.x & 63;
-    for (int i = lane; i < n; i += 64) m = fmaxf(m, p.ws_ml[part(i) * 2]);
-    m = wave_allreduce_max(m);
-    m_ref = m == kNegInf ? 0.0f : m;
-    for (int i = lane; i < n; i += 64) l += p.ws_ml[part(i) * 2 + 1] * __builtin_amdgcn_exp2f(p.ws_ml[part(i) * 2] - m_ref);
-    l = wave_allreduce_sum(l);
-  } else {
-    for (int i = 0; i < n; ++i) m = fmaxf(m, p.ws_ml[part(i) * 2]);
-    m_ref = m == kNegInf ? 0.0f : m;
-    for (int i = 0; i < n; ++i) l += p.ws_ml[part(i) * 2 + 1] * __builtin_amdgcn_exp2f(p.ws_ml[part(i) * 2] - m_ref);
-  }
-  float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-  for (int i = DECODE ? threadIdx.x / TPR : 0; i < n; i += PG) {
-    const int64_t at = part(i);
-    const float f = __builtin_amdgcn_exp2f(p.ws_ml[at * 2] - m_ref);
-    const float4_t x = *(const float4_t *)(p.ws_o + at * D + ch);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) o[e] += x[e] * f;
-  }
-  if constexpr (DECODE) {
-    __shared__ float4_t sum[256];
-    sum[threadIdx.x] = o;
-    __syncthreads();
-    if (threadIdx.x >= TPR) return;
-#pragma unroll
-    for (int g = 1; g < PG; ++g) o += sum[g * TPR + threadIdx.x];
-  }
-  T *out = (T *)p.out + (int64_t)(cut.q_begin + row / G) * p.out_stride + (int64_t)(kvh * G + row % G) * D + ch;
+// share begins a cut tile at most, its last one.  D / 4 threads share a row's channels.  Decode tiles have few
+// rows and up to hundreds of parts: a workgroup takes one row, its thread groups every PG-th part, and the
+// groups are added in LDS.  Chunk tiles have many rows of two or three parts: two rows per thread.  Bound by
+// the latency of its loads: the descriptor, then everything else at once.
+template <typename T>
+__device__ __forceinline__ void store_row(T *out, const float4_t &o, float l) {
   typedef T T4 __attribute__((ext_vector_type(4)));
   T4 y;
 #pragma unroll
   for (int e = 0; e < 4; ++e) y[e] = (T)(l == 0.0f ? 0.0f : o[e] / l);
   *(T4 *)out = y;
 }
+template <int D, typename T, bool DECODE>
+__device__ __forceinline__ void combine_cut(const PagedParams &p, int block) {
+  constexpr int TPR = D / 4, PG = 256 / TPR;
+  constexpr int R = DECODE ? kDecodeRows : kChunkRows, RPB = DECODE ? 1 : 2 * PG;
+  constexpr int blocks = R / RPB;
+  static_assert(R % RPB == 0, "whole workgroups per tile");
+  typedef float float2_t __attribute__((ext_vector_type(2)));
+  const int w = block / (blocks * p.heads_kv), kvh = block / blocks % p.heads_kv;
+  const PagedCut cut = p.cuts[w];
+  const int first = block % blocks * RPB, group = threadIdx.x / TPR, ch = threadIdx.x % TPR * 4;
+  if (cut.parts == 0 || first >= cut.rows) return;  // the whole workgroup
+  const int G = p.sched.group, n = cut.parts;
+  // parts: slot 2 w + 1, then 2 (w + 1), 2 (w + 2), ..
+  const int64_t step = (int64_t)p.heads_kv * R;
+  auto part = [&](int i, int row) { return (int64_t)(2 * (w + i) + (i == 0)) * step + (int64_t)kvh * R + row; };
+  auto out = [&](int row) { return (T *)p.out + (int64_t)(cut.q_begin + row / G) * p.out_stride + (int64_t)(kvh * G + row % G) * D + ch; };
+  if constexpr (DECODE) {
+    constexpr int AHEAD = 4;
+    const int lane = threadIdx.x & 63;
+    float4_t x[AHEAD];  // this group's first parts (behind the last one: that again)
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+      if (u * PG < n) x[u] = *(const float4_t *)(p.ws_o + part(min(u * PG + group, n - 1), first) * D + ch);
+    float2_t ml = {kNegInf, 0.0f};  // of part `lane`, every wave for itself
+    if (lane < n) ml = *(const float2_t *)(p.ws_ml + part(lane, first) * 2);
+    float m = ml[0];
+    for (int i = lane + 64; i < n; i += 64) m = fmaxf(m, p.ws_ml[part(i, first) * 2]);
+    m = wave_allreduce_max(m);
+    const float m_ref = m == kNegInf ? 0.0f : m;
+    const float f64 = __builtin_amdgcn_exp2f(ml[0] - m_ref);  // factors of the first 64 parts
+    float l = ml[1] * f64;
+    for (int i = lane + 64; i < n; i += 64) l += p.ws_ml[part(i, first) * 2 + 1] * __builtin_amdgcn_exp2f(p.ws_ml[part(i, first) * 2] - m_ref);
+    l = wave_allreduce_sum(l);
+    float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+      if (u * PG < n) {  // AHEAD * PG <= 64
+        const int i = u * PG + group;
+        const float f = __shfl(f64, i, 64);
+        if (i < n) o += x[u] * f;
+      }
+#pragma unroll 4
+    for (int i = AHEAD * PG + group; i < n; i += PG) {
+      const int64_t at = part(i, first);
+      o += *(const float4_t *)(p.ws_o + at * D + ch) * __builtin_amdgcn_exp2f(p.ws_ml[at * 2] - m_ref);
+    }
+    __shared__ float4_t sum[256];
+    sum[threadIdx.x] = o;
+    __syncthreads();
+    if (threadIdx.x >= TPR) return;
+#pragma unroll
+    for (int g = 1; g < PG; ++g) o += sum[g * TPR + threadIdx.x];
+    store_row(out(cut.row0 + first), o, l);
+  } else {
+    float4_t x[2][2];
+    float2_t ml[2][2];
+    int row[2];
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      row[k] = first + k * PG + group;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {  // a cut tile has two parts at least
+        const int64_t at = part(i, min(row[k], cut.rows - 1));
+        x[k][i] = *(const float4_t *)(p.ws_o + at * D + ch);
+        ml[k][i] = *(const float2_t *)(p.ws_ml + at * 2);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      float m = kNegInf, l = 0.0f;
+      float4_t o = {0.0f, 0.0f, 0.0f, 0.0f};
+      auto add = [&](const float4_t &xi, const float2_t &mli) {
+        const float m_new = fmaxf(m, mli[0]), m_ref = m_new == kNegInf ? 0.0f : m_new;
+        const float old = __builtin_amdgcn_exp2f(m - m_ref), f = __builtin_amdgcn_exp2f(mli[0] - m_ref);
+        m = m_new;
+        l = l * old + mli[1] * f;
+        o = o * old + xi * f;
+      };
+      add(x[k][0], ml[k][0]);
+      add(x[k][1], ml[k][1]);
+      for (int i = 2; i < n; ++i) {
+        const int64_t at = part(i, min(row[k], cut.rows - 1));
+        add(*(const float4_t *)(p.ws_o + at * D + ch), *(const float2_t *)(p.ws_ml + at * 2));
+      }
+      if (row[k] < cut.rows) store_row(out(cut.row0 + row[k]), o, l);
+    }
+  }
+}
 
 template <int D, bool DECODE>
-constexpr int kCutBlocks = DECODE ? kDecodeRows : kChunkRows / (256 / (D / 4));  // workgroups per cut and KV head
+constexpr int kCutBlocks = DECODE ? kDecodeRows : kChunkRows / (2 * (256 / (D / 4)));  // workgroups per cut and KV head
 
 template <int D, typename T, bool DECODE>
 __global__ __launch_bounds__(256) void paged_combine_kernel(const PagedParams p) {
