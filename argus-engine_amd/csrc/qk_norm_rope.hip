@@ -5,7 +5,8 @@
 //
 // A lane holds the two groups of W channels that rotate into each other (W i .. and rot/2 + W i .., or
 // 2 W i .. 2 W i + 2 W - 1 with adjacent pairs), so the rotation needs no exchange and the norm one
-// reduction over the head's lanes; W = 8, or 4 where alignment or rot_dim asks for it.  Bound by HBM for many tokens, by the launch for few.
+// reduction over the head's lanes; W = 8, or 4 where alignment or rot_dim asks for it.  Bound by HBM for many tokens (8192 of 32/8 heads, d 128,
+// F16: 40.3 us, 5.1 TB/s), by the launch for few (16 in F32: 3.5 us).
 #include "paged_common.hpp"
 
 #include <type_traits>
@@ -150,6 +151,7 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const QkNormRopeParam
 template <int D, int W, typename IN, typename OUT>
 int launch(argus_hip_ctx *ctx, QkNormRopeParams &p, int tokens, hipStream_t stream) {
   constexpr int HPB = 256 / (D / (2 * W));
+  // few tokens: a token's heads over several workgroups, for shorter chains; many: one, which loads the angles once
   const int chunks = (p.heads_q + 2 * p.heads_kv + HPB - 1) / HPB;
   p.chunks = (int64_t)tokens * chunks <= (int64_t)ctx->compute_units * 8 ? chunks : 1;
   const int64_t grid = (int64_t)tokens * p.chunks;
