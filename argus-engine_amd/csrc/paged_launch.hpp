@@ -41,11 +41,7 @@ __global__ __launch_bounds__(256, (ChunkTile<D, std::is_same<T, float>::value>::
   else chunk_share<D, T, CAP, 1>(cp, PagedShare(cp.sched, cp.cu_new, cp.kv_len, w), w, kvh, (_Float16 *)lds);
 }
 
-// Merge of the parts of cut tiles: row m of a tile is sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m).  One
-// share begins a cut tile at most, its last one.  D / 4 threads share a row's channels.  Decode tiles have few
-// rows and up to hundreds of parts: a workgroup takes one row, its thread groups every PG-th part, and the
-// groups are added in LDS.  Chunk tiles have many rows of two or three parts: two rows per thread.  Bound by
-// the latency of its loads: the descriptor, then everything else at once.
+// Four channels of an output row; a row that saw nothing is zeros.
 template <typename T>
 __device__ __forceinline__ void store_row(T *out, const float4_t &o, float l) {
   typedef T T4 __attribute__((ext_vector_type(4)));
@@ -54,6 +50,12 @@ __device__ __forceinline__ void store_row(T *out, const float4_t &o, float l) {
   for (int e = 0; e < 4; ++e) y[e] = (T)(l == 0.0f ? 0.0f : o[e] / l);
   *(T4 *)out = y;
 }
+
+// Merge of the parts of cut tiles: row m of a tile is sum_i o_i 2^(m_i - m) / sum_i l_i 2^(m_i - m).  One
+// share begins a cut tile at most, its last one.  D / 4 threads share a row's channels.  Decode tiles have few
+// rows and up to hundreds of parts: a workgroup takes one row, its thread groups every PG-th part, and the
+// groups are added in LDS.  Chunk tiles have many rows of two or three parts: two rows per thread.  Bound by
+// the latency of its loads: the descriptor, then everything else at once.
 template <int D, typename T, bool DECODE>
 __device__ __forceinline__ void combine_cut(const PagedParams &p, int block) {
   constexpr int TPR = D / 4, PG = 256 / TPR;
