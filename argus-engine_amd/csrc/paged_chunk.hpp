@@ -42,8 +42,10 @@ struct ChunkTile {
 //   phase B   O += V . P(t)                         beside  the first half of tile t + 1's
 // K tiles are staged in LDS two steps ahead, V tiles one; one barrier per step.  Interior steps -- every row
 // of the workgroup sees all of tiles t and t + 1 -- carry no masks and take no maximum: their exponents
-// stand against a reference some earlier tile of the row set, and a probability only leaves F16's range
-// where a logit exceeds it by 16 (log2), which shows in the row sum.
+// stand against a reference some earlier tile of the row set.  A weight only leaves F16's range where a logit
+// exceeds it by 16 (log2), and the row sum tells: of F16 rows it adds the rounded weights, an infinity among
+// them; of F32 rows the weights themselves, none of which is above the sum, so it is held below F16's largest
+// number.  Then the tile is weighed again against its own maximum.
 // Share `w` of KV head `kvh`; ARG: which of the kernel's PagedParams arguments `p` is.
 template <int D, typename T, bool CAP, int ARG>
 __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare work, int w, int kvh, _Float16 *smem) {
@@ -57,6 +59,7 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
   constexpr int SETS = DEEP ? 2 : 1;
   constexpr float kLog2e = 1.4426950408889634f;
   constexpr int kSplit = PS / 2;        // slices of P^T formed in phase B of the step before
+  constexpr float kMostSum = F32 ? 65504.0f : 1e30f;  // of a lane's weights in an interior step, as they are
   constexpr int kAhead = 4, kVAhead = D <= 64 ? 4 : 3;  // operand reads kept in flight
   
   _Float16 *const sK = smem, *const sV = smem + 2 * BN * KP;  // [2][BN][KP], [2][BN][VP]
@@ -398,8 +401,8 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
     if constexpr (INTERIOR) {
       float sum = l_head + exp_part(s_cur, p_cur, p_lo, std::true_type{}, JS{}, JN{});
       sched_qk();
-      if (__builtin_amdgcn_ballot_w64(!(sum < 1e30f)) != 0) {
-        const float over = row_max(s_cur, std::true_type{}) - m_ref, delta = over > kLazy ? over : 0.0f;
+      if (__builtin_amdgcn_ballot_w64(!(sum < kMostSum)) != 0) {
+        const float delta = fmaxf(row_max(s_cur, std::true_type{}) - m_ref, 0.0f);
         rescale(__builtin_amdgcn_exp2f(-delta));
         m_ref += delta;
         m_run = m_ref;

@@ -1,0 +1,105 @@
+"""paged_attention on values that move a softmax's reference, leave F16's range or are not finite, over
+requests long enough for every part of the kernels; against plain softmax attention in 64 bits."""
+import numpy as np
+import pytest
+
+import paged_util as U
+from test_gpu_paged_attention import NP, call, setup
+
+pytestmark = pytest.mark.gpu
+SHAPES = {64: (14, 2), 128: (8, 2), 256: (4, 2)}
+
+
+def reference(q, k, v, kv_len, softcap=0.0, window=0, scale=None):
+    """(out, tolerance) of one request, q [new, Hq, d]; keys whose logit is -inf have no weight.
+
+    Errors, u = 2^-24: a logit is d products summed in F32, scaled by rounded factors, F32 queries held as two
+    F16 halves (2^-22 of the terms' size), the cap's own evaluation ~8 roundings of the cap; a weight is off by
+    twice that (weight and sum).  Sums run over steps of 16 keys.  F16: weights rounded to F16 (2^-11 each, and
+    in the sum), then the output.  F32: weights are two halves, 2^-22 each.  Below F16's smallest normal number
+    a weight is off by half of its smallest step instead, 2^-25 of the largest weight."""
+    f16 = q.dtype == np.float16
+    n, hq, d = q.shape
+    g = hq // k.shape[1]
+    scale = d ** -0.5 if scale is None else scale
+    u = 2.0 ** -24
+    pos = kv_len - n + np.arange(n)
+    key = np.arange(kv_len)
+    sees = key <= pos[:, None]
+    if window:
+        sees &= key > pos[:, None] - window
+    out, tol = np.zeros((n, hq, d)), np.zeros((n, hq, d))
+    for h in range(hq):
+        qq, kk, vv = q[:, h].astype(np.float64), k[:, h // g].astype(np.float64), v[:, h // g].astype(np.float64)
+        with np.errstate(invalid="ignore"):
+            s = qq @ kk.T * scale
+        assert not np.isnan(s).any() and not (s == np.inf).any()
+        see = sees & (s != -np.inf)
+        size = np.where(see, np.abs(qq) @ np.where(np.isfinite(kk), np.abs(kk), 0).T, 0).max(1) * abs(scale)
+        if softcap:
+            s = softcap * np.tanh(s / softcap)
+        s = np.where(see, s, -np.inf)
+        top = s.max(1, keepdims=True)
+        p = np.exp(s - np.where(np.isfinite(top), top, 0))
+        total = p.sum(1, keepdims=True)
+        p = np.divide(p, total, out=np.zeros_like(p), where=total > 0)
+        o = p @ vv
+        a = p @ np.abs(vv)
+        logit = (d + 8) * u * size + (0.0 if f16 else 2.0 ** -22 * size) + 8 * u * softcap
+        w = 2 * logit + 16 * u + 2 * (see.sum(1) / 16 + 64) * u
+        half = 2.0 ** -11 if f16 else 2.0 ** -21
+        floor = 2.0 ** -25 * (see @ np.abs(vv)) * p.max(1, keepdims=True)
+        out[:, h] = o
+        tol[:, h] = a * (w + 2 * half)[:, None] + 2 * floor + (2.0 ** -11 if f16 else u) * np.abs(o) * (1 + 1e-3) + (2.0 ** -25 if f16 else 1e-37)
+    return out, tol
+
+
+def check(st, got, what="", **kw):
+    cu, kv = st["cu"], st["kv"]
+    for s, (k, v) in enumerate(st["rows"]):
+        ref, tol = reference(st["q"][cu[s]:cu[s + 1]], k, v, int(kv[s]), **kw)
+        U.within(got[cu[s]:cu[s + 1]], ref, tol, "%s request %d" % (what, s))
+    assert (got[cu[-1]:] == -9.0).all()
+
+
+def put(st, s, keys, k=None, v=None, ch=slice(None)):
+    """Sets channels `ch` of K and / or V of request s's tokens, in the pools and in the contiguous rows."""
+    page = st["kc"].shape[2]
+    for t in keys:
+        for pool, row, x in ((st["kc"], st["rows"][s][0], k), (st["vc"], st["rows"][s][1], v)):
+            if x is not None:
+                row[t, :, ch] = x
+                pool[st["table"][s, t // page], :, t % page, ch] = x
+
+
+def levels(seed, past, new, d, ty, page=16):
+    """A call whose channel 0 only adds to the logits: queries hold 8 there, keys 0 (see put)."""
+    hq, hkv = SHAPES[d]
+    st = setup(seed, past, new, hq, hkv, d, page, ty, gain=1.0)
+    st["q"][:st["cu"][-1], :, 0] = 8.0
+    for s in range(len(past)):
+        put(st, s, range(past[s] + new[s]), k=0.0, ch=0)
+    return st
+
+
+@pytest.mark.parametrize("ty", ["f16", "f32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("softcap", [0.0, 80.0])
+def test_keys_far_above_the_first_ones(softcap, d, ty):
+    """Keys 12, 20, 30 and 60 nats above those in front of them, where tiles are taken without a maximum:
+    tiles of even and odd number, keys in both halves of a tile, rows that see several of them, and a level
+    that rises again."""
+    nat = np.sqrt(d) / 8
+    for past, new in (([1100], [48]), ([1800], [3]), ([0], [900]), ([2600, 700], [70, 130])):
+        for jump in (12.0, 20.0, 30.0, 60.0):
+            st = levels(d + past[0], past, new, d, ty)
+            for s in range(len(past)):
+                n = past[s] + new[s]
+                for i, at in enumerate((n // 5, n // 5 + 17, n // 3, n // 2, n // 2 + 33, n // 2 + 65, n * 3 // 4)):
+                    put(st, s, [at], k=nat * (jump + (i > 4)), ch=0)
+            check(st, call(st, softcap), "jump %g past %r" % (jump, past), softcap=softcap)
+        st = levels(d + past[0] + 1, past, new, d, ty)  # a level that climbs by 4 nats every 80 keys
+        for s in range(len(past)):
+            for t in range(past[s] + new[s]):
+                put(st, s, [t], k=nat * min(4.0 * (t // 80), 70.0), ch=0)
+        check(st, call(st, softcap), "climbing past %r" % (past,), softcap=softcap)
