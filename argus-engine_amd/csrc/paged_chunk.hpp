@@ -470,6 +470,7 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
       }
       // tile t has its logits but no maximum yet, and its early slices are formed again with the others
       alpha = mask_max(Even{}, t, s_a);
+      if constexpr (F32) __syncthreads();  // it may have read K tile t again, which the next step refills
     }
     for (; t < n_it; t += 2) {
       step(t, s_a, s_b, p_a, p_a, alpha, std::false_type{}, Even{});

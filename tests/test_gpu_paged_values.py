@@ -103,3 +103,21 @@ def test_keys_far_above_the_first_ones(softcap, d, ty):
             for t in range(past[s] + new[s]):
                 put(st, s, [t], k=nat * min(4.0 * (t // 80), 70.0), ch=0)
         check(st, call(st, softcap), "climbing past %r" % (past,), softcap=softcap)
+
+
+def infinite(st, s, keys):
+    """The logits of these keys are -inf in every row: K holds -inf where all queries hold 1."""
+    st["q"][:st["cu"][-1], :, 1] = 1.0
+    put(st, s, keys, k=-np.inf, ch=1)
+
+
+@pytest.mark.parametrize("ty", ["f16", "f32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_an_infinite_key_in_the_tile_behind_the_unmasked_steps(d, ty):
+    """408 tokens in tiles of 32 keys (64 at d 64), none cut: the steps without a maximum end with tile 9 (3).
+    The tile behind them holds the key; the one two further on, which takes its place, does not."""
+    for past, new in (([360], [48]), ([360, 40], [48, 60])):
+        for at in ((256, 259, 318) if d == 64 else (320, 325, 350)):
+            st = setup(d + at, past, new, *SHAPES[d], d, 16, ty, gain=1.0)
+            infinite(st, 0, [at])
+            check(st, call(st), "key %d" % at)
