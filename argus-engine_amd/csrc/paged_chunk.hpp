@@ -64,6 +64,7 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
   
   _Float16 *const sK = smem, *const sV = smem + 2 * BN * KP;  // [2][BN][KP], [2][BN][VP]
   __shared__ int bad_tile[2];  // tile whose V held infinities or NaN under a mask
+  __shared__ int unseen;       // a row's first tile had no logit above -inf
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 31, hl = lane >> 5;
@@ -433,6 +434,7 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
 
   STile s_a, s_b;
   if (threadIdx.x < 2) bad_tile[threadIdx.x] = -1;
+  if (threadIdx.x == 2) unseen = 0;
   if (n_it > 0) {
     constexpr int S1 = DEEP ? 1 : 0;
     typedef std::integral_constant<int, 0> Even;
@@ -442,7 +444,7 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
     if constexpr (DEEP) fetch_k(1, kpre[1]);
     __builtin_amdgcn_sched_barrier(0);
     load_q();
-    __syncthreads();  // bad_tile
+    __syncthreads();  // bad_tile, unseen
     stage_k(Even{}, kpre[0]);
     stage_v(Even{}, 0, vpre[0], seen_whole(0));
     if constexpr (!DEEP) fetch_k(1, kpre[0]);
@@ -455,9 +457,12 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
     qk_tile(Even{}, s_a);
     sched_qk();
     float alpha = mask_max(Even{}, 0, s_a);
+    if (m_run == kNegInf) unseen = 1;
     __syncthreads();  // sK[0] is refilled by the first step
     int t = 0;
-    const int n_int = full_from == 0 ? max(0, full_upto - 1) & ~1 : 0;  // steps whose tile and the next are seen whole
+    // Steps whose tile and the next are seen whole.  They need a reference: where a row has met no key yet (all
+    // its logits are -inf), the masked steps, which set one at the first key, take all tiles.
+    const int n_int = full_from == 0 && !unseen ? max(0, full_upto - 1) & ~1 : 0;
     if (n_int > 0) {
       if constexpr (CAP) {  // an interior step starts from products
         qk_tile(Even{}, s_a);

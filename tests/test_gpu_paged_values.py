@@ -121,3 +121,17 @@ def test_an_infinite_key_in_the_tile_behind_the_unmasked_steps(d, ty):
             st = setup(d + at, past, new, *SHAPES[d], d, 16, ty, gain=1.0)
             infinite(st, 0, [at])
             check(st, call(st), "key %d" % at)
+
+
+@pytest.mark.parametrize("ty", ["f16", "f32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_rows_whose_first_tiles_are_all_minus_infinity(d, ty):
+    """The first keys have no weight in any row; the ones behind them are ordinary, or far below zero (they
+    vanish against a reference of 0), with a long and a short end behind them."""
+    for past, new in (([1100], [48]), ([0], [700]), ([2900, 350], [40, 60])):
+        for level in (0.0, -200.0):
+            st = levels(d + past[0] + 2, past, new, d, ty)
+            for s in range(len(past)):
+                put(st, s, range(past[s] + new[s]), k=np.sqrt(d) / 8 * level, ch=0)
+                infinite(st, s, range(80))
+            check(st, call(st), "level %g past %r" % (level, past))
