@@ -65,6 +65,7 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
   _Float16 *const sK = smem, *const sV = smem + 2 * BN * KP;  // [2][BN][KP], [2][BN][VP]
   __shared__ int bad_tile[2];  // tile whose V held infinities or NaN under a mask
   __shared__ int unseen;       // a row's first tile had no logit above -inf
+  __shared__ int not_a_number;  // a part's row sum
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 31, hl = lane >> 5;
@@ -87,6 +88,10 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
   const int vlane_off = (4 * (g16 >> 1) + (s16 >> 2)) * VP + 16 * (g16 & 1) + 4 * (s16 & 3);
 
   PagedCut cut{0, 0, 0, 0};
+  // F32: rows whose sums come out as NaN are formed once more, in masked steps only.  They tell an infinite logit
+  // from the NaN that its two halves make of it; the others take no such care.
+  bool again = false;
+  uint64_t again_rows = ~0ull;  // of this wave: the rows to store
   while (work.found) {  // the tiles this share touches
   const PagedPlace it = work.at;
   const int64_t from = work.from(), upto = work.upto();
@@ -98,7 +103,7 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
   if (!entire && from == 0) cut = PagedCut{(int)((it.start + it.cost - 1) / work.share) - w + 1, it.s.q_begin, row0, row_last + 1 - row0};
 
   const int row = row0 + 32 * wave + ln;
-  const bool row_ok = row < n_rows;
+  const bool row_ok = row < n_rows && (again_rows >> lane & 1);
   const int rr = min(row, row_last);  // rows past the last one repeat it and are not stored
   const int tok = rr / G, head = kvh * G + rr % G;
   const int pos = it.s.pos0 + tok;
@@ -426,6 +431,7 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
       sched_pv();
       if (!seen_whole(t) && bad_tile[Buf::value] == t) add_bad(t);
       if (t + 1 < n_it) alpha = mask_max(Other{}, t + 1, s_next);
+      else if (F32 && l_run != l_run) not_a_number = 1;
     }
     stage_k(Buf{}, kpre[STAGE]);
     stage_v(Other{}, t + 1, vpre[STAGE], INTERIOR || seen_whole(t + 1));
@@ -445,6 +451,7 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
     __builtin_amdgcn_sched_barrier(0);
     load_q();
     __syncthreads();  // bad_tile, unseen
+    if (threadIdx.x == 2) not_a_number = 0;  // everyone has read the last part's
     stage_k(Even{}, kpre[0]);
     stage_v(Even{}, 0, vpre[0], seen_whole(0));
     if constexpr (!DEEP) fetch_k(1, kpre[0]);
@@ -462,7 +469,7 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
     int t = 0;
     // Steps whose tile and the next are seen whole.  They need a reference: where a row has met no key yet (all
     // its logits are -inf), the masked steps, which set one at the first key, take all tiles.
-    const int n_int = full_from == 0 && !unseen ? max(0, full_upto - 1) & ~1 : 0;
+    const int n_int = full_from == 0 && !unseen && !again ? max(0, full_upto - 1) & ~1 : 0;
     if (n_int > 0) {
       if constexpr (CAP) {  // an interior step starts from products
         qk_tile(Even{}, s_a);
@@ -513,6 +520,16 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
         for (int e = 0; e < 4; ++e) o[e] = (T)(l_run == 0.0f ? 0.0f : o_acc[r][4 * i4 + e] * inv);
         *(T4 *)(out + 32 * r + 8 * i4 + 4 * hl) = o;
       }
+  }
+  if constexpr (F32) {
+    const bool first = !again;
+    again = false;
+    again_rows = ~0ull;
+    if (first && n_it > 0 && __builtin_amdgcn_readfirstlane(not_a_number) != 0) {
+      again = true;
+      again_rows = __builtin_amdgcn_ballot_w64(l_run != l_run);
+      continue;
+    }
   }
   work.next(p.sched, p.cu_new, p.kv_len);
   }

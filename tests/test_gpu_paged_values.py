@@ -135,3 +135,32 @@ def test_rows_whose_first_tiles_are_all_minus_infinity(d, ty):
                 put(st, s, range(past[s] + new[s]), k=np.sqrt(d) / 8 * level, ch=0)
                 infinite(st, s, range(80))
             check(st, call(st), "level %g past %r" % (level, past))
+
+
+@pytest.mark.parametrize("ty", ["f16", "f32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_infinite_keys_anywhere(d, ty):
+    """Keys of -inf logits in tiles that are taken without masks: they have no weight, and a row that sees no
+    other key is zeros."""
+    for past, new in (([1100], [48]), ([0], [900]), ([2900, 350], [40, 60])):
+        st = levels(d + past[0] + 3, past, new, d, ty)
+        for s in range(len(past)):
+            n = past[s] + new[s]
+            infinite(st, s, [n // 7, n // 3, n // 3 + 1, n // 2, n - 3] + list(range(n // 5, n // 5 + 150)))
+        check(st, call(st), "past %r" % (past,))
+        check(st, call(st, softcap=0.0, window=600), "window past %r" % (past,), window=600)
+        for s in range(len(past)):
+            infinite(st, s, range(past[s] + new[s]))
+        assert (call(st)[:st["cu"][-1]] == 0).all()
+
+
+@pytest.mark.parametrize("ty", ["f16", "f32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_a_key_that_is_not_a_number_reaches_the_rows_that_see_it(d, ty):
+    for past, new, at in ((1100, 48, 200), (0, 900, 500), (2900, 40, 2920)):
+        st = setup(d + at, [past], [new], *SHAPES[d], d, 16, ty, gain=1.0)
+        clean = call(st)
+        put(st, 0, [at], k=np.nan, ch=5)
+        got = call(st)[:new]
+        sees = past + np.arange(new) >= at
+        assert np.isnan(got[sees]).all() and np.array_equal(got[~sees], clean[:new][~sees])
