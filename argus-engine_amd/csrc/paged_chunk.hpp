@@ -65,7 +65,7 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
   _Float16 *const sK = smem, *const sV = smem + 2 * BN * KP;  // [2][BN][KP], [2][BN][VP]
   __shared__ int bad_tile[2];  // tile whose V held infinities or NaN under a mask
   __shared__ int unseen;       // a row's first tile had no logit above -inf
-  __shared__ int not_a_number;  // a part's row sum
+  __shared__ int not_a_number;  // a part's row
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int ln = lane & 31, hl = lane >> 5;
@@ -88,8 +88,9 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
   const int vlane_off = (4 * (g16 >> 1) + (s16 >> 2)) * VP + 16 * (g16 & 1) + 4 * (s16 & 3);
 
   PagedCut cut{0, 0, 0, 0};
-  // F32: rows whose sums come out as NaN are formed once more, in masked steps only.  They tell an infinite logit
-  // from the NaN that its two halves make of it; the others take no such care.
+  // F32: rows that come out as NaN are formed once more, in masked steps only.  They tell an infinite logit from
+  // the NaN that its two halves make of it, and add an infinite value by itself, which times the two halves of a
+  // weight is NaN as well; the other steps take no such care.
   bool again = false;
   uint64_t again_rows = ~0ull;  // of this wave: the rows to store
   while (work.found) {  // the tiles this share touches
@@ -169,7 +170,7 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
     for (int i = 0; i < CH; ++i)
       *(half8_t *)(sV + stage_row * VP + 8 * my_col + (decltype(buf_c)::value * BN + RPW * i) * VP) = pre[i];
   };
-  auto seen_whole = [&](int t) __attribute__((always_inline)) { return t >= full_from && t < full_upto; };
+  auto seen_whole = [&](int t) __attribute__((always_inline)) { return !(F32 && again) && t >= full_from && t < full_upto; };
 
   // ---- Q as the B operand: lane (row ln, half hl) holds channels 16 kk + 8 hl .. + 7
   half8_t qh[KK], ql[F32 ? KK : 1];
@@ -390,6 +391,15 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
     }
   };
 
+  auto row_is_nan = [&]() __attribute__((always_inline)) {  // this lane's part of the row, or its sum
+    float x = l_run;
+#pragma unroll
+    for (int r = 0; r < RB; ++r)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x = __builtin_fmaf(o_acc[r][i], 0.0f, x);
+    return x != x;
+  };
+
   PTile p_a, p_b, p_lo;
   float l_head = 0.0f;   // row sum of the slices formed early
   // One step: on entry s_cur holds the logits of tile t (edge steps: masked, their reference set, the sums'
@@ -431,7 +441,7 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
       sched_pv();
       if (!seen_whole(t) && bad_tile[Buf::value] == t) add_bad(t);
       if (t + 1 < n_it) alpha = mask_max(Other{}, t + 1, s_next);
-      else if (F32 && l_run != l_run) not_a_number = 1;
+      else if (F32 && row_is_nan()) not_a_number = 1;
     }
     stage_k(Buf{}, kpre[STAGE]);
     stage_v(Other{}, t + 1, vpre[STAGE], INTERIOR || seen_whole(t + 1));
@@ -527,7 +537,8 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
     again_rows = ~0ull;
     if (first && n_it > 0 && __builtin_amdgcn_readfirstlane(not_a_number) != 0) {
       again = true;
-      again_rows = __builtin_amdgcn_ballot_w64(l_run != l_run);
+      again_rows = __builtin_amdgcn_ballot_w64(row_is_nan());
+      again_rows |= again_rows >> 32 | again_rows << 32;  // a row's two lanes
       continue;
     }
   }

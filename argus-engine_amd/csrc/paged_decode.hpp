@@ -71,6 +71,9 @@ __device__ __forceinline__ void decode_share(const PagedParams &p, PagedShare wo
   __shared__ float lds_m[kWaves][16], lds_l[kWaves][16];
 
   PagedCut cut{0, 0, 0, 0};
+  // F32: an infinite V times the two halves of a weight is NaN.  A wave whose results hold one goes over its keys
+  // again with the care that masked keys get, which adds such values by themselves.
+  bool again = false;
   while (work.found) {  // the requests this share touches
   const PagedPlace it = work.at;
   const int rows = (it.s.q_end - it.s.q_begin) * G;  // at most 16: one tile
@@ -183,7 +186,7 @@ __device__ __forceinline__ void decode_share(const PagedParams &p, PagedShare wo
     }
     load_k(base + kWaves * STEP);
     // keys some row does not see: past the first token's position, in front of the last one's window, past the part
-    const bool edge = base + STEP - 1 > it.s.pos0 || base + STEP > end || (window != 0x7fffffff && base <= pos_last - window);
+    const bool edge = (F32 && again) || base + STEP - 1 > it.s.pos0 || base + STEP > end || (window != 0x7fffffff && base <= pos_last - window);
 #pragma unroll
     for (int tw = 0; tw < TW; ++tw)
 #pragma unroll
@@ -308,6 +311,15 @@ __device__ __forceinline__ void decode_share(const PagedParams &p, PagedShare wo
         }
       }
     load_v();
+  }
+  if constexpr (F32) {
+    float x = 0.0f;
+#pragma unroll
+    for (int a = 0; a < NACC; ++a)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x = __builtin_fmaf(o_acc[a][i], 0.0f, x);
+    again = !again && __builtin_amdgcn_ballot_w64(x != x) != 0;
+    if (again) continue;
   }
 
   // ---- merge: lane groups (row sum), then the waves through LDS -----------------------------------
