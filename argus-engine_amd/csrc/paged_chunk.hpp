@@ -43,7 +43,7 @@ struct ChunkTile {
 // K tiles are staged in LDS two steps ahead, V tiles one; one barrier per step.  Interior steps -- every row
 // of the workgroup sees all of tiles t and t + 1 -- carry no masks and take no maximum: their exponents
 // stand against a reference some earlier tile of the row set.  A weight only leaves F16's range where a logit
-// exceeds it by 16 (log2), and the row sum tells: of F16 rows it adds the rounded weights, an infinity among
+// exceeds it by 16 (log2; 6 in F32 rows), and the row sum tells: of F16 rows it adds the rounded weights, an infinity among
 // them; of F32 rows the weights themselves, none of which is above the sum, so it is held below F16's largest
 // number.  Then the tile is weighed again against its own maximum.
 // Share `w` of KV head `kvh`; ARG: which of the kernel's PagedParams arguments `p` is.
@@ -271,7 +271,11 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
     if constexpr (CAP && decltype(raw_c)::value) mt = soft_cap<F32>(mt, cap, cap_in);
     return mt * ce;
   };
-  constexpr float kLazy = 8.0f;
+  // Weights of F32 rows stand 2^10 higher, so that what a pair of F16 halves cannot hold is 2^-35 of the reference,
+  // not 2^-25 (thousands of keys that far below the largest one add up): its weight is 2^10, and 2^15 where the
+  // reference lags most, which leaves F16's range a factor of two.
+  constexpr float kUp = F32 ? 10.0f : 0.0f;
+  constexpr float kLazy = F32 ? 5.0f : 8.0f;
   // Cap, mask and maximum of tile t.  The reference moves where a row's maximum exceeds it by more than
   // kLazy (log2), or when the row sees its first key; the factor its sums take with it is returned.
   auto mask_max = [&](auto buf_c, int t, STile &s) __attribute__((always_inline)) -> float {
@@ -337,6 +341,7 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
   // probabilities of slices [J0, J1) of a tile; returns their row sum (this half's keys)
   auto exp_part = [&](STile &s, PTile &ph, PTile &pl, auto raw_c, auto j0_c, auto j1_c) __attribute__((always_inline)) -> float {
     float sum = 0.0f;
+    const float off = F32 ? kUp - m_ref : -m_ref;
 #pragma unroll
     for (int jn = decltype(j0_c)::value; jn < decltype(j1_c)::value; ++jn) {
       typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
@@ -344,7 +349,7 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
       for (int e = 0; e < 8; ++e) {
         float x = s[jn / 2][8 * (jn % 2) + e];
         if constexpr (CAP && decltype(raw_c)::value) x = soft_cap<F32>(x, cap, cap_in);
-        x = __builtin_amdgcn_exp2f(__builtin_fmaf(x, ce, -m_ref));
+        x = __builtin_amdgcn_exp2f(__builtin_fmaf(x, ce, off));
         if constexpr (F32) {
           _Float16 hi, lo;
           split_f16(x, hi, lo);

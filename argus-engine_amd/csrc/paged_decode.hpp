@@ -216,11 +216,13 @@ __device__ __forceinline__ void decode_share(const PagedParams &p, PagedShare wo
     m_run = m_new;
     half4_t pa[TW], pl[F32 ? TW : 1];
     float lsum = 0.0f;
+    // Weights of F32 rows stand 2^14 higher: what a pair of F16 halves cannot hold is then 2^-39 of the largest
+    const float off = F32 ? m_ref - 14.0f : m_ref;
 #pragma unroll
     for (int tw = 0; tw < TW; ++tw)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float w = __builtin_amdgcn_exp2f(s[tw][i] - m_ref);
+        const float w = __builtin_amdgcn_exp2f(s[tw][i] - off);
         lsum += w;
         if constexpr (F32) {
           _Float16 hi, lo;

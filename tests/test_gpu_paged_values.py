@@ -16,8 +16,9 @@ def reference(q, k, v, kv_len, softcap=0.0, window=0, scale=None):
     Errors, u = 2^-24: a logit is d products summed in F32, scaled by rounded factors, F32 queries held as two
     F16 halves (2^-22 of the terms' size), the cap's own evaluation ~8 roundings of the cap; a weight is off by
     twice that (weight and sum).  Sums run over steps of 16 keys.  F16: weights rounded to F16 (2^-11 each, and
-    in the sum), then the output.  F32: weights are two halves, 2^-22 each.  Below F16's smallest normal number
-    a weight is off by half of its smallest step instead, 2^-25 of the largest weight."""
+    in the sum), then the output.  F32: weights are two halves, 2^-22 each.  Where a half is below F16's smallest
+    normal number it is off by half of its smallest step instead, 2^-25; F32 rows are weighed with 2^10 at least
+    in the place of 1, which makes that 2^-35 of the largest weight."""
     f16 = q.dtype == np.float16
     n, hq, d = q.shape
     g = hq // k.shape[1]
@@ -48,7 +49,7 @@ def reference(q, k, v, kv_len, softcap=0.0, window=0, scale=None):
         logit = (d + 8) * u * size + (0.0 if f16 else 2.0 ** -22 * size) + 8 * u * softcap
         w = 2 * logit + 16 * u + 2 * (see.sum(1) / 16 + 64) * u
         half = 2.0 ** -11 if f16 else 2.0 ** -21
-        floor = 2.0 ** -25 * (see @ np.abs(vv)) * p.max(1, keepdims=True)
+        floor = (2.0 ** -25 if f16 else 2.0 ** -35) * (see @ np.abs(vv)) * p.max(1, keepdims=True)
         out[:, h] = o
         tol[:, h] = a * (w + 2 * half)[:, None] + 2 * floor + (2.0 ** -11 if f16 else u) * np.abs(o) * (1 + 1e-3) + (2.0 ** -25 if f16 else 1e-37)
     return out, tol
@@ -201,3 +202,19 @@ def test_an_infinite_value_that_all_rows_see(d, ty):
             whole = ~special.any(-1)
             assert np.array_equal(got[:new][whole], want[whole]), (past, new)
             assert (np.abs(rest - want[~special]) <= 1e-4).all(), (past, new)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("softcap", [0.0, 90.0])
+def test_a_long_tail_far_below_one_key_counts_in_f32(softcap, d):
+    """One key takes nearly all the weight and holds 0 in V; what is left of the result is the thousands of keys
+    17 to 22 nats below it."""
+    for past, new in ((8191, 1), (8000, 48), (0, 1000), (20000, 2)):
+        for at in (10, (past + new) // 2, past):
+            for nats in (17.5, 20.0, 22.0):
+                st = levels(d + past + 4, [past], [new], d, "f32")
+                put(st, 0, [at], k=np.sqrt(d) / 8 * nats, ch=0)
+                st["vc"][:] = np.abs(st["vc"])
+                st["rows"][0][1][:] = np.abs(st["rows"][0][1])
+                put(st, 0, [at], v=0.0)
+                check(st, call(st, softcap), "%g nats at %d of %d" % (nats, at, past + new), softcap=softcap)
