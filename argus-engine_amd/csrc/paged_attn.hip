@@ -133,7 +133,7 @@ ARGUS_API int argus_hip_paged_attention(argus_hip_ctx *ctx, const argus_hip_page
   CallPlan pl;
   if (rc == ARGUS_HIP_OK) rc = make_plan(ctx, ctx->compute_units, a, pl);
   if (rc != ARGUS_HIP_OK) return rc;
-  if (a->n_seqs == 0 || a->n_tokens == 0) return ARGUS_HIP_OK;
+  if (a->n_seqs == 0 || a->n_tokens == 0 || pl.d_items + pl.c_items == 0) return ARGUS_HIP_OK;  // no request can have a token
   if (!a->q || !a->k_cache || !a->v_cache || !a->page_table || !a->cu_new || !a->kv_len || !a->out)
     return argus_fail(ctx, ARGUS_HIP_ERR_INVALID, "paged_attention: null pointer");
   if (((uintptr_t)a->q | (uintptr_t)a->k_cache | (uintptr_t)a->v_cache | (uintptr_t)a->out) & 15)

@@ -218,3 +218,10 @@ def test_a_long_tail_far_below_one_key_counts_in_f32(softcap, d):
                 st["rows"][0][1][:] = np.abs(st["rows"][0][1])
                 put(st, 0, [at], v=0.0)
                 check(st, call(st, softcap), "%g nats at %d of %d" % (nats, at, past + new), softcap=softcap)
+
+
+def test_a_step_whose_bounds_leave_no_request_a_token():
+    # rows of a batch of fixed size, every request idle: whoever brings tokens would bring more than there are
+    st = setup(1, [20, 5], [0, 0], 4, 2, 64, 16, "f16", pad_rows=4)
+    assert (call(st, hints=False, min_new=8) == -9.0).all()
+    assert (call(st, hints=False, min_new=8, max_new=8) == -9.0).all()
