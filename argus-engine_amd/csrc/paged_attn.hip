@@ -109,6 +109,8 @@ int check(argus_hip_ctx *ctx, const argus_hip_paged_attention_args *a) {
                       a->min_new, a->max_new, a->max_kv, a->softcap, a->scale);
   if (a->q_stride < 0 || a->out_stride < 0 || (a->q_stride | a->out_stride) % 8)
     return argus_fail(ctx, ARGUS_HIP_ERR_INVALID, "paged_attention: row strides are non-negative multiples of 8 elements");
+  if (a->n_tokens > 1 && a->out_stride && a->out_stride < (int64_t)a->heads_q * a->head_dim)
+    return argus_fail(ctx, ARGUS_HIP_ERR_INVALID, "paged_attention: rows of out overlap (out_stride %lld)", (long long)a->out_stride);
   return ARGUS_HIP_OK;
 }
 

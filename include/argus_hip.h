@@ -702,7 +702,8 @@ int argus_hip_page_plan(argus_hip_ctx *ctx, const argus_hip_page_plan_args *args
  * rot_dim is a multiple of 8, at most head_dim, or 0: no rotation, cos_sin and positions may be NULL
  * (positions that are given mark padding by being negative).
  * Row strides are in elements between tokens, multiples of 4, 0 = packed; rows are 16-byte (F32) or
- * 8-byte (F16) aligned, so slices of one projection's output are read in place. */
+ * 8-byte (F16) aligned, so slices of one projection's output are read in place.  Rows of q_out do not
+ * overlap (ARGUS_HIP_ERR_INVALID for a smaller stride). */
 typedef struct argus_hip_qk_norm_rope_args {
   void *stream;
   const void *q;            /* [tokens, heads_q, head_dim] of in_dtype */
@@ -752,7 +753,7 @@ int argus_hip_qk_norm_rope(argus_hip_ctx *ctx, const argus_hip_qk_norm_rope_args
  * max_new / max_kv: no request brings more new tokens / holds more tokens than this (0 = not known).
  * min_new: no request with any new token brings fewer (0 = not known).
  * They choose kernels; where max_new or min_new does not hold, rows may be left unwritten.  out does not
- * overlap the inputs.
+ * overlap the inputs, nor its rows each other (ARGUS_HIP_ERR_INVALID for a smaller out_stride).
  * The partial results of requests cut along their length need a workspace: the caller's
  * (argus_hip_paged_attention_workspace bytes at least, 256-byte aligned, one per stream at a time), or
  * with workspace NULL the context's, which serves one stream at a time and grows with a device
