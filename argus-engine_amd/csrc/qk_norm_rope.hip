@@ -206,6 +206,8 @@ ARGUS_API int argus_hip_qk_norm_rope(argus_hip_ctx *ctx, const argus_hip_qk_norm
     return argus_fail(ctx, ARGUS_HIP_ERR_INVALID, "qk_norm_rope: row strides are non-negative multiples of 4 elements");
   if (a->tokens > 1 && p.q_out_stride < (int64_t)a->heads_q * d)
     return argus_fail(ctx, ARGUS_HIP_ERR_INVALID, "qk_norm_rope: rows of q_out overlap (q_out_stride %lld)", (long long)p.q_out_stride);
+  if (a->q_out == a->q && (a->in_dtype != a->out_dtype || (a->tokens > 1 && p.q_stride != p.q_out_stride)))
+    return argus_fail(ctx, ARGUS_HIP_ERR_INVALID, "qk_norm_rope: q in place takes one type and one stride");
   const uintptr_t in_mask = a->in_dtype == ARGUS_HIP_F16 ? 7 : 15, out_mask = a->out_dtype == ARGUS_HIP_F16 ? 7 : 15;
   if ((((uintptr_t)a->q | (uintptr_t)a->k | (uintptr_t)a->v) & in_mask) || ((uintptr_t)a->q_out & out_mask) ||
       (((uintptr_t)a->k_cache | (uintptr_t)a->v_cache) & 15) ||

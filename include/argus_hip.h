@@ -698,7 +698,8 @@ int argus_hip_page_plan(argus_hip_ctx *ctx, const argus_hip_page_plan_args *args
  * in F32, rounded once.  q goes to q_out, k and v (v only converted) to row slots[t] of the pools.
  * A token whose slot lies outside the pool leaves the pool alone (its q_out row is written); a token
  * whose position lies outside [0, n_positions) is padding: nothing is written for it.  Two tokens
- * must not have the same slot (its row would hold pieces of either).  q_out may be q itself (same type and stride).
+ * must not have the same slot (its row would hold pieces of either).  q_out may be q itself (same type and
+ * stride, ARGUS_HIP_ERR_INVALID otherwise).
  * rot_dim is a multiple of 8, at most head_dim, or 0: no rotation, cos_sin and positions may be NULL
  * (positions that are given mark padding by being negative).
  * Row strides are in elements between tokens, multiples of 4, 0 = packed; rows are 16-byte (F32) or

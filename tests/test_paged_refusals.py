@@ -29,3 +29,19 @@ def test_overlapping_rows_are_refused_by_the_calls():
                                              torch.arange(4, dtype=torch.int32, device="cuda"), check=False)
     assert rope(f(4, 4, 64), rows) == A.ERR_INVALID
     assert rope(rows, f(4, 4, 64)) == A.OK  # reading a row twice is no harm
+
+
+@pytest.mark.gpu
+def test_queries_in_place_keep_their_type_and_stride():
+    import argus_hip as A
+    import torch
+    from gpu_util import ctx
+    f = lambda *s, ty=torch.float16: torch.zeros(s, dtype=ty, device="cuda")  # noqa: E731
+    wide = f(4, 8, 64)
+    same = wide.view(4, 8, 64)[:, :4]
+    rope = lambda q, out, n=4: ctx().qk_norm_rope(q, f(n, 2, 64, ty=q.dtype), f(n, 2, 64, ty=q.dtype), None, None, out, f(3, 2, 16, 64),  # noqa: E731
+                                                  f(3, 2, 16, 64), torch.arange(n, dtype=torch.int32, device="cuda"), check=False)
+    assert rope(same, same) == A.OK
+    assert rope(same, wide.view(-1)[:1024].view(4, 4, 64)) == A.ERR_INVALID
+    assert rope(same, wide.view(-1)[:2048].view(torch.float32).view(4, 4, 64)) == A.ERR_INVALID
+    assert rope(same[:1], wide.view(-1)[:256].view(1, 4, 64), 1) == A.OK  # one token has no stride
