@@ -344,6 +344,10 @@ class HipPagedKvCache {
   static Result<std::shared_ptr<HipPagedKvCache>> create(HipBackend &be, const Config &c) {
     typedef Result<std::shared_ptr<HipPagedKvCache>> R;
     if (!c.layers || !c.heads_q || !c.heads_kv || !c.n_pages || !c.max_seqs || !c.max_pages_per_seq || !c.max_tokens) return R::Err("paged cache: a size is zero");
+    // what the three calls take; page_size divides below
+    if (c.page_size < 16 || c.page_size > ARGUS_HIP_MAX_PAGE_SIZE || (c.page_size & (c.page_size - 1))) return R::Err("paged cache: page_size is not a power of two from 16 to " + std::to_string(ARGUS_HIP_MAX_PAGE_SIZE));
+    if (c.head_dim != 64 && c.head_dim != 128 && c.head_dim != 256) return R::Err("paged cache: head_dim is not 64, 128 or 256");
+    if (c.heads_q % c.heads_kv) return R::Err("paged cache: heads_q is not a multiple of heads_kv");
     std::shared_ptr<HipPagedKvCache> p(new HipPagedKvCache(be, c));
     const size_t pool = c.n_pages * c.heads_kv * c.page_size * c.head_dim * 2;
     auto get = [&](size_t bytes, void **out) {
