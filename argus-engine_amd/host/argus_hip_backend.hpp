@@ -385,6 +385,7 @@ class HipPagedKvCache {
     if (new_len.size() != c_.max_seqs) return Status::Err("paged cache: one length per request slot");
     size_t tokens = 0, need = 0;
     int32_t most = 0;
+    size_t longest = 0;
     for (size_t s = 0; s < c_.max_seqs; ++s) {
       if (new_len[s] < 0) return Status::Err("paged cache: negative length");
       const size_t want = pages((size_t)past_len_[s] + (size_t)new_len[s]);
@@ -392,6 +393,7 @@ class HipPagedKvCache {
       need += want - pages((size_t)past_len_[s]);
       tokens += (size_t)new_len[s];
       most = std::max(most, new_len[s]);
+      if (new_len[s]) longest = std::max(longest, (size_t)past_len_[s] + (size_t)new_len[s]);
     }
     if (need > free_list_.size()) return Status::Err("paged cache: " + std::to_string(need) + " pages needed, " + std::to_string(free_list_.size()) + " free");
     if (tokens > c_.max_tokens) return Status::Err("paged cache: too many new tokens");
@@ -415,6 +417,7 @@ class HipPagedKvCache {
     new_len_ = new_len;
     tokens_ = tokens;
     max_new_ = most;
+    longest_ = longest;
     return OkStatus();
   }
   // q [tokens, heads_q, head_dim], k / v [tokens, heads_kv, head_dim] of one dtype, packed; q_out like q, F32 or
@@ -424,6 +427,8 @@ class HipPagedKvCache {
     if (layer >= c_.layers || !tokens_) return Status::Err("paged cache: no such layer, or no step is open");
     if (k.dtype != q.dtype || v.dtype != q.dtype) return Status::Err("paged cache: q, k and v have one dtype");
     if (!holds(q, c_.heads_q) || !holds(k, c_.heads_kv) || !holds(v, c_.heads_kv) || !holds(q_out, c_.heads_q)) return Status::Err("paged cache: a tensor is too small for the step's tokens");
+    // the operator takes a position outside the table for padding and writes nothing for it
+    if (rot_dim && longest_ > n_positions) return Status::Err("paged cache: a position lies behind the " + std::to_string(n_positions) + " rows of cos_sin");
     argus_hip_qk_norm_rope_args a{};
     a.q = q.ptr, a.k = k.ptr, a.v = v.ptr, a.q_weight = q_weight, a.k_weight = k_weight, a.cos_sin = cos_sin;
     a.positions = pos_, a.slots = slots_, a.q_out = q_out.ptr, a.k_cache = pools_[2 * layer], a.v_cache = pools_[2 * layer + 1];
@@ -477,7 +482,8 @@ class HipPagedKvCache {
           *counts_ = nullptr;
   std::vector<int32_t> past_len_, new_len_, free_list_;
   std::vector<std::vector<int32_t>> held_;
-  size_t tokens_ = 0;  // of the open step
+  size_t tokens_ = 0;   // of the open step
+  size_t longest_ = 0;  // tokens of the longest request that joins it
   int32_t max_new_ = 0;
 };
 

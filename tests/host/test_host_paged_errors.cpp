@@ -45,6 +45,54 @@ static void test_configs(HipBackend &be) {
   CHECK(!HipPagedKvCache::create(be, c).ok(), "5 heads over 2");
 }
 
+struct DevBuf {
+  HipBackend &be;
+  void *p = nullptr;
+  DevBuf(HipBackend &b, const std::vector<float> &x) : be(b) {
+    auto r = be.alloc(x.size() * 4);
+    CHECK(r.ok() && be.write_buffer(r.value(), x.data(), x.size() * 4).ok(), "upload");
+    p = r.ok() ? r.value() : nullptr;
+  }
+  ~DevBuf() { (void)be.free(p); }
+};
+
+// Tensors of a step of up to `most` tokens and angles of 64 positions.
+struct Step {
+  static constexpr size_t most = 80, hq = 4, hkv = 2, d = 64, positions = 64;
+  std::vector<float> x;
+  DevBuf q, k, v, qo, o, cs;
+  Tensor tq, tk, tv, tqo, to;
+  static std::vector<float> values(size_t n, uint32_t seed) {
+    std::vector<float> x(n);
+    for (float &y : x) seed = seed * 1664525u + 1013904223u, y = (float)(seed >> 8) / 8388608.0f - 1.0f;
+    return x;
+  }
+  Step(HipBackend &be, uint32_t seed)
+      : q(be, values(most * hq * d, seed)), k(be, values(most * hkv * d, seed + 1)), v(be, values(most * hkv * d, seed + 2)),
+        qo(be, std::vector<float>(most * hq * d, 0.0f)), o(be, std::vector<float>(most * hq * d, 0.0f)), cs(be, values(positions * d, 5)),
+        tq{q.p, DType::F32, {most, hq, d}, true}, tk{k.p, DType::F32, {most, hkv, d}, true}, tv{v.p, DType::F32, {most, hkv, d}, true},
+        tqo{qo.p, DType::F32, {most, hq, d}, true}, to{o.p, DType::F32, {most, hq, d}, true} {}
+  Status write(HipPagedKvCache &c, size_t rows = positions, size_t rot = d) {
+    return c.write(0, tq, tk, tv, tqo, nullptr, nullptr, 1e-6f, (const float *)cs.p, rows, rot);
+  }
+};
+
+// Positions behind the table of angles: the operator would take them for padding.
+static void test_positions(HipBackend &be) {
+  auto made = HipPagedKvCache::create(be, config());
+  if (!made.ok()) return;
+  HipPagedKvCache &c = *made.value();
+  Step s(be, 1);
+  CHECK(c.begin_step({40, 10, 0}).ok() && s.write(c).ok() && s.write(c, 40).ok(), "40 positions of 64, and of 40");
+  CHECK(!s.write(c, 39).ok() && s.write(c, 0, 0).ok(), "40 positions of 39; without rotation there are none");
+  c.end_step();
+  CHECK(c.begin_step({24, 0, 0}).ok() && s.write(c).ok(), "the last of 64 positions");
+  c.end_step();
+  CHECK(c.begin_step({0, 1, 0}).ok() && s.write(c).ok(), "an idle request's length does not count");
+  c.end_step();
+  CHECK(c.begin_step({1, 1, 0}).ok() && !s.write(c).ok(), "position 64 of 64");
+}
+
 int main() {
   auto r = HipBackend::create(0);
   if (!r.ok()) {
@@ -52,6 +100,7 @@ int main() {
     return 77;
   }
   test_configs(*r.value());
+  test_positions(*r.value());
   if (g_fail) {
     printf("%d check(s) FAILED\n", g_fail);
     return 1;
