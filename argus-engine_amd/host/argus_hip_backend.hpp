@@ -447,7 +447,7 @@ class HipPagedKvCache {
     a.n_seqs = (int32_t)c_.max_seqs, a.n_tokens = (int32_t)tokens_, a.heads_q = (int32_t)c_.heads_q, a.heads_kv = (int32_t)c_.heads_kv;
     a.head_dim = (int32_t)c_.head_dim, a.n_pages = (int32_t)c_.n_pages, a.page_size = (int32_t)c_.page_size;
     a.table_stride = (int32_t)c_.max_pages_per_seq, a.layout = layout(), a.dtype = (int32_t)q.dtype, a.max_new = max_new_;
-    a.window = (int32_t)window, a.softcap = softcap, a.scale = scale;
+    a.window = (int32_t)std::min<size_t>(window, INT32_MAX), a.softcap = softcap, a.scale = scale;
     return be_.wrap(argus_hip_paged_attention(be_.ctx(), &a));
   }
   Status end_step() {

@@ -93,6 +93,23 @@ static void test_positions(HipBackend &be) {
   CHECK(c.begin_step({1, 1, 0}).ok() && !s.write(c).ok(), "position 64 of 64");
 }
 
+// A window beyond 32 bits is one that hides nothing.
+static void test_windows(HipBackend &be) {
+  auto made = HipPagedKvCache::create(be, config());
+  if (!made.ok()) return;
+  HipPagedKvCache &c = *made.value();
+  Step s(be, 2);
+  const size_t n = 44 * Step::hq * Step::d;
+  std::vector<float> all(n), got(n);
+  CHECK(c.begin_step({40, 4, 0}).ok() && s.write(c).ok() && c.attend(0, s.tqo, s.to).ok(), "no window");
+  be.read_buffer(all.data(), s.o.p, n * 4);
+  for (size_t window : {(size_t)64, (size_t)INT32_MAX, (size_t)1 << 31, ((size_t)1 << 32) + 5, SIZE_MAX}) {
+    CHECK(c.attend(0, s.tqo, s.to, window).ok(), "window %zu", window);
+    be.read_buffer(got.data(), s.o.p, n * 4);
+    CHECK(got == all, "window %zu hides something", window);
+  }
+}
+
 int main() {
   auto r = HipBackend::create(0);
   if (!r.ok()) {
@@ -101,6 +118,7 @@ int main() {
   }
   test_configs(*r.value());
   test_positions(*r.value());
+  test_windows(*r.value());
   if (g_fail) {
     printf("%d check(s) FAILED\n", g_fail);
     return 1;
