@@ -331,6 +331,7 @@ struct HipKvCache {
 //   write(layer, q, k, v, ...)     argus_hip_qk_norm_rope into that layer's pools
 //   attend(layer, q, out, ...)     argus_hip_paged_attention over them
 //   end_step()                     the new tokens count as cached
+//   abandon_step()                 they do not, and their pages are free again (a layer failed)
 //   release(seq)                   the request's pages are free again
 // Page numbers are handed out by the device from the list the host uploads; the host repeats the rule (pages in
 // request order from the front of the list) to know who holds what, and reads nothing back.
@@ -452,6 +453,18 @@ class HipPagedKvCache {
   }
   Status end_step() {
     for (size_t s = 0; s < c_.max_seqs && tokens_; ++s) past_len_[s] += new_len_[s];
+    tokens_ = 0;
+    return OkStatus();
+  }
+  // What the step's calls wrote stays behind the cached tokens, where no row looks and the next step writes.
+  Status abandon_step() {
+    std::vector<int32_t> back;  // in the order they were taken
+    for (size_t s = 0; s < c_.max_seqs && tokens_; ++s) {
+      const auto first = held_[s].begin() + (long)pages((size_t)past_len_[s]);
+      back.insert(back.end(), first, held_[s].end());
+      held_[s].erase(first, held_[s].end());
+    }
+    free_list_.insert(free_list_.begin(), back.begin(), back.end());
     tokens_ = 0;
     return OkStatus();
   }

@@ -110,6 +110,36 @@ static void test_windows(HipBackend &be) {
   }
 }
 
+// A step that is abandoned leaves the cache as it was: the steps around it give the same rows as in a cache
+// that never saw it.
+static void test_abandoned_steps(HipBackend &be) {
+  auto a = HipPagedKvCache::create(be, config()), b = HipPagedKvCache::create(be, config());
+  if (!a.ok() || !b.ok()) return;
+  HipPagedKvCache &plain = *a.value(), &torn = *b.value();
+  const std::vector<std::vector<int32_t>> steps = {{20, 3, 0}, {1, 30, 16}, {12, 1, 1}, {1, 1, 1}};
+  const std::vector<std::vector<int32_t>> lost = {{5, 50, 20}, {30, 0, 1}, {1, 20, 40}, {2, 2, 2}};
+  uint32_t seed = 10;
+  for (size_t i = 0; i < steps.size(); ++i) {
+    Step wrong(be, seed += 3), s(be, seed += 3);
+    const size_t pages = torn.free_pages(), cached = torn.cached(1);
+    CHECK(torn.begin_step(lost[i]).ok() && wrong.write(torn).ok(), "step to be lost");
+    CHECK(i == 3 ? torn.free_pages() == pages : torn.free_pages() < pages, "its pages");  // 35, 3 and 19 tokens fit into 3, 1 and 2
+    CHECK(!torn.attend(9, wrong.tqo, wrong.to).ok() && !torn.begin_step(steps[i]).ok() && torn.abandon_step().ok(), "abandon_step");
+    CHECK(torn.free_pages() == pages && torn.cached(1) == cached && torn.new_tokens() == 0, "nothing is left of it");
+    CHECK(torn.abandon_step().ok() && torn.free_pages() == pages, "without a step");
+    std::vector<float> out[2];
+    for (HipPagedKvCache *c : {&plain, &torn}) {
+      CHECK(c->begin_step(steps[i]).ok() && s.write(*c).ok() && c->attend(0, s.tqo, s.to).ok(), "step %zu", i);
+      std::vector<float> &o = out[c == &torn];
+      o.resize(c->new_tokens() * Step::hq * Step::d);
+      be.read_buffer(o.data(), s.o.p, o.size() * 4);
+      c->end_step();
+    }
+    CHECK(out[0] == out[1] && plain.free_pages() == torn.free_pages(), "step %zu after an abandoned one", i);
+    if (i == 1) CHECK(plain.release(1).ok() && torn.release(1).ok(), "release");
+  }
+}
+
 int main() {
   auto r = HipBackend::create(0);
   if (!r.ok()) {
@@ -119,6 +149,7 @@ int main() {
   test_configs(*r.value());
   test_positions(*r.value());
   test_windows(*r.value());
+  test_abandoned_steps(*r.value());
   if (g_fail) {
     printf("%d check(s) FAILED\n", g_fail);
     return 1;
