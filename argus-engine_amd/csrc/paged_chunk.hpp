@@ -183,7 +183,7 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
       for (int kk = 0; kk < KK; ++kk) {
         const float4_t a = *(const float4_t *)(qp + 16 * kk), b = *(const float4_t *)(qp + 16 * kk + 4);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) largest = fmaxf(largest, __builtin_fabsf(e < 4 ? a[e] : b[e - 4]));
+        for (int e = 0; e < 8; ++e) largest = larger_finite(largest, e < 4 ? a[e] : b[e - 4]);
       }
       shift = row_shift(xor32_combine(largest, [](float a, float b) { return fmaxf(a, b); }));
       if constexpr (CAP) cap_in = __builtin_ldexpf(__builtin_fabsf(p.scale) / cap, -shift);

@@ -150,6 +150,11 @@ __device__ __forceinline__ float soft_cap(float s, float cap, float inv_cap) {
 
 // F32 queries enter the products as F16 pairs, hi + lo.  A row is brought to 2^14 .. 2^15 by a power of two
 // first, which the factor of its logits takes back: so the pair holds 22 bits of it whatever its size is.
+// (An infinite element of the row stays one, and is left out of what is taken for the largest.)
+__device__ __forceinline__ float larger_finite(float largest, float x) {
+  x = __builtin_fabsf(x);
+  return x < __builtin_huge_valf() ? fmaxf(largest, x) : largest;
+}
 __device__ __forceinline__ int row_shift(float largest) {
   const int shift = 15 - __builtin_amdgcn_frexp_expf(largest);
   return shift < 100 ? shift : 100;  // the factor stays a normal number

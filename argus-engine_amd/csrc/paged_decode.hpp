@@ -143,7 +143,7 @@ __device__ __forceinline__ void decode_share(const PagedParams &p, PagedShare wo
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) largest = fmaxf(largest, __builtin_fabsf(qx[kk][e]));
+      for (int e = 0; e < 8; ++e) largest = larger_finite(largest, qx[kk][e]);
     shift = row_shift(rows_allreduce_max(largest));
   }
   const float c = __builtin_ldexpf(CAP ? p.scale : p.scale * kLog2e, -shift);  // of row r: products to logits (CAP) or exponents

@@ -11,7 +11,7 @@ SHAPES = {64: (14, 2), 128: (8, 2), 256: (4, 2)}
 
 
 def reference(q, k, v, kv_len, softcap=0.0, window=0, scale=None):
-    """(out, tolerance) of one request, q [new, Hq, d]; keys whose logit is -inf have no weight.
+    """(out, tolerance) of one request, q [new, Hq, d]; keys whose logit is -inf have no weight without a cap.
 
     Errors, u = 2^-24: a logit is d products summed in F32, scaled by rounded factors, F32 queries held as two
     F16 halves (2^-22 of the terms' size), the cap's own evaluation ~8 roundings of the cap; a weight is off by
@@ -35,7 +35,7 @@ def reference(q, k, v, kv_len, softcap=0.0, window=0, scale=None):
         with np.errstate(invalid="ignore"):
             s = qq @ kk.T * scale
         assert not np.isnan(s).any() and not (s == np.inf).any()
-        see = sees & (s != -np.inf)
+        see = sees & ((s != -np.inf) | (softcap > 0))  # a cap makes them finite
         size = np.where(see, np.abs(qq) @ np.where(np.isfinite(kk), np.abs(kk), 0).T, 0).max(1) * abs(scale)
         if softcap:
             s = softcap * np.tanh(s / softcap)
@@ -143,13 +143,14 @@ def test_rows_whose_first_tiles_are_all_minus_infinity(d, ty):
 def test_infinite_keys_anywhere(d, ty):
     """Keys of -inf logits in tiles that are taken without masks: they have no weight, and a row that sees no
     other key is zeros."""
-    for past, new in (([1100], [48]), ([0], [900]), ([2900, 350], [40, 60])):
+    for past, new in (([1100], [48]), ([0], [900]), ([2900, 350], [40, 60]), ([1500, 700], [1, 1]), ([400], [2])):
         st = levels(d + past[0] + 3, past, new, d, ty)
         for s in range(len(past)):
             n = past[s] + new[s]
             infinite(st, s, [n // 7, n // 3, n // 3 + 1, n // 2, n - 3] + list(range(n // 5, n // 5 + 150)))
         check(st, call(st), "past %r" % (past,))
-        check(st, call(st, softcap=0.0, window=600), "window past %r" % (past,), window=600)
+        check(st, call(st, window=600), "window past %r" % (past,), window=600)
+        check(st, call(st, softcap=4.0), "capped past %r" % (past,), softcap=4.0)
         for s in range(len(past)):
             infinite(st, s, range(past[s] + new[s]))
         assert (call(st)[:st["cu"][-1]] == 0).all()
@@ -225,3 +226,23 @@ def test_a_step_whose_bounds_leave_no_request_a_token():
     st = setup(1, [20, 5], [0, 0], 4, 2, 64, 16, "f16", pad_rows=4)
     assert (call(st, hints=False, min_new=8) == -9.0).all()
     assert (call(st, hints=False, min_new=8, max_new=8) == -9.0).all()
+
+
+@pytest.mark.parametrize("ty", ["f16", "f32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+def test_infinite_queries(d, ty):
+    """A row whose query holds an infinity where all its keys have one sign: all logits -inf, the row is zeros;
+    all +inf, NaN.  The size of its other channels does not matter; other rows are right (their bits may differ:
+    rows of a workgroup share the choice of steps)."""
+    for past, new in ((1100, 48), (700, 1), (900, 2), (0, 300)):
+        st = setup(d + past + 5, [past], [new], *SHAPES[d], d, 16, ty, gain=100.0)
+        put(st, 0, range(past + new), k=0.5, ch=2)
+        st["q"][:new, :, 2] = 0.0
+        ordinary = st["q"].copy()
+        st["q"][0, 0, 2], st["q"][new - 1, 1, 2] = -np.inf, np.inf
+        got = call(st)
+        assert (got[0, 0] == 0).all() and np.isnan(got[new - 1, 1]).all(), (past, new)
+        st["q"] = ordinary
+        base = call(st)
+        got[0, 0], got[new - 1, 1] = base[0, 0], base[new - 1, 1]
+        check(st, got, "beside infinite queries, past %d" % past)
