@@ -78,10 +78,10 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
   const uint32_t lane_off = my_row * row_bytes + 16 * my_col;
   const PagePool k_pool(p.k, p, kvh, D), v_pool(p.v, p, kvh, D);
   // exponents are logit * ce - m_ref (CAP: of the capped logit); a negative scale turns the queries round instead
-  float ce = CAP ? kLog2e : __builtin_fabsf(p.scale) * kLog2e;
+  float ce = CAP ? kLog2e : factor(__builtin_fabsf(p.scale) * kLog2e);
   const float q_sign = p.scale < 0.0f ? -1.0f : 1.0f;
   const float cap = p.softcap;
-  float cap_in = CAP ? __builtin_fabsf(p.scale) / p.softcap : 0.0f;  // cap * tanh(product * cap_in)
+  float cap_in = CAP ? factor(__builtin_fabsf(p.scale) / p.softcap) : 0.0f;  // cap * tanh(product * cap_in)
   // V^T operand: ds_read_b64_tr_b16 gives lane i of 16 channel ch0 + i of keys key0 .. key0 + 3 when lane s
   // addresses V[key0 + s / 4][ch0 + 4 (s % 4)]; P^T holds keys 4 hl + {0..3} and 8 + 4 hl + {0..3} of 16
   const int g16 = lane >> 4, s16 = lane & 15;
@@ -186,8 +186,8 @@ __device__ __forceinline__ void chunk_share(const PagedParams &p, PagedShare wor
         for (int e = 0; e < 8; ++e) largest = larger_finite(largest, e < 4 ? a[e] : b[e - 4]);
       }
       shift = row_shift(xor32_combine(largest, [](float a, float b) { return fmaxf(a, b); }));
-      if constexpr (CAP) cap_in = __builtin_ldexpf(__builtin_fabsf(p.scale) / cap, -shift);
-      else ce = __builtin_ldexpf(__builtin_fabsf(p.scale) * kLog2e, -shift);
+      if constexpr (CAP) cap_in = factor(__builtin_ldexpf(factor(__builtin_fabsf(p.scale) / cap), -shift));
+      else ce = factor(__builtin_ldexpf(factor(__builtin_fabsf(p.scale) * kLog2e), -shift));
       asm volatile("" : "+v"(qp));  // read again rather than held
     }
 #pragma unroll

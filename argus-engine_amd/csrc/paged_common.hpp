@@ -160,6 +160,9 @@ __device__ __forceinline__ int row_shift(float largest) {
   return shift < 100 ? shift : 100;  // the factor stays a normal number
 }
 
+// A factor of logits: where it overflows, the products it meets do so as well, but for zero, which stays zero.
+__device__ __forceinline__ float factor(float x) { return fminf(fmaxf(x, -__FLT_MAX__), __FLT_MAX__); }
+
 __device__ __forceinline__ bool not_finite(_Float16 x) { return (__builtin_bit_cast(uint16_t, x) & 0x7c00) == 0x7c00; }
 #endif
 

@@ -146,7 +146,7 @@ __device__ __forceinline__ void decode_share(const PagedParams &p, PagedShare wo
       for (int e = 0; e < 8; ++e) largest = larger_finite(largest, qx[kk][e]);
     shift = row_shift(rows_allreduce_max(largest));
   }
-  const float c = __builtin_ldexpf(CAP ? p.scale : p.scale * kLog2e, -shift);  // of row r: products to logits (CAP) or exponents
+  const float c = factor(__builtin_ldexpf(factor(CAP ? p.scale : p.scale * kLog2e), -shift));  // of row r: products to logits (CAP) or exponents
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) {
     if constexpr (F32) {

@@ -246,3 +246,19 @@ def test_infinite_queries(d, ty):
         base = call(st)
         got[0, 0], got[new - 1, 1] = base[0, 0], base[new - 1, 1]
         check(st, got, "beside infinite queries, past %d" % past)
+
+
+@pytest.mark.parametrize("ty", ["f16", "f32"])
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("size,scale,softcap", [(1.0, 3.3e38, 0.0), (1.0, 10.0, 1.2e-38), (1e38, 1e5, 0.0), (1e38, 1.0, 1e-3), (1e38, -1e5, 0.0)])
+def test_keys_of_zero_under_the_largest_factors(size, scale, softcap, d, ty):
+    """Logits of zero stay zero whatever they are multiplied by: the rows are means."""
+    if ty == "f16" and size > 60000:
+        size = 60000.0
+    for past, new in (([300], [60]), ([90], [1])):
+        st = setup(d + past[0] + 6, past, new, *SHAPES[d], d, 16, ty, gain=0.2)
+        st["q"] = (st["q"] * np.float32(size)).astype(NP[ty])
+        put(st, 0, range(past[0] + new[0]), k=0.0)
+        got = call(st, softcap, scale=scale)
+        st["q"][:new[0]] = 0.0
+        check(st, got, "scale %g cap %g" % (scale, softcap))
