@@ -3,7 +3,8 @@
 // Requests of at most 16 rows (tokens x heads of a group) take the decode form (paged_decode.hpp, bound by
 // HBM), the others the chunk form (paged_chunk.hpp, bound by the matrix cores).  A call with both runs them in
 // one launch, the decode shares first, one per compute unit, so that they and the first chunk shares overlap.
-// Against a launch of each, 46 single tokens and two chunks (14/2 heads, d 64, F32) take 71 instead of 83 us.
+// Against a launch of each, 46 single tokens and two chunks (14/2 heads, d 64, F32) took 71 instead of 83 us;
+// with the care for values outside F16's range that was added since, 74 us.
 // Dividing the resident workgroups between the two by their estimated times, and workgroups of the two in
 // turn, won as much where the estimate was right and lost up to twice that elsewhere.
 #pragma once

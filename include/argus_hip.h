@@ -749,8 +749,9 @@ int argus_hip_qk_norm_rope(argus_hip_ctx *ctx, const argus_hip_qk_norm_rope_args
  * number outside the pool where its keys lie reads some page of the pool there instead, and keys past
  * table_stride pages do not exist: its rows are not specified, no other request's are touched.
  * dtype F16: logits and sums in F32, probabilities rounded to F16 for the second product; dtype F32: q and
- * the probabilities as F16 pairs (hi + lo), so the result is that of F32 arithmetic,
- * whatever the size of the queries is.
+ * the probabilities as F16 pairs (hi + lo, 2^-22 of a value; of a probability 2^-35 of the row's largest if
+ * that is more), so the result is that of F32 arithmetic, whatever the size of the queries and the spread of
+ * the logits is.
  * max_new / max_kv: no request brings more new tokens / holds more tokens than this (0 = not known).
  * min_new: no request with any new token brings fewer (0 = not known).
  * They choose kernels; where max_new or min_new does not hold, rows may be left unwritten.  out does not
